@@ -188,9 +188,9 @@ __device__ __forceinline__ void load_up(const uint16_t *up, int rank, int64_t ro
 //     ds_read_b128, 16 consecutive rows per lane group);
 //   * partial tiles read clamped rows / columns (the key's last row, its last 8 columns) instead of guarding every load:
 //     pad, don't mask -- only the base loads and the stores are predicated;
-//   * the fold is one packed fma per two accumulators when the scale is a power of two (see below); the base tile's loads are
+//   * the fold is one fma per accumulator when the scale is a power of two (see below); the base tile's loads are
 //     issued behind the first stages and consumed at the first fold;
-//   * finite checks: base and output through a packed fma(x, 0, poison) (NaN iff some x is inf / NaN), factors (edge tiles
+//   * finite checks: base and output through an fma(x, 0, poison) (NaN iff some x is inf / NaN), factors (edge tiles
 //     only, read back from the stage) through a packed 16-bit max of the magnitudes.
 // The whole-line base loads / output stores of the fast path are non-temporal (bit 0 loads, bit 1 stores; tuning switch): touched once,
 // they should not push the factors out of the L2.  SDXL x16: 8.45 -> 8.22 ms; the 32-byte pieces of the accumulator layout, which
@@ -493,8 +493,8 @@ __device__ __forceinline__ void lora_tile_fast(const LoraParams &p, const mecha_
         }
         if (flags & CH_FOLD) {                                            // the run is complete: delta * scale, then addcmul
             // fma(round(acc * scale), weight, total) (lycoris.py:263 then linear.py:76).  With a power-of-two scale (alpha / rank
-            // usually is one) acc * scale and scale * weight are exact, so one fma gives the same bits; two per instruction
-            // (v_pk_fma_f32).  Only results below the normal range could differ, where acc * scale would round and this does not.
+            // usually is one) acc * scale and scale * weight are exact, so one fma gives the same bits.
+            // Only results below the normal range could differ, where acc * scale would round and this does not.
             if (flags & CH_ONE_STEP) {
                 const f32x2 sw = {scale * weight, scale * weight};
 #pragma unroll
@@ -718,8 +718,8 @@ __device__ __forceinline__ void lora_tile_general(const LoraParams &p, const mec
         if (now.k0 + KC >= rank) {                                        // the network is complete: delta * scale, then addcmul
             const float scale = nets[now.n].scale, weight = nets[now.n].weight;
             // fma(round(acc * scale), weight, total) (lycoris.py:263 then linear.py:76).  With a power-of-two scale (alpha / rank
-            // usually is one) acc * scale and scale * weight are exact, so one fma gives the same bits; two per instruction
-            // (v_pk_fma_f32).  Only results below the normal range could differ, where acc * scale would round and this does not.
+            // usually is one) acc * scale and scale * weight are exact, so one fma gives the same bits.
+            // Only results below the normal range could differ, where acc * scale would round and this does not.
             const uint32_t sb = __float_as_uint(scale), swb = __float_as_uint(scale * weight);
             const bool one_step = ((sb & 0x007fffffu) == 0u) && (((sb >> 23) & 0xffu) - 1u < 254u) && (((swb >> 23) & 0xffu) - 1u < 254u);
             if (one_step) {

@@ -349,7 +349,7 @@ __device__ __forceinline__ void bred_operands(const BredParams &p, int64_t e, in
             if constexpr (MODE == RM_ADDPERP) c[j] = (j < valid) ? load1<IN_DT>(p.c, e + j) : 0.0f;
         }
     }
-    // fma(v, 0, poison) stays 0 while every input is finite and turns NaN after an inf or a NaN (two values per v_pk_fma_f32)
+    // fma(v, 0, poison) stays 0 while every input is finite and turns NaN after an inf or a NaN
     f32x2 poison = {0.0f, 0.0f};
     const f32x2 zero2 = {0.0f, 0.0f};
 #pragma unroll

@@ -1077,7 +1077,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void ties_merge_kernel(TiesParams p, M
             const bool vec = p.vec_ok && valid == 8;
             const int64_t e = seg.offset + local;
             float b[8];
-            f32x2 poison = {0.0f, 0.0f};           // fma(x, 0, poison): stays 0 while every input is finite, NaN after inf / NaN (v_pk_fma_f32)
+            f32x2 poison = {0.0f, 0.0f};           // fma(x, 0, poison): stays 0 while every input is finite, NaN after inf / NaN
             bool hit = false;                      // some |delta| of this lane lies in an ambiguous bin
             // every load of this position is issued before the first one is consumed
             Raw8<W32> rb, rv[CAP];
@@ -1247,7 +1247,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void ties_merge_kernel(TiesParams p, M
 //   * the agree count needs no pass of its own: agreeing - disagreeing = |vote| and agreeing + disagreeing = kept, so
 //     count = (vote * elected + kept) / 2, kept counted by the filter's own compare (elected = 0: every selected value is a
 //     zero, the quotient is +0 or 0 * inf = NaN -> 0, like the reference's 0 / count);
-//   * subtraction, sums and the finishing fmas on two values per instruction (v_pk_add_f32 / v_pk_fma_f32).
+//   * subtraction, sums and the finishing fmas written on pairs of values.
 // E elements of 16-bit storage per lane: 8 (one 16-byte access) or 4 (one 8-byte access)
 template <int E> struct RawWords { uint32_t w[E / 2]; };
 template <int E>
