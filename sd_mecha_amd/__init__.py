@@ -3,7 +3,8 @@
 Public surface mirrors the reference for this path only: the builtin merge-method names
 (callable on tensors = the method body, callable on recipe nodes = a recipe, ``.__wrapped__`` = the body),
 ``StateDictKeyError`` / ``NonFiniteStateDictKeyError``, ``model()``, ``literal()``, ``merge()``, ``serialize()``
-and the ``@merge_method`` decorator for user-defined per-key methods.
+and the ``@merge_method`` decorator for user-defined per-key methods.  Beside it, on tensors only: 8-bit weights with a scale
+for each block of 128 (``cast_blocks``, ``uncast_blocks``, ``block_product``) and an AdamW step over an arena of keys (``adamw_step``).
 """
 import collections as _collections
 
@@ -69,5 +70,7 @@ lora_delta = merge_method(_mm.lora_delta)
 
 from .lora import convert  # noqa: E402,F401   convert(model(lora_file), base): the reference's sd_mecha.convert for kohya LoRAs
 from .merging import merge  # noqa: E402,F401
+from .blocks import BlockScaled, block_product, cast_blocks, uncast_blocks  # noqa: E402,F401   8-bit weights
+from .training import adamw_state, adamw_step  # noqa: E402,F401   one AdamW step for the keys of an arena
 
 __version__ = "0.1.0"

@@ -14,6 +14,8 @@ F32, F16, BF16 = 0, 1, 2
 FLAG_INPUT_NONFINITE = 1
 FLAG_OUTPUT_NONFINITE = 2
 MAX_MODELS = 32
+SCALE_BLOCK = 128        # MECHA_SCALE_BLOCK
+SCALE_F32, SCALE_E8M0 = 0, 1
 LORA_TILE = 128          # MECHA_LORA_TILE
 ABI_VERSION = 1
 
@@ -41,8 +43,8 @@ class MechaError(RuntimeError):
 
 _lib = None
 
-c_p, c_i, c_i64, c_f, c_d, c_sz, c_u64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
-                                          ctypes.c_double, ctypes.c_size_t, ctypes.c_uint64)
+c_p, c_i, c_i64, c_f, c_d, c_sz, c_u64, c_u32 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
+                                                 ctypes.c_double, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_uint32)
 
 # name -> (restype, argtypes); every symbol include/mecha_hip.h declares
 SIGNATURES = {
@@ -108,6 +110,14 @@ SIGNATURES = {
     "mecha_batched_ties_workspace_bytes": (c_sz, [c_i, c_i, c_i64]),
     "mecha_batched_add_difference_ties": (c_i, [c_p, c_p, c_i, c_p, c_p, c_p, c_i, c_i64, c_i, c_i, c_d, c_f, c_i,
                                                 c_p, c_p, c_sz, c_p, c_p]),
+    "mecha_cast_blocks": (c_i, [c_p, c_i64, c_i64, c_i64, c_i, c_i, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p]),
+    "mecha_uncast_blocks": (c_i, [c_p, c_i64, c_p, c_i64, c_i, c_i, c_i64, c_i64, c_p, c_i, c_p, c_p]),
+    "mecha_block_product": (c_i, [c_p, c_i64, c_p, c_i64, c_i, c_p, c_i64, c_p, c_i64, c_i, c_i, c_p, c_p, c_i64, c_i64, c_i64, c_i, c_i, c_f,
+                                  c_p, c_p]),
+    "mecha_batched_adamw": (c_i, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_i64, c_i, c_i, c_i, c_i, c_d, c_d, c_d, c_d, c_d, c_p, c_i64, c_p,
+                                  c_u32, c_p, c_p, c_p]),
+    "mecha_batched_grad_norm_workspace_bytes": (c_sz, [c_i64]),
+    "mecha_batched_grad_norm": (c_i, [c_p, c_p, c_i, c_i64, c_i, c_d, c_p, c_p, c_sz, c_p]),
 }
 
 

@@ -22,7 +22,7 @@ long long g_prof_launches[MK_COUNT];
 const char *const g_prof_names[MK_COUNT] = {
     "streaming_ew", "ties_tile_index", "ties_hist1", "ties_hist2", "ties_hist3", "ties_scan", "ties_merge",
     "reduce_partial", "reduce_finish", "reduce_apply", "reduce_fixup", "lora_mfma", "rotate_gemm_mfma", "rotate_gram_norms",
-    "ties_sample", "ties_count", "ties_resolve", "ties_fixup"};
+    "ties_sample", "ties_count", "ties_resolve", "ties_fixup", "blocks_cast", "blocks_product", "adamw"};
 thread_local ProfRecord t_current;
 }  // namespace
 

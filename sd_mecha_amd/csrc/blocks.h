@@ -1,0 +1,37 @@
+// blocks.h -- e4m3 codes and the power-of-two scale of a block of 128, shared by blocks.hip and adamw.hip.
+#pragma once
+#include "common.h"
+
+constexpr int SCALE_BLOCK = MECHA_SCALE_BLOCK;      // 128
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// The smallest e >= -127 with amax <= 448 * 2^e, from the bits of amax (finite, >= 0): 448 = 1.75 * 2^8, so e is amax's exponent
+// less 8, one more where its mantissa is over 1.75.  Zero and subnormal amax end at the clamp.
+__device__ __forceinline__ int block_exponent(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+// 2^e for -126 <= e <= 127; a block's -e is in -120..127
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 2^(byte - 127); byte 0 is 2^-127, a subnormal; byte 255 is NaN
+__device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
+    return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
+
+// four floats, |x| <= 448 or NaN, to the nearest codes (ties to even)
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+__device__ __forceinline__ void unpack_e4m3x4(uint32_t w, float *v) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+}
+
+// max over the 16 lanes that share a block of 128 (8 elements each); every lane gets it
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 16));
+    return v;
+}

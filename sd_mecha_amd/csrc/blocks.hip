@@ -1,0 +1,595 @@
+// blocks.hip -- 8-bit weights: e4m3 codes with a scale for each block of 128, made from and turned back into 16- and 32-bit keys,
+// and the product of two such matrices, fused with add_difference into a base key.
+//
+// A block-scaled matrix: codes [rows][pitch] (pitch a multiple of 128 bytes, at least the columns rounded up to 128) and scales
+// [rows or ceil(rows / 128)][ceil(cols / 128)]: a scale for 128 columns of one row, or of a 128 x 128 square.  value = code * scale.
+#include <type_traits>
+#include "blocks.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------------- cast
+// rows form, codes of the matrix as it lies: 16 lanes own a block of 128, 8 elements each; one pass over memory, the block's maximum
+// goes round the 16 lanes.  Scaling by a power of two is exact, the only rounding is the code's.
+struct CastParams {
+    const void *a;
+    int64_t rows, cols, ld;            // elements
+    uint8_t *q; int64_t q_pitch;       // bytes; q may be NULL (tile kernel)
+    uint8_t *s; int64_t s_pitch;
+    uint8_t *qt; int64_t qt_pitch;     // transposed, may be NULL
+    uint8_t *st; int64_t st_pitch;
+    uint32_t *flags;
+};
+
+// 8 elements of row `row` from column c; zeros behind the last column
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_row8(const CastParams &p, int64_t row, int64_t c, float (&v)[8]) {
+    const int64_t i = row * p.ld + c;
+    if (VEC && c + 8 <= p.cols) {
+        load8<DT>(p.a, i, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = c + j < p.cols ? load1<DT>(p.a, i + j) : 0.0f;
+    }
+}
+// largest finite magnitude of 8 values; bad: one is inf or NaN
+__device__ __forceinline__ float amax8(const float (&v)[8], bool &bad) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const bool nf = nonfinite_f32(v[j]);
+        bad |= nf;
+        m = fmaxf(m, nf ? 0.0f : fabsf(v[j]));
+    }
+    return m;
+}
+// inf and NaN become the NaN code, and take no part in the scale
+__device__ __forceinline__ float scaled(float x, float inv, bool bad) {
+    return bad && nonfinite_f32(x) ? __uint_as_float(0x7fc00000u) : x * inv;
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, int64_t n_groups, int64_t blocks_per_row) {
+    const int64_t group = (int64_t)blockIdx.x * (MECHA_BLOCK / 16) + (threadIdx.x >> 4);
+    if (group >= n_groups) return;
+    const int64_t row = n_groups < (1ll << 31) ? (int64_t)((uint32_t)group / (uint32_t)blocks_per_row) : group / blocks_per_row;
+    const int64_t kb = group - row * blocks_per_row;
+    const int l = threadIdx.x & 15;
+    const int64_t c = kb * SCALE_BLOCK + 8 * l;
+    float v[8];
+    load_row8<DT, VEC>(p, row, c, v);
+    bool bad = false;
+    const int e = block_exponent(max16(amax8(v, bad)));
+    const float inv = pow2f(-e);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = scaled(v[j], inv, bad);
+    const u32x2 w = {pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7])};
+    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = w;
+    if (l == 0) p.s[row * p.s_pitch + kb] = (uint8_t)(e + 127);
+    if (bad && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
+}
+
+// 128 x 128 squares: tile scales and / or codes of the transposed matrix.  Thread (t / 16, t % 16) holds rows 8 (t / 16) .. + 7 and
+// columns 8 (t % 16) .. + 7 in registers, so that a row's maximum stays within 16 lanes, a column's needs one round through LDS,
+// and an 8 x 8 square of codes turns over in registers; transposed codes go through 16 KiB of LDS to leave as whole 128-byte lines.
+template <int DT, bool VEC, bool TILE>
+__global__ __launch_bounds__(MECHA_BLOCK) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
+    __shared__ float col_max[16][SCALE_BLOCK + 8];
+    __shared__ u32x2 turned[SCALE_BLOCK][16];
+    const int t = threadIdx.x, tr = t >> 4, tc = t & 15;
+    const int64_t sr = blockIdx.x / squares_per_row, sc = blockIdx.x - sr * squares_per_row;
+    const int64_t row0 = sr * SCALE_BLOCK + 8 * tr, c = sc * SCALE_BLOCK + 8 * tc;
+    float v[8][8];
+    bool bad = false;
+    float rmax[8], cmax[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (row0 + i < p.rows) load_row8<DT, VEC>(p, row0 + i, c, v[i]);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        rmax[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const bool nf = nonfinite_f32(v[i][j]);
+            bad |= nf;
+            const float m = nf ? 0.0f : fabsf(v[i][j]);
+            rmax[i] = fmaxf(rmax[i], m);
+            cmax[j] = fmaxf(cmax[j], m);
+        }
+    }
+    if (bad && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
+    int re[8], ce[8];                            // exponents of this thread's rows and columns
+    if constexpr (TILE) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, rmax[i]);
+        m = max16(m);
+        if (tc == 0) col_max[0][tr] = m;
+        __syncthreads();
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) m = fmaxf(m, col_max[0][i]);
+        const int e = block_exponent(m);
+#pragma unroll
+        for (int i = 0; i < 8; i++) re[i] = ce[i] = e;
+        if (t == 0) {
+            if (p.q) p.s[sr * p.s_pitch + sc] = (uint8_t)(e + 127);
+            if (p.qt) p.st[sc * p.st_pitch + sr] = (uint8_t)(e + 127);
+        }
+    } else {
+        if (p.q) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                re[i] = block_exponent(max16(rmax[i]));
+                if (tc == 0 && row0 + i < p.rows) p.s[(row0 + i) * p.s_pitch + sc] = (uint8_t)(re[i] + 127);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) col_max[tr][8 * tc + j] = cmax[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) m = fmaxf(m, col_max[i][8 * tc + j]);
+            ce[j] = block_exponent(m);
+            if (tr == 0 && c + j < p.cols) p.st[(c + j) * p.st_pitch + sr] = (uint8_t)(ce[j] + 127);
+        }
+    }
+    if (p.q) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float inv = pow2f(-re[i]);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = scaled(v[i][j], inv, bad);
+            if (row0 + i < p.rows)
+                *reinterpret_cast<u32x2 *>(p.q + (row0 + i) * p.q_pitch + c) =
+                    u32x2{pack_e4m3x4(y[0], y[1], y[2], y[3]), pack_e4m3x4(y[4], y[5], y[6], y[7])};
+        }
+    }
+    if (p.qt) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float inv = pow2f(-ce[j]);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = scaled(v[i][j], inv, bad);
+            // slot XOR the column's group: 16 lanes (columns 8 apart, 1 KiB) write to 16 different slots
+            turned[8 * tc + j][tr ^ tc] = u32x2{pack_e4m3x4(y[0], y[1], y[2], y[3]), pack_e4m3x4(y[4], y[5], y[6], y[7])};
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int col = 16 * i + tr;
+            const u32x2 w = turned[col][tc ^ (col >> 3)];
+            const int64_t oc = sc * SCALE_BLOCK + col;
+            if (oc < p.cols) *reinterpret_cast<u32x2 *>(p.qt + oc * p.qt_pitch + sr * SCALE_BLOCK + 8 * tc) = w;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ uncast
+template <int OUT_DT, bool E8M0, bool VEC>
+__global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, int64_t q_pitch, const void *s, int64_t s_pitch, int tile,
+                                                             int64_t rows, int64_t cols, int64_t vec_per_row, void *out, uint32_t *flags) {
+    const int64_t i = (int64_t)blockIdx.x * MECHA_BLOCK + threadIdx.x;
+    if (i >= rows * vec_per_row) return;
+    const int64_t row = rows * vec_per_row < (1ll << 31) ? (int64_t)((uint32_t)i / (uint32_t)vec_per_row) : i / vec_per_row;
+    const int64_t c = 8 * (i - row * vec_per_row);
+    const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(q + row * q_pitch + c));
+    const int64_t si = (tile ? row / SCALE_BLOCK : row) * s_pitch + c / SCALE_BLOCK;
+    float scale;
+    if constexpr (E8M0) scale = e8m0_to_f32(static_cast<const uint8_t *>(s)[si]);
+    else scale = static_cast<const float *>(s)[si];
+    float v[8];
+    unpack_e4m3x4(w.x, v);
+    unpack_e4m3x4(w.y, v + 4);
+    bool bad_in = nonfinite_f32(scale), bad_out = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        bad_in |= c + j < cols && nonfinite_f32(v[j]);
+        v[j] *= scale;
+        bad_out |= c + j < cols && nonfinite_f32(v[j]);
+    }
+    if (VEC && c + 8 <= cols) store8<OUT_DT, true>(out, row * cols + c, v);
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (c + j < cols) store1<OUT_DT>(out, row * cols + c + j, v[j]);
+    }
+    if ((bad_in || bad_out) && flags) atomicOr(flags, (bad_in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+}
+
+// ------------------------------------------------------------------------------------------------------------ product
+// out[m][n] = base[m][n] + alpha * sum over the blocks kb of sa[m][kb] sb[n][kb] * (sum over the block's k of a[m][k] b[n][k]),
+// on v_mfma_scale_f32_16x16x128_f8f6f4: one instruction takes a whole block of 128 of 16 rows of each side and, with
+// power-of-two scales, the two scales of every row as well, so they cost nothing.  With float32 scales the block's sum comes out of the
+// matrix unit by itself and is added with one fma an element.  Sums are float32.
+//
+// What the 8-bit matrix instructions lose (all of them; measured with single products): the products of 8 neighbouring k are aligned to
+// the largest, and what lies under 2^-13 of it is cut off; the groups are then added in float32.  That is 1.5e-5 of a result (2-norm, normal
+// codes), 1/14 of what rounding to float16 loses and 1/110 of bfloat16's, so results of 16 bits are made this way.  A float32 result
+// would show it: there the codes are turned into bfloat16, which holds each exactly, and multiplied on v_mfma_f32_16x16x32_bf16, which
+// adds in float32 (1e-8 to 5e-8 measured) at half the rate.
+//
+// b's rows are the instruction's A operand (accumulator rows) and a's rows its B operand (accumulator columns): lane l holds 4
+// accumulators of output row m = l % 16.  b's rows are dealt to the fragments so that a lane's accumulators of 4 fragments are 16
+// CONTIGUOUS columns: row r of fragment f is column 16 (r / 4) + 4 f + r % 4 of the wave's 64.
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+struct ProductParams {
+    const uint8_t *a; int64_t a_pitch; const void *sa; int64_t sa_pitch; int a_tile;
+    const uint8_t *b; int64_t b_pitch; const void *sb; int64_t sb_pitch; int b_tile;
+    const void *base; void *out;
+    int64_t m, n, k;
+    int base_dt, out_dt;
+    float alpha;
+    uint32_t *flags;
+    int tiles_m, tiles_n;
+};
+
+// global -> LDS: lane l's 16 bytes at base + off go to dst + 16 l (dst wave-uniform).  Inline assembly because the compiler cannot tell
+// which LDS bytes the builtin form writes and would wait for all of them in front of every LDS read; the kernels wait with counted
+// s_waitcnt vmcnt themselves.  M0 is the compiler's and is put back.
+__device__ __forceinline__ void dma4(const uint8_t *base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t dst) {
+    unsigned keep;
+    const uint32_t d1 = dst + 1024u, d2 = dst + 2048u, d3 = dst + 3072u;
+    asm volatile("s_mov_b32 %0, m0\n\t"
+                 "s_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                 "s_mov_b32 m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+                 "s_mov_b32 m0, %8\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+                 "s_mov_b32 m0, %9\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(dst), "s"(d1), "s"(d2), "s"(d3) : "memory");
+}
+__device__ __forceinline__ void wait_vm0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// 16-byte slot of a row's 128 bytes in LDS, so that the 16 rows of a fragment lie in 16 different (row parity, slot) places of
+// the 256-byte bank row: a's fragments are 16 consecutive rows, b's are rows 16 (r / 4) + r % 4 (+ 4 f).
+__device__ __forceinline__ int swz_a(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int swz_b(int row) { return ((row >> 1) & 1) | ((row >> 3) & 6); }
+
+__device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
+    return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+// the first n of 16 bytes
+__device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int left = n - 4 * j;
+        w[j] = left >= 4 ? w[j] : left <= 0 ? 0u : (w[j] & ((1u << (8 * left)) - 1u));
+    }
+    return w;
+}
+
+// a block's sums from codes as bfloat16: a quarter of the lane's 32 codes an instruction
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8 codes_to_bf16(int lo, int hi) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+__device__ __forceinline__ f32x4v exact_block(i32x8 a, i32x8 b, f32x4v c) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(a[2 * q], a[2 * q + 1]), codes_to_bf16(b[2 * q], b[2 * q + 1]), c, 0, 0, 0);
+    return c;
+}
+
+template <int OUT_DT>
+__device__ __forceinline__ void store_row16(const ProductParams &p, int64_t m, int64_t n, const float (&acc)[16], bool vec) {
+    // 16 contiguous columns of one output row: base + alpha * acc
+    if (m >= p.m || n >= p.n) return;
+    const int64_t i = m * p.n + n;
+    float r[16], b[16];
+    bool bad_in = false, bad_out = false;
+    const bool whole = vec && n + 16 <= p.n;
+    if (p.base) {
+        const int dt = p.base_dt;
+        if (whole) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float t[8];
+                if (dt == MECHA_F32) load8<MECHA_F32>(p.base, i + 8 * h, t);
+                else if (dt == MECHA_F16) load8<MECHA_F16>(p.base, i + 8 * h, t);
+                else load8<MECHA_BF16>(p.base, i + 8 * h, t);
+#pragma unroll
+                for (int j = 0; j < 8; j++) b[8 * h + j] = t[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                b[j] = n + j < p.n ? (dt == MECHA_F32 ? load1<MECHA_F32>(p.base, i + j) : dt == MECHA_F16 ? load1<MECHA_F16>(p.base, i + j) : load1<MECHA_BF16>(p.base, i + j)) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) r[j] = __builtin_fmaf(acc[j], p.alpha, b[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) { b[j] = 0.0f; r[j] = acc[j] * p.alpha; }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const bool in = n + j < p.n;
+        bad_in |= in && (nonfinite_f32(b[j]) || r[j] != r[j]);
+        bad_out |= in && nonfinite_f32(r[j]);
+    }
+    if (whole) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = r[8 * h + j];
+            store8<OUT_DT>(p.out, i + 8 * h, t);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (n + j < p.n) store1<OUT_DT>(p.out, i + j, r[j]);
+    }
+    if ((bad_in || bad_out) && p.flags) atomicOr(p.flags, (bad_in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+}
+
+// Scales of a tile's 128 rows, CH words each: four blocks a word for the matrix unit, else a float a block.
+constexpr int CH = 16;
+enum : int { HW_SCALES = 0, F32_SCALES = 1, EXACT_F32 = 2, EXACT_E8M0 = 3 };   // how a kernel multiplies and what its scales are
+template <int MODE>
+__device__ __forceinline__ void fill_scales(uint32_t (*to)[128], const void *s, int64_t pitch, int tile, int64_t row0, int64_t rows, int64_t kb0, int64_t n_kb) {
+    for (int i = threadIdx.x; i < CH * 128; i += MECHA_BLOCK) {
+        const int r = i & 127, w = i >> 7;
+        int64_t row = row0 + r;
+        if (row >= rows) row = rows - 1;
+        if (tile) row /= SCALE_BLOCK;
+        uint32_t v = 0;
+        if constexpr (MODE == HW_SCALES) {
+            const uint8_t *at = static_cast<const uint8_t *>(s) + row * pitch;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t kb = kb0 + 4 * w + j;
+                if (kb < n_kb) v |= (uint32_t)at[kb] << (8 * j);
+            }
+        } else {
+            const int64_t kb = kb0 + w;
+            if (kb < n_kb) {
+                if constexpr (MODE == EXACT_E8M0) v = __float_as_uint(e8m0_to_f32(static_cast<const uint8_t *>(s)[row * pitch + kb]));
+                else v = __float_as_uint(static_cast<const float *>(s)[row * pitch + kb]);
+            }
+        }
+        to[w][r] = v;
+    }
+}
+
+// 128 x 128 outputs, 4 waves of 64 x 64; a K step is one block of 128, two stages of 32 KiB in LDS, the next one in flight while
+// this one is multiplied; two workgroups a CU.
+template <int MODE, int OUT_DT>
+__global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[2][2][128 * 128];     // [stage][a, b][row][128]
+    __shared__ __attribute__((aligned(16))) uint32_t s_a[CH][128], s_b[CH][128];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int g = lane >> 4, r = lane & 15;
+    const int tile_m = blockIdx.x % p.tiles_m, tile_n = blockIdx.x / p.tiles_m;
+    const int64_t m0 = (int64_t)tile_m * 128, n0 = (int64_t)tile_n * 128;
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int64_t n_kb = (p.k + SCALE_BLOCK - 1) / SCALE_BLOCK;
+    const int tail = (int)(p.k - (n_kb - 1) * SCALE_BLOCK);                       // k's in the last block
+
+    // DMA: piece 4 wave + i of each side = 8 rows; rows behind the last one read the last one
+    uint32_t oa[4], ob[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = 8 * (4 * wave + i) + (lane >> 3), slot = lane & 7;
+        int64_t ra = p.m - 1 - m0, rb = p.n - 1 - n0;
+        ra = row < ra ? row : ra;
+        rb = row < rb ? row : rb;
+        oa[i] = (uint32_t)(ra * p.a_pitch) + 16u * (uint32_t)(slot ^ swz_a(row));
+        ob[i] = (uint32_t)(rb * p.b_pitch) + 16u * (uint32_t)(slot ^ swz_b(row));
+    }
+    const uint8_t *ga = p.a + m0 * p.a_pitch, *gb = p.b + n0 * p.b_pitch;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte *)&stage[0][0][0]) + (uint32_t)wave * 4096u;
+    auto issue = [&](int64_t kb) {
+        const uint32_t dst = lds0 + (uint32_t)(kb & 1) * 32768u;
+        dma4(ga + kb * SCALE_BLOCK, oa[0], oa[1], oa[2], oa[3], dst);
+        dma4(gb + kb * SCALE_BLOCK, ob[0], ob[1], ob[2], ob[3], dst + 16384u);
+    };
+    f32x4v acc[4][4];                                                             // [a fragment][b fragment]
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int f = 0; f < 4; f++) acc[i][f] = f32x4v{0, 0, 0, 0};
+
+    auto step = [&](int64_t kb, bool last) {
+        const uint8_t *la = &stage[kb & 1][0][0], *lb = &stage[kb & 1][1][0];
+        i32x8 fa[4], fb[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int ra = wm + 16 * i + r, rb = wn + 16 * (r >> 2) + 4 * i + (r & 3);
+            u32x4 a0 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g) ^ swz_a(ra)));
+            u32x4 a1 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g + 1) ^ swz_a(ra)));
+            u32x4 b0 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g) ^ swz_b(rb)));
+            u32x4 b1 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g + 1) ^ swz_b(rb)));
+            if (last) {                                                           // bytes behind column k are not the matrix's
+                a0 = first_bytes(a0, tail - 32 * g); a1 = first_bytes(a1, tail - 32 * g - 16);
+                b0 = first_bytes(b0, tail - 32 * g); b1 = first_bytes(b1, tail - 32 * g - 16);
+            }
+            fa[i] = join(a0, a1);
+            fb[i] = join(b0, b1);
+        }
+        if constexpr (MODE == HW_SCALES) {
+            const int w = (int)(kb >> 2) & (CH - 1), sh = 8 * (int)(kb & 3);
+            uint32_t ka[4], kbs[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ka[i] = s_a[w][wm + 16 * i + r] >> sh;
+                kbs[i] = s_b[w][wn + 16 * (r >> 2) + 4 * i + (r & 3)] >> sh;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int f = 0; f < 4; f++)
+                    acc[i][f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i], acc[i][f], 0, 0, 0, (int)kbs[f], 0, (int)ka[i]);
+        } else {
+            const int w = (int)kb & (CH - 1);
+            float sa[4];
+            f32x4v sb[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sa[i] = __uint_as_float(s_a[w][wm + 16 * i + r]);
+                sb[i] = *reinterpret_cast<const f32x4v *>(&s_b[w][wn + 16 * g + 4 * i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    f32x4v d = {0, 0, 0, 0};
+                    if constexpr (MODE == F32_SCALES) d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i], d, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    else d = exact_block(fb[f], fa[i], d);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[e], sa[i] * sb[f][e], acc[i][f][e]);
+                }
+        }
+    };
+
+    constexpr int PER = MODE == HW_SCALES ? 4 * CH : CH;                                       // blocks whose scales are in LDS
+    if (n_kb > 0) issue(0);
+    for (int64_t kb = 0; kb < n_kb; kb++) {
+        if (kb % PER == 0) {
+            __syncthreads();                                                      // the last chunk's scales have been read
+            fill_scales<MODE>(s_a, p.sa, p.sa_pitch, p.a_tile, m0, p.m, kb, n_kb);
+            fill_scales<MODE>(s_b, p.sb, p.sb_pitch, p.b_tile, n0, p.n, kb, n_kb);
+        }
+        wait_vm0();                                                               // this wave's part of stage kb has landed
+        __syncthreads();                                                          // everyone's has, and stage kb - 1 has been read
+        if (kb + 1 < n_kb) issue(kb + 1);
+        step(kb, kb + 1 == n_kb && tail < SCALE_BLOCK);
+    }
+    const bool vec = p.n % 8 == 0 && mecha_aligned16(p.out) && (p.base == nullptr || mecha_aligned16(p.base));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float row[16];
+#pragma unroll
+        for (int f = 0; f < 4; f++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) row[4 * f + e] = acc[i][f][e];
+        store_row16<OUT_DT>(p, m0 + wm + 16 * i + r, n0 + wn + 16 * g, row, vec);
+    }
+}
+
+int check_matrix(const char *what, const void *q, int64_t rows, int64_t cols, int64_t pitch, const void *s, int64_t s_pitch) {
+    MECHA_REQUIRE(q != nullptr && s != nullptr, "%s: codes or scales are NULL", what);
+    MECHA_REQUIRE(mecha_aligned16(q), "%s: codes must be 16-byte aligned", what);
+    MECHA_REQUIRE(pitch % SCALE_BLOCK == 0 && pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK,
+                  "%s: the row pitch %lld must be a multiple of 128 and hold %lld columns rounded up to 128", what, (long long)pitch, (long long)cols);
+    MECHA_REQUIRE(s_pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, "%s: a row of scales holds %lld, %lld are needed", what, (long long)s_pitch,
+                  (long long)((cols + SCALE_BLOCK - 1) / SCALE_BLOCK));
+    return MECHA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mecha_cast_blocks(const void *a, int64_t rows, int64_t cols, int64_t row_stride, int in_dtype, int tile, void *codes, int64_t pitch,
+                      void *scales, int64_t scale_pitch, void *codes_t, int64_t pitch_t, void *scales_t, int64_t scale_pitch_t,
+                      uint32_t *flags, void *stream) {
+    MECHA_REQUIRE(rows >= 0 && cols >= 0 && mecha_valid_dtype(in_dtype), "bad matrix: %lld x %lld, dtype %d", (long long)rows, (long long)cols, in_dtype);
+    MECHA_REQUIRE(codes != nullptr || codes_t != nullptr, "neither codes nor transposed codes are asked for");
+    if (rows == 0 || cols == 0) return MECHA_OK;
+    MECHA_REQUIRE(a != nullptr && row_stride >= cols, "a is NULL or its rows overlap (stride %lld, %lld columns)", (long long)row_stride, (long long)cols);
+    if (codes) { const int st = check_matrix("codes", codes, rows, cols, pitch, scales, scale_pitch); if (st) return st; }
+    if (codes_t) { const int st = check_matrix("transposed codes", codes_t, cols, rows, pitch_t, scales_t, scale_pitch_t); if (st) return st; }
+    CastParams p{a, rows, cols, row_stride, static_cast<uint8_t *>(codes), pitch, static_cast<uint8_t *>(scales), scale_pitch,
+                 static_cast<uint8_t *>(codes_t), pitch_t, static_cast<uint8_t *>(scales_t), scale_pitch_t, flags};
+    const bool vec = mecha_aligned16(a) && (row_stride * (int64_t)mecha_dtype_size(in_dtype)) % 16 == 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t bc = (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, br = (rows + SCALE_BLOCK - 1) / SCALE_BLOCK;
+    const bool flat = codes_t == nullptr && !tile;
+    const int64_t blocks = flat ? (rows * bc + MECHA_BLOCK / 16 - 1) / (MECHA_BLOCK / 16) : br * bc;
+    MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
+    dim3 grid((unsigned)blocks), block(MECHA_BLOCK);
+    auto go = [&](auto dt, auto v) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool V = decltype(v)::value;
+        if (flat) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_rows_kernel<DT, V>), grid, block, 0, s, p, rows * bc, bc);
+        else if (tile) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, V, true>), grid, block, 0, s, p, bc);
+        else MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, V, false>), grid, block, 0, s, p, bc);
+    };
+    auto with_vec = [&](auto dt) { if (vec) go(dt, std::true_type{}); else go(dt, std::false_type{}); };
+    switch (in_dtype) {
+        case MECHA_F32: with_vec(std::integral_constant<int, MECHA_F32>{}); break;
+        case MECHA_F16: with_vec(std::integral_constant<int, MECHA_F16>{}); break;
+        default: with_vec(std::integral_constant<int, MECHA_BF16>{}); break;
+    }
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+
+int mecha_uncast_blocks(const void *codes, int64_t pitch, const void *scales, int64_t scale_pitch, int scale_dtype, int tile, int64_t rows,
+                        int64_t cols, void *out, int out_dtype, uint32_t *flags, void *stream) {
+    MECHA_REQUIRE(rows >= 0 && cols >= 0 && mecha_valid_dtype(out_dtype), "bad matrix: %lld x %lld, dtype %d", (long long)rows, (long long)cols, out_dtype);
+    MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
+    if (rows == 0 || cols == 0) return MECHA_OK;
+    MECHA_REQUIRE(out != nullptr, "out is NULL");
+    const int st = check_matrix("codes", codes, rows, cols, pitch, scales, scale_pitch);
+    if (st) return st;
+    const int64_t vec_per_row = (cols + 7) / 8, blocks = (rows * vec_per_row + MECHA_BLOCK - 1) / MECHA_BLOCK;
+    MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
+    const bool vec = mecha_aligned16(out) && (cols * (int64_t)mecha_dtype_size(out_dtype)) % 16 == 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto go = [&](auto dt, auto e8, auto v) {
+        MECHA_LAUNCH(MK_BLOCKS_CAST, (uncast_kernel<decltype(dt)::value, decltype(e8)::value, decltype(v)::value>), dim3((unsigned)blocks), dim3(MECHA_BLOCK), 0, s,
+                     static_cast<const uint8_t *>(codes), pitch, scales, scale_pitch, tile, rows, cols, vec_per_row, out, flags);
+    };
+    auto with_vec = [&](auto dt, auto e8) { if (vec) go(dt, e8, std::true_type{}); else go(dt, e8, std::false_type{}); };
+    auto with_scale = [&](auto dt) { if (scale_dtype == MECHA_SCALE_E8M0) with_vec(dt, std::true_type{}); else with_vec(dt, std::false_type{}); };
+    switch (out_dtype) {
+        case MECHA_F32: with_scale(std::integral_constant<int, MECHA_F32>{}); break;
+        case MECHA_F16: with_scale(std::integral_constant<int, MECHA_F16>{}); break;
+        default: with_scale(std::integral_constant<int, MECHA_BF16>{}); break;
+    }
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+
+int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, int64_t a_scale_pitch, int a_tile, const void *b, int64_t b_pitch,
+                        const void *b_scales, int64_t b_scale_pitch, int b_tile, int scale_dtype, const void *base, void *out, int64_t m,
+                        int64_t n, int64_t k, int base_dtype, int out_dtype, float alpha, uint32_t *flags, void *stream) {
+    MECHA_REQUIRE(m >= 0 && n >= 0 && k >= 1, "bad product: %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
+    MECHA_REQUIRE(mecha_valid_dtype(out_dtype) && (base == nullptr || mecha_valid_dtype(base_dtype)), "unknown dtype code (base %d, out %d)", base_dtype, out_dtype);
+    MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
+    if (m == 0 || n == 0) return MECHA_OK;
+    MECHA_REQUIRE(out != nullptr, "out is NULL");
+    int st = check_matrix("a", a, m, k, a_pitch, a_scales, a_scale_pitch);
+    if (st) return st;
+    st = check_matrix("b", b, n, k, b_pitch, b_scales, b_scale_pitch);
+    if (st) return st;
+    MECHA_REQUIRE(a_pitch <= (1 << 24) && b_pitch <= (1 << 24), "rows of more than 2^24 bytes (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
+    const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128;
+    MECHA_REQUIRE(tm * tn < (1ll << 24), "%lld x %lld outputs are beyond one launch", (long long)m, (long long)n);
+    ProductParams p{static_cast<const uint8_t *>(a), a_pitch, a_scales, a_scale_pitch, a_tile, static_cast<const uint8_t *>(b), b_pitch, b_scales,
+                    b_scale_pitch, b_tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
+    auto go = [&](auto mode, auto dt) {
+        MECHA_LAUNCH(MK_BLOCKS_PRODUCT, (product_kernel<decltype(mode)::value, decltype(dt)::value>), dim3((unsigned)(tm * tn)), dim3(MECHA_BLOCK), 0, s, p);
+    };
+    auto with_mode = [&](auto power, auto real, auto dt) { if (e8m0) go(power, dt); else go(real, dt); };
+    typedef std::integral_constant<int, HW_SCALES> Hw;
+    typedef std::integral_constant<int, F32_SCALES> F32;
+    switch (out_dtype) {
+        case MECHA_F32: with_mode(std::integral_constant<int, EXACT_E8M0>{}, std::integral_constant<int, EXACT_F32>{}, std::integral_constant<int, MECHA_F32>{}); break;
+        case MECHA_F16: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_F16>{}); break;
+        default: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_BF16>{}); break;
+    }
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+
+}  // extern "C"

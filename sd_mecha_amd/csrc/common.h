@@ -35,7 +35,7 @@ static inline bool mecha_isclose(double a, double b) {
     const double diff = a > b ? a - b : b - a, aa = a < 0 ? -a : a, ab = b < 0 ? -b : b;
     return diff <= 1e-9 * (aa > ab ? aa : ab);
 }
-static inline bool mecha_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static __host__ __device__ inline bool mecha_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------- per-kernel timers
 // Off by default.  When enabled (mecha_profile_enable) every launch is bracketed by HIP events on its own
@@ -43,7 +43,7 @@ static inline bool mecha_aligned16(const void *p) { return (reinterpret_cast<uin
 enum MechaKernelId : int {
     MK_STREAMING = 0, MK_TIES_INDEX, MK_TIES_HIST1, MK_TIES_HIST2, MK_TIES_HIST3, MK_TIES_SCAN, MK_TIES_MERGE,
     MK_RED_REDUCE, MK_RED_FINISH, MK_RED_APPLY, MK_RED_FIXUP, MK_LORA, MK_ROT_GEMM, MK_ROT_NORMS,
-    MK_TIES_SAMPLE, MK_TIES_COUNT, MK_TIES_RESOLVE, MK_TIES_FIXUP, MK_COUNT
+    MK_TIES_SAMPLE, MK_TIES_COUNT, MK_TIES_RESOLVE, MK_TIES_FIXUP, MK_BLOCKS_CAST, MK_BLOCKS_PRODUCT, MK_ADAMW, MK_COUNT
 };
 extern bool g_mecha_profiling;
 void mecha_prof_begin(hipStream_t s, int id);

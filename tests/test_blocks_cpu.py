@@ -1,0 +1,184 @@
+"""8-bit weights and the AdamW step without a GPU: layouts, refusals in Python and at the C entries."""
+import numpy as np
+import pytest
+import torch
+
+import blocks_reference as R
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def codes(rows, cols):
+    return torch.zeros(rows, cols).to(E4M3)
+
+
+def test_block_scaled_forms_and_layout():
+    import sd_mecha_amd as amd
+    q = amd.BlockScaled(codes(5, 100), torch.ones(5, 1))
+    assert q.pitch == 128 and q.values.stride(0) == 128 and not q.tile and q.shape == (5, 100)
+    q = amd.BlockScaled(codes(300, 256), torch.ones(3, 2).to(E8M0))
+    assert q.pitch == 256 and q.tile and q.scale_pitch == 2
+    whole = codes(4, 384)
+    q = amd.BlockScaled(whole[:, 128:256], torch.ones(4, 1))                 # a view that can stay where it is
+    assert q.values.data_ptr() == whole[:, 128:].data_ptr() and q.pitch == 384
+    q = amd.BlockScaled(whole[:, 300:384], torch.ones(4, 1))                 # not 16-byte aligned
+    assert q.pitch == 128 and q.values.data_ptr() != whole[:, 300:].data_ptr()
+    short = torch.zeros(3 * 256 + 100, dtype=torch.uint8).view(E4M3).as_strided((4, 100), (256, 1))
+    q = amd.BlockScaled(short, torch.ones(4, 1))                             # the last row's block of 128 ends behind the storage
+    assert q.values.data_ptr() != short.data_ptr() and q.pitch == 128
+    q = amd.BlockScaled(codes(256, 7).t(), torch.ones(7, 2))                 # columns next to each other in memory
+    assert q.values.stride() == (256, 1)
+    q = amd.BlockScaled(codes(1, 200), torch.ones(1, 2))
+    assert not q.tile and q.pitch == 256
+    s = torch.ones(2, 6)[:, ::3]
+    q = amd.BlockScaled(codes(2, 256), s)
+    assert q.scales.stride(1) == 1
+    for rows, cols in ((0, 128), (4, 0)):
+        assert amd.BlockScaled(codes(rows, cols), torch.ones(rows, R.blocks(cols))).shape == (rows, cols)
+
+
+def test_laying_out_keeps_the_values():
+    import sd_mecha_amd as amd
+    g = torch.Generator().manual_seed(0)
+    v = torch.randn(9, 131, generator=g).to(E4M3)
+    q = amd.BlockScaled(v, torch.rand(9, 2, generator=g))
+    assert torch.equal(q.values.view(torch.uint8), v.view(torch.uint8)) and q.pitch == 256
+
+
+@pytest.mark.parametrize("values, scales, error", [
+    (torch.zeros(4, 128), torch.ones(4, 1), TypeError),
+    (codes(4, 128), torch.ones(4, 1, dtype=torch.float64), TypeError),
+    (codes(4, 128), [1.0], TypeError),
+    (codes(4, 128), torch.ones(4), ValueError),
+    (codes(4, 128), torch.ones(4, 2), ValueError),
+    (codes(300, 128), torch.ones(2, 1), ValueError),
+    (codes(4, 128)[0], torch.ones(1, 1), ValueError),
+])
+def test_block_scaled_refusals(values, scales, error):
+    import sd_mecha_amd as amd
+    with pytest.raises(error):
+        amd.BlockScaled(values, scales)
+
+
+def test_calls_refuse_the_cpu_and_wrong_kinds():
+    import sd_mecha_amd as amd
+    q = amd.BlockScaled(codes(4, 128), torch.ones(4, 1))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        amd.cast_blocks(torch.zeros(4, 4))
+    with pytest.raises(TypeError):
+        amd.cast_blocks(torch.zeros(4, 4, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        amd.cast_blocks(torch.zeros(4, 4), sides="left")
+    with pytest.raises(amd.StateDictKeyError):
+        amd.cast_blocks({}, key="absent")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        amd.uncast_blocks(q)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        amd.block_product(q, q)
+    with pytest.raises(TypeError):
+        amd.block_product(q.values, q)
+
+
+ADAMW = dict(step=1)
+
+
+def arenas(n=256, bits=32):
+    import sd_mecha_amd as amd
+    st = amd.adamw_state(n, "cpu", bits)
+    return dict(params=torch.zeros(n), grads=torch.zeros(n), segments=torch.tensor([[0, n]]), step=1, **st)
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(), RuntimeError),                                                # all in order, but for the CPU
+    (dict(params=torch.zeros(256, dtype=torch.float64)), TypeError),
+    (dict(grads=torch.zeros(255)), ValueError),
+    (dict(exp_avg=torch.zeros(256, dtype=torch.bfloat16)), TypeError),
+    (dict(grads=torch.zeros(512)[::2]), ValueError),
+    (dict(segments=torch.zeros(1, 2, dtype=torch.int32)), ValueError),
+    (dict(segments=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(step=0), ValueError),
+    (dict(step=torch.tensor([1.0])), ValueError),
+    (dict(betas=(0.9, 1.0)), ValueError),
+    (dict(lr=-1.0), ValueError),
+    (dict(lr=float("nan")), ValueError),
+    (dict(weight_decay=torch.zeros(2)), ValueError),
+    (dict(max_norm=-1.0), ValueError),
+    (dict(max_norm=float("nan")), ValueError),
+    (dict(flags=torch.zeros(2, dtype=torch.int32)), ValueError),
+    (dict(copy=torch.zeros(255)), ValueError),
+    (dict(exp_avg_scales=torch.zeros(2, dtype=torch.uint8).view(E8M0)), TypeError),     # float32 states with a scale
+])
+def test_adamw_refusals(change, error):
+    import sd_mecha_amd as amd
+    with pytest.raises(error):
+        amd.adamw_step(**{**arenas(), **change})
+
+
+def test_adamw_8bit_refusals_and_states():
+    import sd_mecha_amd as amd
+    a = arenas(bits=8)
+    assert a["exp_avg"].dtype == E4M3 and a["exp_avg_sq_scales"].numel() == 2
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        amd.adamw_step(**a)
+    with pytest.raises(ValueError):
+        amd.adamw_state(130, "cpu", 8)
+    with pytest.raises(ValueError):
+        amd.adamw_state(128, "cpu", 16)
+    with pytest.raises(TypeError):
+        amd.adamw_step(**{**a, "exp_avg_sq_scales": None})
+    with pytest.raises(ValueError):
+        amd.adamw_step(**{**a, "exp_avg_sq_scales": a["exp_avg_sq_scales"][:1]})
+
+
+def test_c_entries_refuse_before_any_launch():
+    """Every one of these returns an error code from the host's checks, with a message; nothing is launched."""
+    from sd_mecha_amd import _lib
+    L = _lib.lib()
+    at = 4096                                                               # an address that is never read
+    cast = lambda **k: L.mecha_cast_blocks(*[k.get(n, d) for n, d in (                                         # noqa: E731
+        ("a", at), ("rows", 4), ("cols", 100), ("ld", 100), ("dt", _lib.F32), ("tile", 0), ("q", at), ("pitch", 128), ("s", at), ("sp", 1),
+        ("qt", None), ("pt", 0), ("st", None), ("spt", 0), ("flags", None), ("stream", None))])
+    for bad in (dict(rows=-1), dict(dt=7), dict(q=None), dict(ld=99), dict(pitch=100), dict(pitch=0), dict(sp=0), dict(s=None), dict(q=at + 8),
+                dict(a=None), dict(qt=at, pt=100, st=at, spt=1)):
+        assert cast(**bad) < 0 and L.mecha_last_error(), bad
+    un = lambda **k: L.mecha_uncast_blocks(*[k.get(n, d) for n, d in (                                         # noqa: E731
+        ("q", at), ("pitch", 128), ("s", at), ("sp", 1), ("sdt", 0), ("tile", 0), ("rows", 4), ("cols", 100), ("out", at), ("dt", 0), ("flags", None), ("stream", None))])
+    for bad in (dict(q=None), dict(pitch=64), dict(sdt=5), dict(dt=9), dict(out=None), dict(cols=-1)):
+        assert un(**bad) < 0, bad
+    prod = lambda **k: L.mecha_block_product(*[k.get(n, d) for n, d in (                                       # noqa: E731
+        ("a", at), ("ap", 128), ("sa", at), ("sap", 1), ("at", 0), ("b", at), ("bp", 128), ("sb", at), ("sbp", 1), ("bt", 0), ("sdt", 1),
+        ("base", None), ("out", at), ("m", 4), ("n", 4), ("k", 100), ("bdt", 0), ("odt", 0), ("alpha", 1.0), ("flags", None), ("stream", None))])
+    for bad in (dict(m=-1), dict(k=0), dict(odt=3), dict(base=at, bdt=4), dict(sdt=2), dict(out=None), dict(a=None), dict(bp=127), dict(sap=0),
+                dict(ap=1 << 25), dict(b=at + 4), dict(m=1 << 20, n=1 << 30)):
+        assert prod(**bad) < 0, bad
+    ad = lambda **k: L.mecha_batched_adamw(*[k.get(n, d) for n, d in (                                         # noqa: E731
+        ("p", at), ("g", at), ("m", at), ("v", at), ("ms", None), ("vs", None), ("copy", None), ("segs", at), ("n", 1), ("total", 256), ("pd", 0),
+        ("gd", 0), ("cd", 0), ("bits", 32), ("lr", 1e-3), ("b1", 0.9), ("b2", 0.999), ("eps", 1e-8), ("wd", 0.0), ("kwd", None), ("step", 1),
+        ("sd", None), ("seed", 0), ("clip", None), ("flags", None), ("stream", None))])
+    for bad in (dict(n=0), dict(segs=None), dict(total=-1), dict(total=1 << 36), dict(pd=5), dict(copy=at, cd=9), dict(bits=16), dict(b1=1.0),
+                dict(lr=-1.0), dict(eps=-1.0), dict(step=0), dict(p=None), dict(bits=8), dict(bits=8, ms=at, vs=at, total=130), dict(bits=8, ms=at, vs=at, m=at + 4)):
+        assert ad(**bad) < 0, bad
+    norm = lambda **k: L.mecha_batched_grad_norm(*[k.get(n, d) for n, d in (                                   # noqa: E731
+        ("g", at), ("segs", at), ("n", 1), ("total", 256), ("gd", 0), ("max", 1.0), ("out", at), ("ws", at), ("size", 1 << 20), ("stream", None))])
+    for bad in (dict(g=None), dict(out=None), dict(max=-1.0), dict(ws=None), dict(size=8), dict(gd=4), dict(n=0)):
+        assert norm(**bad) < 0, bad
+
+
+def test_reference_cast_is_the_nearest_code():
+    """The tests' own oracle: torch's conversion to e4m3 and the definition agree."""
+    rng = np.random.default_rng(3)
+    y = rng.uniform(-448, 448, 4096) * np.exp2(rng.integers(-18, 1, 4096))
+    y32 = y.astype(np.float32).astype(np.float64)
+    near = np.rint(y32 / R.spacing(y32)) * R.spacing(y32)
+    assert np.array_equal(near, torch.from_numpy(y32).float().to(E4M3).double().numpy())
+
+
+def test_reference_dither_moves_slow_means_on_average():
+    """A mean that moves by 1/100 of its codes' distance a step moves in 1/100 of the elements, step after step."""
+    n, hits = 1 << 16, []
+    for step in range(1, 9):
+        u = R.dither(n, step, 7)
+        hits.append((np.floor(8.01 + (u & np.uint64(0xFFFF)).astype(np.float64) / 65536) == 9).mean())
+        assert abs((u >> np.uint64(16)).astype(np.float64).mean() / 65536 - 0.5) < 5 * (1 / 12) ** 0.5 / n ** 0.5
+    # a share of 0.01 of n: standard deviation sqrt(0.01 * 0.99 / n), five of them
+    assert all(abs(h - 0.01) < 5 * (0.01 * 0.99 / n) ** 0.5 for h in hits)
