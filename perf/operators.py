@@ -271,7 +271,7 @@ def run(state):
     if case["op"] == "uncast":
         values, scales = state["a"]
         if own:
-            return amd.uncast_blocks(amd.BlockScaled(values, scales), out_dtype=TYPES[case["type"]])
+            return amd.uncast_blocks(amd.BlockScaled(values, scales), out_dtype=TYPES[case["type"]], check_finite=False)
         return (values.to(torch.float32) * spread(scales, *values.shape)).to(TYPES[case["type"]])
     if case["op"] == "product":
         (a, sa), (b, sb), base = state["a"], state["b"], state.get("base")
