@@ -4,9 +4,8 @@ a ROCm device, works on the current stream and has no CPU path.  No counterpart 
 32 bits (streaming.py:395-425)."""
 from __future__ import annotations
 
-import ctypes
 from contextlib import nullcontext
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import torch
 
@@ -25,73 +24,75 @@ def _blocks(n: int) -> int:
 
 def _on(device: torch.device):
     """The device a call's tensors live on, made current for its launches."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = nullcontext()
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class BlockScaled(NamedTuple("BlockScaled", [("values", torch.Tensor), ("scales", torch.Tensor)])):
+class BlockScaled:
     """A matrix in 8 bits: ``values`` float8_e4m3fn [rows, cols], ``scales`` float32 or float8_e8m0fnu (powers of two), either
     [rows, ceil(cols / 128)] -- one for 128 columns of a row -- or [ceil(rows / 128), ceil(cols / 128)] -- one for a 128 x 128
-    square.  What a value stands for is ``values.float() * its scale``.
+    square (``tile``).  What a value stands for is ``values.float() * its scale``.
 
-    The kernels read rows in whole blocks of 128 bytes: ``cast_blocks`` lays rows a multiple of 128 bytes apart, with zeros behind the
-    last column.  Values that lie otherwise (a stored tensor whose columns are no multiple of 128) are laid out so here, once."""
-    __slots__ = ()
+    The kernels read rows in whole blocks of 128 bytes: ``cast_blocks`` lays rows a multiple of 128 bytes apart (``pitch``), with zeros
+    behind the last column.  Values that lie otherwise (a stored tensor whose columns are no multiple of 128) are laid out so here, once."""
+    __slots__ = ("values", "scales", "rows", "cols", "tile", "pitch", "scale_pitch", "scale_code")
 
-    def __new__(cls, values: torch.Tensor, scales: torch.Tensor):
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor):
             raise TypeError("BlockScaled takes two tensors: values and scales")
-        if values.dtype != CODES or scales.dtype not in _SCALE_DT:
+        code = _SCALE_DT.get(scales.dtype)
+        if values.dtype is not CODES or code is None:
             raise TypeError(f"BlockScaled: values of {values.dtype} (float8_e4m3fn) and scales of {scales.dtype} (float32, float8_e8m0fnu)")
-        if values.dim() != 2 or scales.dim() != 2 or values.device != scales.device:
-            raise ValueError(f"BlockScaled: values {tuple(values.shape)} on {values.device} and scales {tuple(scales.shape)} on {scales.device} "
+        shape, s_shape = values.shape, scales.shape
+        if len(shape) != 2 or len(s_shape) != 2 or values.device != scales.device:
+            raise ValueError(f"BlockScaled: values {tuple(shape)} on {values.device} and scales {tuple(s_shape)} on {scales.device} "
                              "must be matrices on one device")
-        rows, cols = values.shape
-        if scales.shape[1] != _blocks(cols) or scales.shape[0] not in (rows, _blocks(rows)):
+        (rows, cols), (s_rows, s_cols) = shape, s_shape
+        if s_cols != _blocks(cols) or (s_rows != rows and s_rows != _blocks(rows)):
             raise ValueError(f"BlockScaled: values {rows} x {cols} take scales {rows} x {_blocks(cols)} or {_blocks(rows)} x {_blocks(cols)}, "
-                             f"got {tuple(scales.shape)}")
-        if scales.stride(1) != 1 and scales.shape[1] > 1 or scales.stride(0) < scales.shape[1] and scales.shape[0] > 1:
-            scales = scales.contiguous()
-        if rows and cols and not cls._laid_out(values):
-            whole = torch.zeros((rows, _blocks(cols) * SCALE_BLOCK), dtype=torch.uint8, device=values.device).view(CODES)
+                             f"got {tuple(s_shape)}")
+        s_pitch, s_step = scales.stride()
+        if (s_step != 1 and s_cols > 1) or (s_pitch < s_cols and s_rows > 1):
+            scales, s_pitch = scales.contiguous(), s_cols
+        width = s_cols * SCALE_BLOCK
+        pitch, step = values.stride()
+        if rows == 1:
+            pitch = width
+        if rows and cols and ((step != 1 and cols > 1) or pitch % SCALE_BLOCK or pitch < width or values.data_ptr() % 16
+                              # the last row's block of 128 has to lie inside the storage
+                              or values.storage_offset() + (rows - 1) * pitch + width > values.untyped_storage().nbytes()):
+            whole = torch.zeros((rows, width), dtype=torch.uint8, device=values.device).view(CODES)
             whole[:, :cols] = values
-            values = whole[:, :cols]
-        return super().__new__(cls, values, scales)
+            values, pitch = whole[:, :cols], width
+        self._set(values, scales, rows, cols, s_rows != rows, pitch, s_pitch if s_rows > 1 else s_cols, code)
 
-    @staticmethod
-    def _laid_out(values: torch.Tensor) -> bool:
-        """Rows in place for the kernels, and the last one's block of 128 inside the storage."""
-        (rows, cols), (pitch, step) = values.shape, values.stride()
-        width = _blocks(cols) * SCALE_BLOCK
-        if (step != 1 and cols > 1) or (rows > 1 and (pitch % SCALE_BLOCK or pitch < width)) or values.data_ptr() % 16:
-            return False
-        return values.storage_offset() + (rows - 1) * pitch + width <= values.untyped_storage().nbytes()
-
-    @property
-    def tile(self) -> bool:
-        """One scale for a 128 x 128 square (else for 128 columns of a row)."""
-        return self.scales.shape[0] != self.values.shape[0]
+    def _set(self, *of):
+        self.values, self.scales, self.rows, self.cols, self.tile, self.pitch, self.scale_pitch, self.scale_code = of
 
     @property
     def shape(self) -> torch.Size:
         return self.values.shape
 
-    @property
-    def pitch(self) -> int:
-        """Bytes from row to row."""
-        return self.values.stride(0) if self.values.shape[0] > 1 else _blocks(self.values.shape[1]) * SCALE_BLOCK
-
-    @property
-    def scale_pitch(self) -> int:
-        return self.scales.stride(0) if self.scales.shape[0] > 1 else self.scales.shape[1]
+    def __repr__(self):
+        return f"BlockScaled({self.rows} x {self.cols}, {self.scales.dtype} scales {tuple(self.scales.shape)}, {self.values.device})"
 
 
 def _empty(rows: int, cols: int, tile: bool, device) -> BlockScaled:
-    codes = torch.empty((rows, _blocks(cols) * SCALE_BLOCK), dtype=CODES, device=device)
-    return tuple.__new__(BlockScaled, (codes[:, :cols], torch.empty((_blocks(rows) if tile else rows, _blocks(cols)), dtype=torch.float8_e8m0fnu, device=device)))
+    """Room for a cast's codes and scales."""
+    s_cols = _blocks(cols)
+    width = s_cols * SCALE_BLOCK
+    codes = torch.empty((rows, width), dtype=CODES, device=device)
+    s_rows = _blocks(rows) if tile else rows
+    q = BlockScaled.__new__(BlockScaled)
+    q._set(codes if cols == width else codes[:, :cols], torch.empty((s_rows, s_cols), dtype=torch.float8_e8m0fnu, device=device), rows, cols,
+           s_rows != rows, width, s_cols, SCALE_E8M0)
+    return q
 
 
 def _check_blocks(q, what: str) -> None:
@@ -99,6 +100,14 @@ def _check_blocks(q, what: str) -> None:
         raise TypeError(f"{what} takes a BlockScaled, got {type(q).__name__}")
     if not q.values.is_cuda:
         raise RuntimeError(f"{what}: the matrix is on {q.values.device}; the MI355X backend has no CPU path")
+
+
+def _flags(device, flags, check_finite: bool):
+    """(pointer of the flag word or None, what raises for it)"""
+    if flags is None and not check_finite:
+        return None, None
+    fl = _Flags(device, flags, check_finite)
+    return fl.ptr, fl
 
 
 def cast_blocks(a, *, tile: bool = False, sides: str = "straight", key=None, flags=None, check_finite: bool = True):
@@ -118,38 +127,44 @@ def cast_blocks(a, *, tile: bool = False, sides: str = "straight", key=None, fla
         raise RuntimeError(f"cast_blocks: the key is on {a.device}; the MI355X backend has no CPU path")
     if a.dim() == 0:
         raise ValueError("cast_blocks: a 0-d key has no block")
-    a = a.unsqueeze(0) if a.dim() == 1 else a.flatten(start_dim=1)
-    rows, cols = a.shape
-    if (a.stride(1) != 1 and cols > 1) or (a.stride(0) < cols and rows > 1):
-        a = a.contiguous()
+    if a.dim() != 2:
+        a = a.unsqueeze(0) if a.dim() == 1 else a.flatten(start_dim=1)
+    (rows, cols), (stride, step) = a.shape, a.stride()
+    if (step != 1 and cols > 1) or stride < cols:
+        if rows > 1 or step != 1:
+            a = a.contiguous()
+        stride = cols
     device, tile = a.device, bool(tile)
     q = _empty(rows, cols, tile, device) if sides != "transposed" else None
     qt = _empty(cols, rows, tile, device) if sides != "straight" else None
     if rows and cols:
         with _on(device):
-            fl = _Flags(device, flags, check_finite)
+            word, fl = _flags(device, flags, check_finite)
             _lib.check(_lib.lib().mecha_cast_blocks(
-                a.data_ptr(), rows, cols, a.stride(0) if rows > 1 else cols, _DT[a.dtype], tile,
+                a.data_ptr(), rows, cols, stride, _DT[a.dtype], tile,
                 *((q.values.data_ptr(), q.pitch, q.scales.data_ptr(), q.scale_pitch) if q is not None else (None, 0, None, 0)),
                 *((qt.values.data_ptr(), qt.pitch, qt.scales.data_ptr(), qt.scale_pitch) if qt is not None else (None, 0, None, 0)),
-                fl.ptr, _stream(device)), "mecha_cast_blocks")
-            fl.finish(key)
+                word, _stream(device)), "mecha_cast_blocks")
+            if fl is not None:
+                fl.finish(key)
     return q if qt is None else qt if q is None else (q, qt)
 
 
 def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check_finite: bool = True) -> torch.Tensor:
     """``values * scales`` in float32 as a contiguous matrix of ``out_dtype`` (default float32)."""
     _check_blocks(q, "uncast_blocks")
-    device, (rows, cols) = q.values.device, q.shape
-    out = torch.empty((rows, cols), dtype=out_dtype or torch.float32, device=device)
-    if out.dtype not in _DT:
-        raise TypeError(f"uncast_blocks: unsupported out_dtype {out.dtype} (float32, float16, bfloat16)")
+    dtype = out_dtype or torch.float32
+    if dtype not in _DT:
+        raise TypeError(f"uncast_blocks: unsupported out_dtype {dtype} (float32, float16, bfloat16)")
+    device, rows, cols = q.values.device, q.rows, q.cols
+    out = torch.empty((rows, cols), dtype=dtype, device=device)
     if rows and cols:
         with _on(device):
-            fl = _Flags(device, flags, check_finite)
-            _lib.check(_lib.lib().mecha_uncast_blocks(q.values.data_ptr(), q.pitch, q.scales.data_ptr(), q.scale_pitch, _SCALE_DT[q.scales.dtype], q.tile,
-                                                      rows, cols, out.data_ptr(), _DT[out.dtype], fl.ptr, _stream(device)), "mecha_uncast_blocks")
-            fl.finish(key)
+            word, fl = _flags(device, flags, check_finite)
+            _lib.check(_lib.lib().mecha_uncast_blocks(q.values.data_ptr(), q.pitch, q.scales.data_ptr(), q.scale_pitch, q.scale_code, q.tile,
+                                                      rows, cols, out.data_ptr(), _DT[dtype], word, _stream(device)), "mecha_uncast_blocks")
+            if fl is not None:
+                fl.finish(key)
     return out
 
 
@@ -165,7 +180,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
     A NaN result or a non-finite base raises ``NonFiniteStateDictKeyError`` (``check_finite``) or sets bit 0 of ``flags``."""
     _check_blocks(a, "block_product")
     _check_blocks(b, "block_product")
-    (m, k), (n, kb), device = a.shape, b.shape, a.values.device
+    m, k, n, kb, device = a.rows, a.cols, b.rows, b.cols, a.values.device
     if k != kb or b.values.device != device:
         raise ValueError(f"block_product: a {m} x {k} on {device} and b {n} x {kb} on {b.values.device} do not go together (a @ b.T)")
     if isinstance(alpha, torch.Tensor):
@@ -180,26 +195,32 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
     else:
         shape = (m, n)
     if out is None:
+        if out_dtype is not None and out_dtype not in _DT:
+            raise TypeError(f"block_product: unsupported out_dtype {out_dtype} (float32, float16, bfloat16)")
         out = torch.empty(shape, dtype=out_dtype or torch.float32, device=device)
     elif out.device != device or out.numel() != m * n or not out.is_contiguous() or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"block_product: out must be a contiguous tensor of {m} x {n} elements on {device}, of the out_dtype if that is given")
     if out.dtype not in _DT:
         raise TypeError(f"block_product: unsupported result dtype {out.dtype} (float32, float16, bfloat16)")
-    if base is not None and out.numel() and out.dtype != base.dtype and out.untyped_storage().data_ptr() == base.untyped_storage().data_ptr():
-        raise ValueError("block_product: out may be base only with base's dtype")
+    if base is not None and (base.dtype != out.dtype or base.data_ptr() != out.data_ptr()):
+        at, to = base.data_ptr(), out.data_ptr()
+        if to < at + m * n * base.element_size() and at < to + m * n * out.element_size():
+            raise ValueError("block_product: out may be base itself, of the same dtype, but not overlap it otherwise")
     if out.numel() == 0:
         return out
     if k == 0:
         return out.zero_() if base is None else out if out is base else out.copy_(cast(base, out.dtype, key=key, flags=flags, check_finite=check_finite))
-    sa, sb = a.scales, b.scales
-    if sa.dtype != sb.dtype:
-        sa, sb = sa.to(torch.float32), sb.to(torch.float32)
+    sa, sb, code = a.scales, b.scales, a.scale_code
+    sa_pitch, sb_pitch = a.scale_pitch, b.scale_pitch
+    if code != b.scale_code:
+        sa, sb, code = sa.to(torch.float32).contiguous(), sb.to(torch.float32).contiguous(), SCALE_F32
+        sa_pitch, sb_pitch = sa.shape[1], sb.shape[1]
     with _on(device):
-        fl = _Flags(device, flags, check_finite)
+        word, fl = _flags(device, flags, check_finite)
         _lib.check(_lib.lib().mecha_block_product(
-            a.values.data_ptr(), a.pitch, sa.data_ptr(), sa.stride(0) if sa.shape[0] > 1 else sa.shape[1], a.tile,
-            b.values.data_ptr(), b.pitch, sb.data_ptr(), sb.stride(0) if sb.shape[0] > 1 else sb.shape[1], b.tile, _SCALE_DT[sa.dtype],
+            a.values.data_ptr(), a.pitch, sa.data_ptr(), sa_pitch, a.tile, b.values.data_ptr(), b.pitch, sb.data_ptr(), sb_pitch, b.tile, code,
             base.data_ptr() if base is not None else None, out.data_ptr(), m, n, k, _DT[base.dtype] if base is not None else _lib.F32,
-            _DT[out.dtype], ctypes.c_float(alpha), fl.ptr, _stream(device)), "mecha_block_product")
-        fl.finish(key)
+            _DT[out.dtype], alpha, word, _stream(device)), "mecha_block_product")
+        if fl is not None:
+            fl.finish(key)
     return out

@@ -9,45 +9,128 @@
 namespace {
 
 // ------------------------------------------------------------------------------------------------------------- cast
-// rows form, codes of the matrix as it lies: 16 lanes own a block of 128, 8 elements each; one pass over memory, the block's maximum
-// goes round the 16 lanes.  Scaling by a power of two is exact, the only rounding is the code's.
 struct CastParams {
     const void *a;
     int64_t rows, cols, ld;            // elements
-    uint8_t *q; int64_t q_pitch;       // bytes; q may be NULL (tile kernel)
+    uint8_t *q; int64_t q_pitch;       // bytes; q may be NULL (square kernel)
     uint8_t *s; int64_t s_pitch;
     uint8_t *qt; int64_t qt_pitch;     // transposed, may be NULL
     uint8_t *st; int64_t st_pitch;
     uint32_t *flags;
 };
 
+// 8 elements as they lie in memory: maxima are taken on the magnitudes' bits, two 16-bit elements an instruction, and gfx950 converts
+// two elements of any of the three types straight to codes of x / 2^e.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+template <int DT> constexpr int WORDS = DT == MECHA_F32 ? 8 : 4;
+template <int DT> struct Vec8 { uint32_t w[WORDS<DT>]; };
+template <int DT> constexpr uint32_t MAG = DT == MECHA_F32 ? 0x7fffffffu : 0x7fff7fffu;
+template <int DT> constexpr uint32_t INF = DT == MECHA_F32 ? 0x7f800000u : DT == MECHA_BF16 ? 0x7f80u : 0x7c00u;
+
 // 8 elements of row `row` from column c; zeros behind the last column
 template <int DT, bool VEC>
-__device__ __forceinline__ void load_row8(const CastParams &p, int64_t row, int64_t c, float (&v)[8]) {
+__device__ __forceinline__ Vec8<DT> load_row8(const CastParams &p, int64_t row, int64_t c) {
+    Vec8<DT> v;
     const int64_t i = row * p.ld + c;
     if (VEC && c + 8 <= p.cols) {
-        load8<DT>(p.a, i, v);
+        const u32x4 *at = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.a) + i * (DT == MECHA_F32 ? 4 : 2));
+#pragma unroll
+        for (int h = 0; h < WORDS<DT> / 4; h++) {
+            const u32x4 r = __builtin_nontemporal_load(at + h);
+            v.w[4 * h] = r.x; v.w[4 * h + 1] = r.y; v.w[4 * h + 2] = r.z; v.w[4 * h + 3] = r.w;
+        }
+    } else if constexpr (DT == MECHA_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v.w[j] = c + j < p.cols ? static_cast<const uint32_t *>(p.a)[i + j] : 0u;
     } else {
+        const uint16_t *at = static_cast<const uint16_t *>(p.a) + i;
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = c + j < p.cols ? load1<DT>(p.a, i + j) : 0.0f;
+        for (int j = 0; j < 4; j++) v.w[j] = (c + 2 * j < p.cols ? at[2 * j] : 0u) | (c + 2 * j + 1 < p.cols ? (uint32_t)at[2 * j + 1] << 16 : 0u);
     }
+    return v;
 }
-// largest finite magnitude of 8 values; bad: one is inf or NaN
-__device__ __forceinline__ float amax8(const float (&v)[8], bool &bad) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const bool nf = nonfinite_f32(v[j]);
-        bad |= nf;
-        m = fmaxf(m, nf ? 0.0f : fabsf(v[j]));
+// element by element, or both halves
+template <int DT>
+__device__ __forceinline__ uint32_t max_mag(uint32_t a, uint32_t b) {
+    if constexpr (DT == MECHA_F32) return a > b ? a : b;
+    else return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// the larger half of a word of two
+template <int DT>
+__device__ __forceinline__ uint32_t one_mag(uint32_t m) {
+    if constexpr (DT == MECHA_F32) return m;
+    else return max_mag<DT>(m, m >> 16) & 0xffffu;
+}
+// max over the 16 lanes of a row of lanes, by rotations within it
+template <int DT>
+__device__ __forceinline__ uint32_t max_mag16(uint32_t m) {
+    m = max_mag<DT>(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xf, 0xf, true));
+    m = max_mag<DT>(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xf, 0xf, true));
+    m = max_mag<DT>(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, true));
+    return max_mag<DT>(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, true));
+}
+// exponent of a block from its largest magnitude, one of DT's
+template <int DT>
+__device__ __forceinline__ int exponent_of_mag(uint32_t m) {
+    if constexpr (DT == MECHA_F32) return block_exponent(__uint_as_float(m));
+    else if constexpr (DT == MECHA_BF16) return block_exponent(__uint_as_float(m << 16));
+    else return block_exponent(f16_bits_to_f32(m));
+}
+// 2^e as the conversions take it: only the exponent's byte counts, 0 being 2^-127
+__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// codes of two elements into half `HI` of r
+template <int DT, bool HI>
+__device__ __forceinline__ s16x2 codes2(s16x2 r, uint32_t lo, uint32_t hi, float scale) {     // 16-bit types: both elements in lo
+    if constexpr (DT == MECHA_F32) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __uint_as_float(lo), __uint_as_float(hi), scale, HI);
+    else if constexpr (DT == MECHA_BF16) return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), scale, HI);
+    else return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, lo), scale, HI);
+}
+template <int DT>
+__device__ __forceinline__ u32x2 codes8(const Vec8<DT> &v, float scale) {
+    s16x2 r0 = {0, 0}, r1 = {0, 0};
+    if constexpr (DT == MECHA_F32) {
+        r0 = codes2<DT, false>(r0, v.w[0], v.w[1], scale); r0 = codes2<DT, true>(r0, v.w[2], v.w[3], scale);
+        r1 = codes2<DT, false>(r1, v.w[4], v.w[5], scale); r1 = codes2<DT, true>(r1, v.w[6], v.w[7], scale);
+    } else {
+        r0 = codes2<DT, false>(r0, v.w[0], 0, scale); r0 = codes2<DT, true>(r0, v.w[1], 0, scale);
+        r1 = codes2<DT, false>(r1, v.w[2], 0, scale); r1 = codes2<DT, true>(r1, v.w[3], 0, scale);
     }
+    return u32x2{__builtin_bit_cast(uint32_t, r0), __builtin_bit_cast(uint32_t, r1)};
+}
+template <int DT>
+__device__ __forceinline__ uint32_t mag8(const Vec8<DT> &v) {
+    uint32_t m = v.w[0] & MAG<DT>;
+#pragma unroll
+    for (int j = 1; j < WORDS<DT>; j++) m = max_mag<DT>(m, v.w[j] & MAG<DT>);
     return m;
 }
-// inf and NaN become the NaN code, and take no part in the scale
-__device__ __forceinline__ float scaled(float x, float inv, bool bad) {
-    return bad && nonfinite_f32(x) ? __uint_as_float(0x7fc00000u) : x * inv;
+// inf and NaN out of 8 elements: they become 0 and their bits are set (rare)
+template <int DT>
+__device__ __forceinline__ uint32_t take_out(Vec8<DT> &v) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t w = DT == MECHA_F32 ? v.w[j % WORDS<DT>] : (v.w[j / 2] >> (16 * (j & 1))) & 0xffffu;
+        if ((w & INF<DT>) == INF<DT>) {
+            out |= 1u << j;
+            if constexpr (DT == MECHA_F32) v.w[j] = 0u;
+            else v.w[j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
+        }
+    }
+    return out;
+}
+__device__ __forceinline__ u32x2 with_nan(u32x2 codes, uint32_t bits) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (bits & (1u << j)) codes[j / 4] = (codes[j / 4] & ~(0xffu << (8 * (j & 3)))) | (0x7fu << (8 * (j & 3)));
+    return codes;
 }
 
+// Rows form, codes of the matrix as it lies: 16 lanes own a block of 128, 8 elements each; one pass over memory, the block's
+// maximum goes round the 16 lanes.  Dividing by a power of two is exact, the only rounding is the code's.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, int64_t n_groups, int64_t blocks_per_row) {
     const int64_t group = (int64_t)blockIdx.x * (MECHA_BLOCK / 16) + (threadIdx.x >> 4);
@@ -56,65 +139,60 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
     const int64_t kb = group - row * blocks_per_row;
     const int l = threadIdx.x & 15;
     const int64_t c = kb * SCALE_BLOCK + 8 * l;
-    float v[8];
-    load_row8<DT, VEC>(p, row, c, v);
-    bool bad = false;
-    const int e = block_exponent(max16(amax8(v, bad)));
-    const float inv = pow2f(-e);
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = scaled(v[j], inv, bad);
-    const u32x2 w = {pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7])};
-    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = w;
+    Vec8<DT> v = load_row8<DT, VEC>(p, row, c);
+    uint32_t m = one_mag<DT>(mag8<DT>(v)), nan = 0;
+    if (m >= INF<DT>) {
+        nan = take_out<DT>(v);
+        m = one_mag<DT>(mag8<DT>(v));
+    }
+    const int e = exponent_of_mag<DT>(max_mag16<DT>(m));
+    u32x2 codes = codes8<DT>(v, scale_of(e));
+    if (nan) codes = with_nan(codes, nan);
+    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = codes;
     if (l == 0) p.s[row * p.s_pitch + kb] = (uint8_t)(e + 127);
-    if (bad && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
+    if (nan && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
 }
 
 // 128 x 128 squares: tile scales and / or codes of the transposed matrix.  Thread (t / 16, t % 16) holds rows 8 (t / 16) .. + 7 and
-// columns 8 (t % 16) .. + 7 in registers, so that a row's maximum stays within 16 lanes, a column's needs one round through LDS,
-// and an 8 x 8 square of codes turns over in registers; transposed codes go through 16 KiB of LDS to leave as whole 128-byte lines.
+// columns 8 (t % 16) .. + 7 in registers, so that a row's maximum stays within 16 lanes, a column's takes one exchange between the
+// waves, and an 8 x 8 square of codes turns over in registers; transposed codes go through 16 KiB of LDS to leave as whole
+// 128-byte lines.
 template <int DT, bool VEC, bool TILE>
-__global__ __launch_bounds__(MECHA_BLOCK) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
-    __shared__ float col_max[16][SCALE_BLOCK + 8];
+__global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
+    constexpr int W = WORDS<DT>;
+    __shared__ uint32_t wave_max[4][16][W];
     __shared__ u32x2 turned[SCALE_BLOCK][16];
-    const int t = threadIdx.x, tr = t >> 4, tc = t & 15;
+    const int t = threadIdx.x, tr = t >> 4, tc = t & 15, lane = t & 63, wave = t >> 6;
     const int64_t sr = blockIdx.x / squares_per_row, sc = blockIdx.x - sr * squares_per_row;
     const int64_t row0 = sr * SCALE_BLOCK + 8 * tr, c = sc * SCALE_BLOCK + 8 * tc;
-    float v[8][8];
-    bool bad = false;
-    float rmax[8], cmax[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    Vec8<DT> v[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        if (row0 + i < p.rows) load_row8<DT, VEC>(p, row0 + i, c, v[i]);
+        if (row0 + i < p.rows) v[i] = load_row8<DT, VEC>(p, row0 + i, c);
         else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
+            for (int j = 0; j < W; j++) v[i].w[j] = 0u;
         }
     }
+    uint32_t rmax[8], nan[2] = {0, 0}, all = 0;      // nan: 8 bits a row
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        rmax[i] = 0.0f;
+    for (int i = 0; i < 8; i++) { rmax[i] = mag8<DT>(v[i]); all = max_mag<DT>(all, rmax[i]); }
+    const bool bad = one_mag<DT>(all) >= INF<DT>;
+    if (bad) {
+        all = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const bool nf = nonfinite_f32(v[i][j]);
-            bad |= nf;
-            const float m = nf ? 0.0f : fabsf(v[i][j]);
-            rmax[i] = fmaxf(rmax[i], m);
-            cmax[j] = fmaxf(cmax[j], m);
-        }
+        for (int i = 0; i < 8; i++) { nan[i >> 2] |= take_out<DT>(v[i]) << (8 * (i & 3)); rmax[i] = mag8<DT>(v[i]); all = max_mag<DT>(all, rmax[i]); }
+        if (p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
     }
-    if (bad && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
     int re[8], ce[8];                            // exponents of this thread's rows and columns
     if constexpr (TILE) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, rmax[i]);
-        m = max16(m);
-        if (tc == 0) col_max[0][tr] = m;
+        uint32_t m = max_mag16<DT>(one_mag<DT>(all));
+        if (tc == 0) wave_max[wave][tr & 3][0] = m;
         __syncthreads();
-        m = 0.0f;
+        m = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) m = fmaxf(m, col_max[0][i]);
-        const int e = block_exponent(m);
+        for (int i = 0; i < 16; i++) { const uint32_t o = wave_max[i >> 2][i & 3][0]; m = m > o ? m : o; }
+        const int e = exponent_of_mag<DT>(m);
 #pragma unroll
         for (int i = 0; i < 8; i++) re[i] = ce[i] = e;
         if (t == 0) {
@@ -122,46 +200,90 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_square_kernel(CastParams p, 
             if (p.qt) p.st[sc * p.st_pitch + sr] = (uint8_t)(e + 127);
         }
     } else {
-        if (p.q) {
+        // columns: over this thread's rows, the wave's 4 row groups (lanes 16 and 32 apart), the 4 waves
+        uint32_t cmax[W];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                re[i] = block_exponent(max16(rmax[i]));
-                if (tc == 0 && row0 + i < p.rows) p.s[(row0 + i) * p.s_pitch + sc] = (uint8_t)(re[i] + 127);
-            }
+        for (int j = 0; j < W; j++) {
+            uint32_t m = v[0].w[j] & MAG<DT>;
+#pragma unroll
+            for (int i = 1; i < 8; i++) m = max_mag<DT>(m, v[i].w[j] & MAG<DT>);
+            const auto x = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+            m = max_mag<DT>(x[0], x[1]);
+            const auto y = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+            cmax[j] = max_mag<DT>(y[0], y[1]);
         }
+        if (lane < 16) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) col_max[tr][8 * tc + j] = cmax[j];
+            for (int j = 0; j < W; j++) wave_max[wave][lane][j] = cmax[j];
+        }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            float m = 0.0f;
+        for (int j = 0; j < W; j++) {
+            uint32_t m = wave_max[0][tc][j];
 #pragma unroll
-            for (int i = 0; i < 16; i++) m = fmaxf(m, col_max[i][8 * tc + j]);
-            ce[j] = block_exponent(m);
-            if (tr == 0 && c + j < p.cols) p.st[(c + j) * p.st_pitch + sr] = (uint8_t)(ce[j] + 127);
+            for (int i = 1; i < 4; i++) m = max_mag<DT>(m, wave_max[i][tc][j]);
+            if constexpr (DT == MECHA_F32) ce[j] = exponent_of_mag<DT>(m);
+            else { ce[2 * j] = exponent_of_mag<DT>(m & 0xffffu); ce[2 * j + 1] = exponent_of_mag<DT>(m >> 16); }
+        }
+        if (tr == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c + j < p.cols) p.st[(c + j) * p.st_pitch + sr] = (uint8_t)(ce[j] + 127);
+        }
+        if (p.q) {
+            if constexpr (DT == MECHA_F32) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) re[i] = exponent_of_mag<DT>(max_mag16<DT>(rmax[i]));
+            } else {                             // two rows a word go round the lanes together
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const uint32_t m = max_mag16<DT>(one_mag<DT>(rmax[i]) | one_mag<DT>(rmax[i + 1]) << 16);
+                    re[i] = exponent_of_mag<DT>(m & 0xffffu);
+                    re[i + 1] = exponent_of_mag<DT>(m >> 16);
+                }
+            }
+            if (tc == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (row0 + i < p.rows) p.s[(row0 + i) * p.s_pitch + sc] = (uint8_t)(re[i] + 127);
+            }
         }
     }
     if (p.q) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float inv = pow2f(-re[i]);
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = scaled(v[i][j], inv, bad);
-            if (row0 + i < p.rows)
-                *reinterpret_cast<u32x2 *>(p.q + (row0 + i) * p.q_pitch + c) =
-                    u32x2{pack_e4m3x4(y[0], y[1], y[2], y[3]), pack_e4m3x4(y[4], y[5], y[6], y[7])};
+            u32x2 codes = codes8<DT>(v[i], scale_of(re[i]));
+            if (bad) codes = with_nan(codes, nan[i >> 2] >> (8 * (i & 3)));
+            if (row0 + i < p.rows) *reinterpret_cast<u32x2 *>(p.q + (row0 + i) * p.q_pitch + c) = codes;
         }
     }
     if (p.qt) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float inv = pow2f(-ce[j]);
-            float y[8];
+            const float scale = scale_of(ce[j]);
+            u32x2 codes;
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = scaled(v[i][j], inv, bad);
+            for (int h = 0; h < 2; h++) {
+                s16x2 r = {0, 0};
+                const int i = 4 * h;
+                if constexpr (DT == MECHA_F32) {
+                    r = codes2<DT, false>(r, v[i].w[j], v[i + 1].w[j], scale);
+                    r = codes2<DT, true>(r, v[i + 2].w[j], v[i + 3].w[j], scale);
+                } else {                         // the column's halves of two rows
+                    const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+                    r = codes2<DT, false>(r, __builtin_amdgcn_perm(v[i + 1].w[j / 2], v[i].w[j / 2], pick), 0, scale);
+                    r = codes2<DT, true>(r, __builtin_amdgcn_perm(v[i + 3].w[j / 2], v[i + 2].w[j / 2], pick), 0, scale);
+                }
+                codes[h] = __builtin_bit_cast(uint32_t, r);
+            }
+            if (bad) {
+                uint32_t column = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) column |= ((nan[i >> 2] >> (8 * (i & 3) + j)) & 1u) << i;
+                codes = with_nan(codes, column);
+            }
             // slot XOR the column's group: 16 lanes (columns 8 apart, 1 KiB) write to 16 different slots
-            turned[8 * tc + j][tr ^ tc] = u32x2{pack_e4m3x4(y[0], y[1], y[2], y[3]), pack_e4m3x4(y[4], y[5], y[6], y[7])};
+            turned[8 * tc + j][tr ^ tc] = codes;
         }
         __syncthreads();
 #pragma unroll
@@ -272,7 +394,6 @@ __device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
 }
 
 // a block's sums from codes as bfloat16: a quarter of the lane's 32 codes an instruction
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ bf16x8 codes_to_bf16(int lo, int hi) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
