@@ -19,11 +19,6 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
     return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
 }
 
-// four floats, |x| <= 448 or NaN, to the nearest codes (ties to even)
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-}
 __device__ __forceinline__ void unpack_e4m3x4(uint32_t w, float *v) {
     const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
@@ -34,4 +29,15 @@ __device__ __forceinline__ float max16(float v) {
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 16));
     return v;
+}
+
+// the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept
+static inline int mecha_check_blocks(const char *what, const void *q, int64_t rows, int64_t cols, int64_t pitch, const void *s, int64_t s_pitch) {
+    MECHA_REQUIRE(q != nullptr && s != nullptr, "%s: codes or scales are NULL", what);
+    MECHA_REQUIRE(mecha_aligned16(q), "%s: codes must be 16-byte aligned", what);
+    MECHA_REQUIRE(pitch % SCALE_BLOCK == 0 && pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK,
+                  "%s: the row pitch %lld must be a multiple of 128 and hold %lld columns rounded up to 128", what, (long long)pitch, (long long)cols);
+    MECHA_REQUIRE(s_pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, "%s: a row of scales holds %lld, %lld are needed", what, (long long)s_pitch,
+                  (long long)((cols + SCALE_BLOCK - 1) / SCALE_BLOCK));
+    return MECHA_OK;
 }

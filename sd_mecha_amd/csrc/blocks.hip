@@ -1,5 +1,4 @@
-// blocks.hip -- 8-bit weights: e4m3 codes with a scale for each block of 128, made from and turned back into 16- and 32-bit keys,
-// and the product of two such matrices, fused with add_difference into a base key.
+// blocks.hip -- 8-bit weights: e4m3 codes with a scale for each block of 128, made from and turned back into 16- and 32-bit keys.
 //
 // A block-scaled matrix: codes [rows][pitch] (pitch a multiple of 128 bytes, at least the columns rounded up to 128) and scales
 // [rows or ceil(rows / 128)][ceil(cols / 128)]: a scale for 128 columns of one row, or of a 128 x 128 square.  value = code * scale.
@@ -328,291 +327,6 @@ __global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, i
     if ((bad_in || bad_out) && flags) atomicOr(flags, (bad_in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
 }
 
-// ------------------------------------------------------------------------------------------------------------ product
-// out[m][n] = base[m][n] + alpha * sum over the blocks kb of sa[m][kb] sb[n][kb] * (sum over the block's k of a[m][k] b[n][k]),
-// on v_mfma_scale_f32_16x16x128_f8f6f4: one instruction takes a whole block of 128 of 16 rows of each side and, with
-// power-of-two scales, the two scales of every row as well, so they cost nothing.  With float32 scales the block's sum comes out of the
-// matrix unit by itself and is added with one fma an element.  Sums are float32.
-//
-// What the 8-bit matrix instructions lose (all of them; measured with single products): the products of 8 neighbouring k are aligned to
-// the largest, and what lies under 2^-13 of it is cut off; the groups are then added in float32.  That is 1.5e-5 of a result (2-norm, normal
-// codes), 1/14 of what rounding to float16 loses and 1/110 of bfloat16's, so results of 16 bits are made this way.  A float32 result
-// would show it: there the codes are turned into bfloat16, which holds each exactly, and multiplied on v_mfma_f32_16x16x32_bf16, which
-// adds in float32 (1e-8 to 5e-8 measured) at half the rate.
-//
-// b's rows are the instruction's A operand (accumulator rows) and a's rows its B operand (accumulator columns): lane l holds 4
-// accumulators of output row m = l % 16.  b's rows are dealt to the fragments so that a lane's accumulators of 4 fragments are 16
-// CONTIGUOUS columns: row r of fragment f is column 16 (r / 4) + 4 f + r % 4 of the wave's 64.
-typedef float f32x4v __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) unsigned char lds_byte;
-
-struct ProductParams {
-    const uint8_t *a; int64_t a_pitch; const void *sa; int64_t sa_pitch; int a_tile;
-    const uint8_t *b; int64_t b_pitch; const void *sb; int64_t sb_pitch; int b_tile;
-    const void *base; void *out;
-    int64_t m, n, k;
-    int base_dt, out_dt;
-    float alpha;
-    uint32_t *flags;
-    int tiles_m, tiles_n;
-};
-
-// global -> LDS: lane l's 16 bytes at base + off go to dst + 16 l (dst wave-uniform).  Inline assembly because the compiler cannot tell
-// which LDS bytes the builtin form writes and would wait for all of them in front of every LDS read; the kernels wait with counted
-// s_waitcnt vmcnt themselves.  M0 is the compiler's and is put back.
-__device__ __forceinline__ void dma4(const uint8_t *base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t dst) {
-    unsigned keep;
-    const uint32_t d1 = dst + 1024u, d2 = dst + 2048u, d3 = dst + 3072u;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
-                 "s_mov_b32 m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
-                 "s_mov_b32 m0, %8\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
-                 "s_mov_b32 m0, %9\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(dst), "s"(d1), "s"(d2), "s"(d3) : "memory");
-}
-__device__ __forceinline__ void wait_vm0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// 16-byte slot of a row's 128 bytes in LDS, so that the 16 rows of a fragment lie in 16 different (row parity, slot) places of
-// the 256-byte bank row: a's fragments are 16 consecutive rows, b's are rows 16 (r / 4) + r % 4 (+ 4 f).
-__device__ __forceinline__ int swz_a(int row) { return (row >> 1) & 7; }
-__device__ __forceinline__ int swz_b(int row) { return ((row >> 1) & 1) | ((row >> 3) & 6); }
-
-__device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
-    return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-}
-// the first n of 16 bytes
-__device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int left = n - 4 * j;
-        w[j] = left >= 4 ? w[j] : left <= 0 ? 0u : (w[j] & ((1u << (8 * left)) - 1u));
-    }
-    return w;
-}
-
-// a block's sums from codes as bfloat16: a quarter of the lane's 32 codes an instruction
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ bf16x8 codes_to_bf16(int lo, int hi) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
-    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-__device__ __forceinline__ f32x4v exact_block(i32x8 a, i32x8 b, f32x4v c) {
-#pragma unroll
-    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(a[2 * q], a[2 * q + 1]), codes_to_bf16(b[2 * q], b[2 * q + 1]), c, 0, 0, 0);
-    return c;
-}
-
-template <int OUT_DT>
-__device__ __forceinline__ void store_row16(const ProductParams &p, int64_t m, int64_t n, const float (&acc)[16], bool vec) {
-    // 16 contiguous columns of one output row: base + alpha * acc
-    if (m >= p.m || n >= p.n) return;
-    const int64_t i = m * p.n + n;
-    float r[16], b[16];
-    bool bad_in = false, bad_out = false;
-    const bool whole = vec && n + 16 <= p.n;
-    if (p.base) {
-        const int dt = p.base_dt;
-        if (whole) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float t[8];
-                if (dt == MECHA_F32) load8<MECHA_F32>(p.base, i + 8 * h, t);
-                else if (dt == MECHA_F16) load8<MECHA_F16>(p.base, i + 8 * h, t);
-                else load8<MECHA_BF16>(p.base, i + 8 * h, t);
-#pragma unroll
-                for (int j = 0; j < 8; j++) b[8 * h + j] = t[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                b[j] = n + j < p.n ? (dt == MECHA_F32 ? load1<MECHA_F32>(p.base, i + j) : dt == MECHA_F16 ? load1<MECHA_F16>(p.base, i + j) : load1<MECHA_BF16>(p.base, i + j)) : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; j++) r[j] = __builtin_fmaf(acc[j], p.alpha, b[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) { b[j] = 0.0f; r[j] = acc[j] * p.alpha; }
-    }
-#pragma unroll
-    for (int j = 0; j < 16; j++) {
-        const bool in = n + j < p.n;
-        bad_in |= in && (nonfinite_f32(b[j]) || r[j] != r[j]);
-        bad_out |= in && nonfinite_f32(r[j]);
-    }
-    if (whole) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float t[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = r[8 * h + j];
-            store8<OUT_DT>(p.out, i + 8 * h, t);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (n + j < p.n) store1<OUT_DT>(p.out, i + j, r[j]);
-    }
-    if ((bad_in || bad_out) && p.flags) atomicOr(p.flags, (bad_in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
-}
-
-// Scales of a tile's 128 rows, CH words each: four blocks a word for the matrix unit, else a float a block.
-constexpr int CH = 16;
-enum : int { HW_SCALES = 0, F32_SCALES = 1, EXACT_F32 = 2, EXACT_E8M0 = 3 };   // how a kernel multiplies and what its scales are
-template <int MODE>
-__device__ __forceinline__ void fill_scales(uint32_t (*to)[128], const void *s, int64_t pitch, int tile, int64_t row0, int64_t rows, int64_t kb0, int64_t n_kb) {
-    for (int i = threadIdx.x; i < CH * 128; i += MECHA_BLOCK) {
-        const int r = i & 127, w = i >> 7;
-        int64_t row = row0 + r;
-        if (row >= rows) row = rows - 1;
-        if (tile) row /= SCALE_BLOCK;
-        uint32_t v = 0;
-        if constexpr (MODE == HW_SCALES) {
-            const uint8_t *at = static_cast<const uint8_t *>(s) + row * pitch;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t kb = kb0 + 4 * w + j;
-                if (kb < n_kb) v |= (uint32_t)at[kb] << (8 * j);
-            }
-        } else {
-            const int64_t kb = kb0 + w;
-            if (kb < n_kb) {
-                if constexpr (MODE == EXACT_E8M0) v = __float_as_uint(e8m0_to_f32(static_cast<const uint8_t *>(s)[row * pitch + kb]));
-                else v = __float_as_uint(static_cast<const float *>(s)[row * pitch + kb]);
-            }
-        }
-        to[w][r] = v;
-    }
-}
-
-// 128 x 128 outputs, 4 waves of 64 x 64; a K step is one block of 128, two stages of 32 KiB in LDS, the next one in flight while
-// this one is multiplied; two workgroups a CU.
-template <int MODE, int OUT_DT>
-__global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
-    __shared__ __attribute__((aligned(1024))) uint8_t stage[2][2][128 * 128];     // [stage][a, b][row][128]
-    __shared__ __attribute__((aligned(16))) uint32_t s_a[CH][128], s_b[CH][128];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int g = lane >> 4, r = lane & 15;
-    const int tile_m = blockIdx.x % p.tiles_m, tile_n = blockIdx.x / p.tiles_m;
-    const int64_t m0 = (int64_t)tile_m * 128, n0 = (int64_t)tile_n * 128;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const int64_t n_kb = (p.k + SCALE_BLOCK - 1) / SCALE_BLOCK;
-    const int tail = (int)(p.k - (n_kb - 1) * SCALE_BLOCK);                       // k's in the last block
-
-    // DMA: piece 4 wave + i of each side = 8 rows; rows behind the last one read the last one
-    uint32_t oa[4], ob[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int row = 8 * (4 * wave + i) + (lane >> 3), slot = lane & 7;
-        int64_t ra = p.m - 1 - m0, rb = p.n - 1 - n0;
-        ra = row < ra ? row : ra;
-        rb = row < rb ? row : rb;
-        oa[i] = (uint32_t)(ra * p.a_pitch) + 16u * (uint32_t)(slot ^ swz_a(row));
-        ob[i] = (uint32_t)(rb * p.b_pitch) + 16u * (uint32_t)(slot ^ swz_b(row));
-    }
-    const uint8_t *ga = p.a + m0 * p.a_pitch, *gb = p.b + n0 * p.b_pitch;
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte *)&stage[0][0][0]) + (uint32_t)wave * 4096u;
-    auto issue = [&](int64_t kb) {
-        const uint32_t dst = lds0 + (uint32_t)(kb & 1) * 32768u;
-        dma4(ga + kb * SCALE_BLOCK, oa[0], oa[1], oa[2], oa[3], dst);
-        dma4(gb + kb * SCALE_BLOCK, ob[0], ob[1], ob[2], ob[3], dst + 16384u);
-    };
-    f32x4v acc[4][4];                                                             // [a fragment][b fragment]
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int f = 0; f < 4; f++) acc[i][f] = f32x4v{0, 0, 0, 0};
-
-    auto step = [&](int64_t kb, bool last) {
-        const uint8_t *la = &stage[kb & 1][0][0], *lb = &stage[kb & 1][1][0];
-        i32x8 fa[4], fb[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int ra = wm + 16 * i + r, rb = wn + 16 * (r >> 2) + 4 * i + (r & 3);
-            u32x4 a0 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g) ^ swz_a(ra)));
-            u32x4 a1 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g + 1) ^ swz_a(ra)));
-            u32x4 b0 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g) ^ swz_b(rb)));
-            u32x4 b1 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g + 1) ^ swz_b(rb)));
-            if (last) {                                                           // bytes behind column k are not the matrix's
-                a0 = first_bytes(a0, tail - 32 * g); a1 = first_bytes(a1, tail - 32 * g - 16);
-                b0 = first_bytes(b0, tail - 32 * g); b1 = first_bytes(b1, tail - 32 * g - 16);
-            }
-            fa[i] = join(a0, a1);
-            fb[i] = join(b0, b1);
-        }
-        if constexpr (MODE == HW_SCALES) {
-            const int w = (int)(kb >> 2) & (CH - 1), sh = 8 * (int)(kb & 3);
-            uint32_t ka[4], kbs[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                ka[i] = s_a[w][wm + 16 * i + r] >> sh;
-                kbs[i] = s_b[w][wn + 16 * (r >> 2) + 4 * i + (r & 3)] >> sh;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int f = 0; f < 4; f++)
-                    acc[i][f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i], acc[i][f], 0, 0, 0, (int)kbs[f], 0, (int)ka[i]);
-        } else {
-            const int w = (int)kb & (CH - 1);
-            float sa[4];
-            f32x4v sb[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                sa[i] = __uint_as_float(s_a[w][wm + 16 * i + r]);
-                sb[i] = *reinterpret_cast<const f32x4v *>(&s_b[w][wn + 16 * g + 4 * i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int f = 0; f < 4; f++) {
-                    f32x4v d = {0, 0, 0, 0};
-                    if constexpr (MODE == F32_SCALES) d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i], d, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-                    else d = exact_block(fb[f], fa[i], d);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[e], sa[i] * sb[f][e], acc[i][f][e]);
-                }
-        }
-    };
-
-    constexpr int PER = MODE == HW_SCALES ? 4 * CH : CH;                                       // blocks whose scales are in LDS
-    if (n_kb > 0) issue(0);
-    for (int64_t kb = 0; kb < n_kb; kb++) {
-        if (kb % PER == 0) {
-            __syncthreads();                                                      // the last chunk's scales have been read
-            fill_scales<MODE>(s_a, p.sa, p.sa_pitch, p.a_tile, m0, p.m, kb, n_kb);
-            fill_scales<MODE>(s_b, p.sb, p.sb_pitch, p.b_tile, n0, p.n, kb, n_kb);
-        }
-        wait_vm0();                                                               // this wave's part of stage kb has landed
-        __syncthreads();                                                          // everyone's has, and stage kb - 1 has been read
-        if (kb + 1 < n_kb) issue(kb + 1);
-        step(kb, kb + 1 == n_kb && tail < SCALE_BLOCK);
-    }
-    const bool vec = p.n % 8 == 0 && mecha_aligned16(p.out) && (p.base == nullptr || mecha_aligned16(p.base));
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float row[16];
-#pragma unroll
-        for (int f = 0; f < 4; f++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) row[4 * f + e] = acc[i][f][e];
-        store_row16<OUT_DT>(p, m0 + wm + 16 * i + r, n0 + wn + 16 * g, row, vec);
-    }
-}
-
-int check_matrix(const char *what, const void *q, int64_t rows, int64_t cols, int64_t pitch, const void *s, int64_t s_pitch) {
-    MECHA_REQUIRE(q != nullptr && s != nullptr, "%s: codes or scales are NULL", what);
-    MECHA_REQUIRE(mecha_aligned16(q), "%s: codes must be 16-byte aligned", what);
-    MECHA_REQUIRE(pitch % SCALE_BLOCK == 0 && pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK,
-                  "%s: the row pitch %lld must be a multiple of 128 and hold %lld columns rounded up to 128", what, (long long)pitch, (long long)cols);
-    MECHA_REQUIRE(s_pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, "%s: a row of scales holds %lld, %lld are needed", what, (long long)s_pitch,
-                  (long long)((cols + SCALE_BLOCK - 1) / SCALE_BLOCK));
-    return MECHA_OK;
-}
-
 }  // namespace
 
 extern "C" {
@@ -624,8 +338,8 @@ int mecha_cast_blocks(const void *a, int64_t rows, int64_t cols, int64_t row_str
     MECHA_REQUIRE(codes != nullptr || codes_t != nullptr, "neither codes nor transposed codes are asked for");
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(a != nullptr && row_stride >= cols, "a is NULL or its rows overlap (stride %lld, %lld columns)", (long long)row_stride, (long long)cols);
-    if (codes) { const int st = check_matrix("codes", codes, rows, cols, pitch, scales, scale_pitch); if (st) return st; }
-    if (codes_t) { const int st = check_matrix("transposed codes", codes_t, cols, rows, pitch_t, scales_t, scale_pitch_t); if (st) return st; }
+    if (codes) { const int st = mecha_check_blocks("codes", codes, rows, cols, pitch, scales, scale_pitch); if (st) return st; }
+    if (codes_t) { const int st = mecha_check_blocks("transposed codes", codes_t, cols, rows, pitch_t, scales_t, scale_pitch_t); if (st) return st; }
     CastParams p{a, rows, cols, row_stride, static_cast<uint8_t *>(codes), pitch, static_cast<uint8_t *>(scales), scale_pitch,
                  static_cast<uint8_t *>(codes_t), pitch_t, static_cast<uint8_t *>(scales_t), scale_pitch_t, flags};
     const bool vec = mecha_aligned16(a) && (row_stride * (int64_t)mecha_dtype_size(in_dtype)) % 16 == 0;
@@ -658,7 +372,7 @@ int mecha_uncast_blocks(const void *codes, int64_t pitch, const void *scales, in
     MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(out != nullptr, "out is NULL");
-    const int st = check_matrix("codes", codes, rows, cols, pitch, scales, scale_pitch);
+    const int st = mecha_check_blocks("codes", codes, rows, cols, pitch, scales, scale_pitch);
     if (st) return st;
     const int64_t vec_per_row = (cols + 7) / 8, blocks = (rows * vec_per_row + MECHA_BLOCK - 1) / MECHA_BLOCK;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
@@ -674,40 +388,6 @@ int mecha_uncast_blocks(const void *codes, int64_t pitch, const void *scales, in
         case MECHA_F32: with_scale(std::integral_constant<int, MECHA_F32>{}); break;
         case MECHA_F16: with_scale(std::integral_constant<int, MECHA_F16>{}); break;
         default: with_scale(std::integral_constant<int, MECHA_BF16>{}); break;
-    }
-    MECHA_CHECK_HIP(hipGetLastError());
-    return MECHA_OK;
-}
-
-int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, int64_t a_scale_pitch, int a_tile, const void *b, int64_t b_pitch,
-                        const void *b_scales, int64_t b_scale_pitch, int b_tile, int scale_dtype, const void *base, void *out, int64_t m,
-                        int64_t n, int64_t k, int base_dtype, int out_dtype, float alpha, uint32_t *flags, void *stream) {
-    MECHA_REQUIRE(m >= 0 && n >= 0 && k >= 1, "bad product: %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
-    MECHA_REQUIRE(mecha_valid_dtype(out_dtype) && (base == nullptr || mecha_valid_dtype(base_dtype)), "unknown dtype code (base %d, out %d)", base_dtype, out_dtype);
-    MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
-    if (m == 0 || n == 0) return MECHA_OK;
-    MECHA_REQUIRE(out != nullptr, "out is NULL");
-    int st = check_matrix("a", a, m, k, a_pitch, a_scales, a_scale_pitch);
-    if (st) return st;
-    st = check_matrix("b", b, n, k, b_pitch, b_scales, b_scale_pitch);
-    if (st) return st;
-    MECHA_REQUIRE(a_pitch <= (1 << 24) && b_pitch <= (1 << 24), "rows of more than 2^24 bytes (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
-    const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128;
-    MECHA_REQUIRE(tm * tn < (1ll << 24), "%lld x %lld outputs are beyond one launch", (long long)m, (long long)n);
-    ProductParams p{static_cast<const uint8_t *>(a), a_pitch, a_scales, a_scale_pitch, a_tile, static_cast<const uint8_t *>(b), b_pitch, b_scales,
-                    b_scale_pitch, b_tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
-    auto go = [&](auto mode, auto dt) {
-        MECHA_LAUNCH(MK_BLOCKS_PRODUCT, (product_kernel<decltype(mode)::value, decltype(dt)::value>), dim3((unsigned)(tm * tn)), dim3(MECHA_BLOCK), 0, s, p);
-    };
-    auto with_mode = [&](auto power, auto real, auto dt) { if (e8m0) go(power, dt); else go(real, dt); };
-    typedef std::integral_constant<int, HW_SCALES> Hw;
-    typedef std::integral_constant<int, F32_SCALES> F32;
-    switch (out_dtype) {
-        case MECHA_F32: with_mode(std::integral_constant<int, EXACT_E8M0>{}, std::integral_constant<int, EXACT_F32>{}, std::integral_constant<int, MECHA_F32>{}); break;
-        case MECHA_F16: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_F16>{}); break;
-        default: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_BF16>{}); break;
     }
     MECHA_CHECK_HIP(hipGetLastError());
     return MECHA_OK;

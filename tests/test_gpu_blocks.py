@@ -198,6 +198,47 @@ def test_product(m, n, k, scales, dtype):
     check_product(out, a, b, base, -2.0)
 
 
+LARGE = [(2100, 2056, 1100), (2049, 2048, 2300), (5000, 4200, 640), (300, 16392, 513), (16500, 264, 4097)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", LARGE)
+def test_product_large(m, n, k, scales, dtype):
+    """Many tiles, several to a workgroup, ragged in every direction, more blocks of k than scales are held at a time."""
+    import sd_mecha_amd as amd
+    for fa, fb in (("rows", "tile"), ("tile", "rows")):
+        a, b = matrix(m, k, fa, scales, m + 1, ints=True), matrix(n, k, fb, scales, n + 2, ints=True)
+        want = torch.from_numpy(R.values(a)).cuda() @ torch.from_numpy(R.values(b)).cuda().t()
+        got = amd.block_product(a, b, alpha=2.0 ** -7, out_dtype=dtype)
+        assert torch.equal(got, (want * 2.0 ** -7).float().to(dtype)), (fa, fb)
+        base = torch.randint(-64, 64, (m, n), device="cuda").to(dtype)
+        want = (want + base.double()).float().to(dtype)
+        assert torch.equal(amd.block_product(a, b, base, out_dtype=dtype), want), (fa, fb)
+        assert torch.equal(amd.block_product(a, b, base, out=base), want), (fa, fb)
+    a, b = matrix(m, k, "rows", scales, m + 3), matrix(n, k, "tile", scales, n + 4)
+    a = amd.BlockScaled(a.values, (a.scales.float() / 2.0 ** 17).to(a.scales.dtype))
+    check_product(amd.block_product(a, b, out_dtype=dtype), a, b)
+    v = a.values.clone()
+    v.view(torch.uint8)[m - 1, k - 1] = 0x7F
+    with pytest.raises(amd.NonFiniteStateDictKeyError):
+        amd.block_product(amd.BlockScaled(v, a.scales), b, out_dtype=dtype)
+
+
+def test_product_extreme_scales():
+    """Powers of two from 2^-127 on one side against large ones on the other."""
+    import sd_mecha_amd as amd
+    for m, n, k in ((40, 50, 300), (2100, 2056, 1100)):
+        for ea, eb in ((0, 220), (3, 250), (20, 235), (127, 1)):
+            a, b = matrix(m, k, "rows", "e8m0", 1, ints=True), matrix(n, k, "tile", "e8m0", 2, ints=True)
+            a = amd.BlockScaled(a.values, torch.full_like(a.scales.view(torch.uint8), ea).view(E8M0))
+            b = amd.BlockScaled(b.values, torch.full_like(b.scales.view(torch.uint8), eb).view(E8M0))
+            for dtype in (torch.float32, torch.bfloat16):
+                va, vb = torch.from_numpy(a.values.float().cpu().double().numpy()).cuda(), torch.from_numpy(b.values.float().cpu().double().numpy()).cuda()
+                want = va @ vb.t() * 2.0 ** (ea + eb - 254)
+                assert torch.equal(amd.block_product(a, b, out_dtype=dtype), want.float().to(dtype)), (m, ea, eb, dtype)
+
+
 def test_product_mixed_scales_base_types_and_shapes():
     import sd_mecha_amd as amd
     a, b = matrix(70, 200, "rows", "e8m0", 1), matrix(90, 200, "tile", "fp32", 2)
