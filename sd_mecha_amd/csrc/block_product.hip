@@ -17,8 +17,9 @@ namespace {
 // adds in float32 (1e-8 to 5e-8 measured) at half the rate.
 //
 // b's rows are the instruction's A operand (accumulator rows) and a's rows its B operand (accumulator columns): lane l holds 4
-// accumulators of output row m = l % 16.  b's rows are dealt to the fragments so that a lane's accumulators of 4 fragments are 16
-// CONTIGUOUS columns: row r of fragment f is column 16 (r / 4) + 4 f + r % 4 of the wave's 64.
+// accumulators of output row m = l % 16.  b's rows are dealt to the fragments so that a lane's accumulators of 2 fragments are 8
+// CONTIGUOUS columns and the 4 lanes of an output row write 64 bytes (16-bit results) side by side: row r of fragment f is column
+// 32 (f / 2) + 8 (r / 4) + 4 (f % 2) + r % 4 of the wave's 64.
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -51,10 +52,14 @@ __device__ __forceinline__ void dma4(const uint8_t *base, uint32_t o0, uint32_t 
 }
 __device__ __forceinline__ void wait_vm0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// 16-byte slot of a row's 128 bytes in LDS, so that the 16 rows of a fragment lie in 16 different (row parity, slot) places of
-// the 256-byte bank row: a's fragments are 16 consecutive rows, b's are rows 16 (r / 4) + r % 4 (+ 4 f).
+// 16-byte slot of a row's 128 bytes in LDS.  A fragment's lane (g, r) = (l / 16, l % 16) reads parts g and g + 4 of row r -- any dealing of k
+// to the lanes does, if both sides have the same.  Row r's part c lies in slot c ^ (r / 2): measured, the four parts g side by side and 8
+// different slots for the rows of one parity make a 1-KiB read take 4 cycles; parts 2 g and 2 g + 1 instead, 8.
+// a's fragments are 16 consecutive rows; b's are rows 8 (r / 4) + r % 4 (+ 4, + 32) and get the same slots for the same r.
 __device__ __forceinline__ int swz_a(int row) { return (row >> 1) & 7; }
-__device__ __forceinline__ int swz_b(int row) { return ((row >> 1) & 1) | ((row >> 3) & 6); }
+__device__ __forceinline__ int swz_b(int row) { return ((row >> 1) & 1) | ((row >> 2) & 6); }
+// first row of b's fragment f, and of lane r's 8 columns, in a wave's 64
+__device__ __forceinline__ constexpr int b_row(int f) { return 32 * (f >> 1) + 4 * (f & 1); }
 
 __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
     return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
@@ -72,9 +77,9 @@ __device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
 // a block's sums from codes as bfloat16: a quarter of the lane's 32 codes an instruction
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ bf16x8 codes_to_bf16(int lo, int hi) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+__device__ __forceinline__ bf16x8 codes_to_bf16(int lo, int hi, float scale = 1.0f) {       // scale: a power of two
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
     return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 __device__ __forceinline__ f32x4v exact_block(i32x8 a, i32x8 b, f32x4v c) {
@@ -83,64 +88,45 @@ __device__ __forceinline__ f32x4v exact_block(i32x8 a, i32x8 b, f32x4v c) {
     return c;
 }
 
-// 16 contiguous columns of one output row: base + alpha * acc.  Finite checks: fma(x, 0, poison) stays 0 while every x is finite.
+// 8 contiguous columns of one output row, of any base and alignment: base + alpha * acc.  Finite checks: fma(x, 0, poison) stays 0
+// while every x is finite.
 template <int OUT_DT>
-__device__ __forceinline__ void store_row16(const ProductParams &p, int64_t m, int64_t n, const float (&acc)[16], bool vec) {
+__device__ __forceinline__ void store_any8(const ProductParams &p, int64_t m, int64_t n, const float (&acc)[8], bool vec) {
     if (m >= p.m || n >= p.n) return;
     const int64_t i = m * p.n + n;
-    const bool whole = vec && n + 16 <= p.n;
-    float r[16], poison_in = 0.0f, poison_out = 0.0f;
+    float r[8], b[8], poison_in = 0.0f, poison_out = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) b[j] = 0.0f;
     if (p.base) {
         const int dt = p.base_dt;
-        float b[16];
-        if (whole) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float t[8];
-                if (dt == MECHA_F32) load8<MECHA_F32>(p.base, i + 8 * h, t);
-                else if (dt == MECHA_F16) load8<MECHA_F16>(p.base, i + 8 * h, t);
-                else load8<MECHA_BF16>(p.base, i + 8 * h, t);
-#pragma unroll
-                for (int j = 0; j < 8; j++) b[8 * h + j] = t[j];
-            }
+        if (vec) {
+            if (dt == MECHA_F32) load8<MECHA_F32>(p.base, i, b);
+            else if (dt == MECHA_F16) load8<MECHA_F16>(p.base, i, b);
+            else load8<MECHA_BF16>(p.base, i, b);
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                b[j] = n + j < p.n ? (dt == MECHA_F32 ? load1<MECHA_F32>(p.base, i + j) : dt == MECHA_F16 ? load1<MECHA_F16>(p.base, i + j) : load1<MECHA_BF16>(p.base, i + j)) : 0.0f;
+            for (int j = 0; j < 8; j++)
+                if (n + j < p.n) b[j] = dt == MECHA_F32 ? load1<MECHA_F32>(p.base, i + j) : dt == MECHA_F16 ? load1<MECHA_F16>(p.base, i + j) : load1<MECHA_BF16>(p.base, i + j);
         }
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            if (p.flags) poison_in = __builtin_fmaf(b[j], 0.0f, poison_in);
-            r[j] = __builtin_fmaf(acc[j], p.alpha, b[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) r[j] = acc[j] * p.alpha;
     }
-    if (whole) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float t[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = r[8 * h + j];
-            store8<OUT_DT>(p.out, i + 8 * h, t);
+    for (int j = 0; j < 8; j++) {
+        r[j] = p.base ? __builtin_fmaf(acc[j], p.alpha, b[j]) : acc[j] * p.alpha;
+        if (n + j < p.n) {
+            poison_in = __builtin_fmaf(b[j], 0.0f, poison_in);
+            poison_out = __builtin_fmaf(r[j], 0.0f, poison_out);
+            nan |= r[j] != r[j];
         }
-    } else {
+    }
+    if (vec) store8<OUT_DT>(p.out, i, r);
+    else {
 #pragma unroll
-        for (int j = 0; j < 16; j++)
+        for (int j = 0; j < 8; j++)
             if (n + j < p.n) store1<OUT_DT>(p.out, i + j, r[j]);
     }
-    if (p.flags) {
-        bool nan = poison_in != 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            if (n + j < p.n) {
-                poison_out = __builtin_fmaf(r[j], 0.0f, poison_out);
-                nan |= r[j] != r[j];
-            }
-        }
-        if (nan || poison_out != 0.0f) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
-    }
+    nan |= poison_in != 0.0f;
+    if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
 }
 
 // Scales of a tile's 128 rows, CH words each: four blocks a word for the matrix unit, else a float a block.
@@ -215,14 +201,14 @@ __global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
         i32x8 fa[4], fb[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int ra = wm + 16 * i + r, rb = wn + 16 * (r >> 2) + 4 * i + (r & 3);
-            u32x4 a0 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g) ^ swz_a(ra)));
-            u32x4 a1 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((2 * g + 1) ^ swz_a(ra)));
-            u32x4 b0 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g) ^ swz_b(rb)));
-            u32x4 b1 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((2 * g + 1) ^ swz_b(rb)));
+            const int ra = wm + 16 * i + r, rb = wn + b_row(i) + 8 * (r >> 2) + (r & 3);
+            u32x4 a0 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * (g ^ swz_a(ra)));
+            u32x4 a1 = *reinterpret_cast<const u32x4 *>(la + ra * 128 + 16 * ((g + 4) ^ swz_a(ra)));
+            u32x4 b0 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * (g ^ swz_b(rb)));
+            u32x4 b1 = *reinterpret_cast<const u32x4 *>(lb + rb * 128 + 16 * ((g + 4) ^ swz_b(rb)));
             if (last) {                                                           // bytes behind column k are not the matrix's
-                a0 = first_bytes(a0, tail - 32 * g); a1 = first_bytes(a1, tail - 32 * g - 16);
-                b0 = first_bytes(b0, tail - 32 * g); b1 = first_bytes(b1, tail - 32 * g - 16);
+                a0 = first_bytes(a0, tail - 16 * g); a1 = first_bytes(a1, tail - 64 - 16 * g);
+                b0 = first_bytes(b0, tail - 16 * g); b1 = first_bytes(b1, tail - 64 - 16 * g);
             }
             fa[i] = join(a0, a1);
             fb[i] = join(b0, b1);
@@ -233,7 +219,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 ka[i] = s_a[w][wm + 16 * i + r] >> sh;
-                kbs[i] = s_b[w][wn + 16 * (r >> 2) + 4 * i + (r & 3)] >> sh;
+                kbs[i] = s_b[w][wn + b_row(i) + 8 * (r >> 2) + (r & 3)] >> sh;
             }
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -247,7 +233,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 sa[i] = __uint_as_float(s_a[w][wm + 16 * i + r]);
-                sb[i] = *reinterpret_cast<const f32x4v *>(&s_b[w][wn + 16 * g + 4 * i]);
+                sb[i] = *reinterpret_cast<const f32x4v *>(&s_b[w][wn + b_row(i) + 8 * g]);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -277,53 +263,253 @@ __global__ __launch_bounds__(MECHA_BLOCK) void product_kernel(ProductParams p) {
     }
     const bool vec = p.n % 8 == 0 && mecha_aligned16(p.out) && (p.base == nullptr || mecha_aligned16(p.base));
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float row[16];
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int f = 0; f < 4; f++)
+        for (int h = 0; h < 2; h++) {
+            float row[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) row[4 * f + e] = acc[i][f][e];
-        store_row16<OUT_DT>(p, m0 + wm + 16 * i + r, n0 + wn + 16 * g, row, vec);
+            for (int f = 0; f < 2; f++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) row[4 * f + e] = acc[i][2 * h + f][e];
+            store_any8<OUT_DT>(p, m0 + wm + 16 * i + r, n0 + wn + 32 * h + 8 * g, row, vec);
+        }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+// ---------------------------------------------------------------------------------------------------- small products
+// 16 AI x 16 BI outputs by 8 waves that share out the blocks of k: a wave's codes go from memory straight into its registers, all of
+// them in flight at once, and the 8 partial sums meet in LDS, added in the order of the waves.  For results of few tiles, down to one
+// row: what counts there is one trip to memory, and that every CU has a piece of b.
+constexpr int DIRECT_WAVES = 8, DIRECT_THREADS = 64 * DIRECT_WAVES;
+
+template <int MODE, int AI, int BI>
+__global__ __launch_bounds__(DIRECT_THREADS, 2) void product_direct_kernel(ProductParams p) {
+    constexpr int TM = 16 * AI, TN = 16 * BI, LINE = TN + 4;                      // floats of a line in LDS
+    constexpr bool EXACT = MODE == EXACT_F32 || MODE == EXACT_E8M0;
+    extern __shared__ __attribute__((aligned(16))) float sums[];                  // [wave][row][LINE]
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int g = lane >> 4, r = lane & 15;
+    const int64_t m0 = (int64_t)(blockIdx.x % (uint32_t)p.tiles_m) * TM, n0 = (int64_t)(blockIdx.x / (uint32_t)p.tiles_m) * TN;
+    const int n_kb = (int)((p.k + SCALE_BLOCK - 1) / SCALE_BLOCK);
+    const int tail = (int)(p.k - (int64_t)(n_kb - 1) * SCALE_BLOCK);
+
+    // rows behind the last one read the last one
+    const uint8_t *a[AI], *b[BI];
+    int64_t as[AI], bs[BI];                                                       // first scale of this lane's row
+#pragma unroll
+    for (int i = 0; i < AI; i++) {
+        int64_t row = m0 + 16 * i + r;
+        row = row < p.m ? row : p.m - 1;
+        a[i] = p.a + row * p.a_pitch + 16 * g;
+        as[i] = (p.a_tile ? row / SCALE_BLOCK : row) * p.sa_pitch;
+    }
+#pragma unroll
+    for (int f = 0; f < BI; f++) {
+        int64_t row = n0 + 16 * f + r;
+        row = row < p.n ? row : p.n - 1;
+        b[f] = p.b + row * p.b_pitch + 16 * g;
+        bs[f] = (p.b_tile ? row / SCALE_BLOCK : row) * p.sb_pitch;
+    }
+    // float32 scales of b belong to the accumulators' rows, 4 g + e of a fragment
+    int64_t bse[BI][4];
+    if constexpr (MODE == F32_SCALES || MODE == EXACT_F32) {
+#pragma unroll
+        for (int f = 0; f < BI; f++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                int64_t row = n0 + 16 * f + 4 * g + e;
+                row = row < p.n ? row : p.n - 1;
+                bse[f][e] = (p.b_tile ? row / SCALE_BLOCK : row) * p.sb_pitch;
+            }
+    }
+    f32x4v acc[AI][BI];
+#pragma unroll
+    for (int i = 0; i < AI; i++)
+#pragma unroll
+        for (int f = 0; f < BI; f++) acc[i][f] = f32x4v{0, 0, 0, 0};
+
+    struct Step { i32x8 a[AI], b[BI]; uint32_t sa[AI], sb[BI]; f32x4v sbe[BI]; };
+    auto load = [&](int kb, Step &s) {
+        const int64_t at = (int64_t)kb * SCALE_BLOCK;
+#pragma unroll
+        for (int f = 0; f < BI; f++) s.b[f] = join(*reinterpret_cast<const u32x4 *>(b[f] + at), *reinterpret_cast<const u32x4 *>(b[f] + at + 64));
+#pragma unroll
+        for (int i = 0; i < AI; i++) s.a[i] = join(*reinterpret_cast<const u32x4 *>(a[i] + at), *reinterpret_cast<const u32x4 *>(a[i] + at + 64));
+        if constexpr (MODE == HW_SCALES || MODE == EXACT_E8M0) {
+#pragma unroll
+            for (int i = 0; i < AI; i++) s.sa[i] = static_cast<const uint8_t *>(p.sa)[as[i] + kb];
+#pragma unroll
+            for (int f = 0; f < BI; f++) s.sb[f] = static_cast<const uint8_t *>(p.sb)[bs[f] + kb];
+        } else {
+#pragma unroll
+            for (int i = 0; i < AI; i++) s.sa[i] = static_cast<const uint32_t *>(p.sa)[as[i] + kb];
+#pragma unroll
+            for (int f = 0; f < BI; f++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s.sbe[f][e] = static_cast<const float *>(p.sb)[bse[f][e] + kb];
+        }
+    };
+    auto cut = [&](i32x8 &v) {                                                    // bytes behind column k are not the matrix's
+        const u32x4 lo = first_bytes(u32x4{(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]}, tail - 16 * g);
+        const u32x4 hi = first_bytes(u32x4{(uint32_t)v[4], (uint32_t)v[5], (uint32_t)v[6], (uint32_t)v[7]}, tail - 64 - 16 * g);
+        v = join(lo, hi);
+    };
+    auto multiply = [&](int kb, Step &s) {
+        if (kb + 1 == n_kb && tail < SCALE_BLOCK) {
+#pragma unroll
+            for (int i = 0; i < AI; i++) cut(s.a[i]);
+#pragma unroll
+            for (int f = 0; f < BI; f++) cut(s.b[f]);
+        }
+        if constexpr (MODE == HW_SCALES) {
+#pragma unroll
+            for (int i = 0; i < AI; i++)
+#pragma unroll
+                for (int f = 0; f < BI; f++) acc[i][f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(s.b[f], s.a[i], acc[i][f], 0, 0, 0, (int)s.sb[f], 0, (int)s.sa[i]);
+        } else if constexpr (MODE == EXACT_E8M0) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                bf16x8 bq[BI];
+#pragma unroll
+                for (int f = 0; f < BI; f++) bq[f] = codes_to_bf16(s.b[f][2 * q], s.b[f][2 * q + 1], __uint_as_float(s.sb[f] << 23));
+#pragma unroll
+                for (int i = 0; i < AI; i++) {
+                    const bf16x8 aq = codes_to_bf16(s.a[i][2 * q], s.a[i][2 * q + 1], __uint_as_float(s.sa[i] << 23));
+#pragma unroll
+                    for (int f = 0; f < BI; f++) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f], aq, acc[i][f], 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < AI; i++)
+#pragma unroll
+                for (int f = 0; f < BI; f++) {
+                    f32x4v d = {0, 0, 0, 0};
+                    if constexpr (EXACT) d = exact_block(s.b[f], s.a[i], d);
+                    else d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(s.b[f], s.a[i], d, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[e], __uint_as_float(s.sa[i]) * s.sbe[f][e], acc[i][f][e]);
+                }
+        }
+    };
+    // two steps in flight
+    Step s0, s1;
+    int kb = wave;
+    if (kb < n_kb) load(kb, s0);
+    while (kb < n_kb) {
+        if (kb + DIRECT_WAVES < n_kb) load(kb + DIRECT_WAVES, s1);
+        multiply(kb, s0);
+        kb += DIRECT_WAVES;
+        if (kb >= n_kb) break;
+        if (kb + DIRECT_WAVES < n_kb) load(kb + DIRECT_WAVES, s0);
+        multiply(kb, s1);
+        kb += DIRECT_WAVES;
+    }
+#pragma unroll
+    for (int i = 0; i < AI; i++)
+#pragma unroll
+        for (int f = 0; f < BI; f++) *reinterpret_cast<f32x4v *>(&sums[(wave * TM + 16 * i + r) * LINE + 16 * f + 4 * g]) = acc[i][f];
+    __syncthreads();
+    // 4 columns a thread
+    const int used = n_kb < DIRECT_WAVES ? n_kb : DIRECT_WAVES;
+    const int esize = p.out_dt == MECHA_F32 ? 4 : 2, bsize = p.base_dt == MECHA_F32 ? 4 : 2;
+    const bool vec = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) % (4 * esize)) == 0 && (p.base == nullptr || (reinterpret_cast<uintptr_t>(p.base) % (4 * bsize)) == 0);
+    for (int x = t; x < TM * BI * 4; x += DIRECT_THREADS) {
+        const int row = x / (BI * 4), col = 4 * (x - row * (BI * 4));
+        const int64_t m = m0 + row, n = n0 + col, at = m * p.n + n;
+        if (m >= p.m || n >= p.n) continue;
+        f32x4v sum = *reinterpret_cast<const f32x4v *>(&sums[row * LINE + col]);
+        for (int w = 1; w < used; w++) {
+            const f32x4v v = *reinterpret_cast<const f32x4v *>(&sums[(w * TM + row) * LINE + col]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += v[e];
+        }
+        float base[4] = {0, 0, 0, 0}, out[4];
+        if (p.base) {
+            if (vec && p.base_dt == MECHA_F32) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p.base) + at);
+#pragma unroll
+                for (int e = 0; e < 4; e++) base[e] = v[e];
+            } else if (vec) {
+                const u32x2 v = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.base) + at);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t half = e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xffffu;
+                    base[e] = p.base_dt == MECHA_BF16 ? bf16_bits_to_f32(half) : f16_bits_to_f32(half);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (n + e < p.n) base[e] = p.base_dt == MECHA_F32 ? load1<MECHA_F32>(p.base, at + e) : p.base_dt == MECHA_F16 ? load1<MECHA_F16>(p.base, at + e) : load1<MECHA_BF16>(p.base, at + e);
+            }
+        }
+        float poison = 0.0f, poison_in = 0.0f;
+        bool nan = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            out[e] = p.base ? __builtin_fmaf(sum[e], p.alpha, base[e]) : sum[e] * p.alpha;
+            if (n + e < p.n) {
+                poison = __builtin_fmaf(out[e], 0.0f, poison);
+                poison_in = __builtin_fmaf(base[e], 0.0f, poison_in);
+                nan |= out[e] != out[e];
+            }
+        }
+        if (vec && p.out_dt == MECHA_F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + at) = f32x4{out[0], out[1], out[2], out[3]};
+        else if (vec)
+            *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p.out) + at) =
+                p.out_dt == MECHA_BF16 ? u32x2{pack_bf16(out[0], out[1]), pack_bf16(out[2], out[3])} : u32x2{pack_f16(out[0], out[1]), pack_f16(out[2], out[3])};
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.n) {
+                    if (p.out_dt == MECHA_F32) store1<MECHA_F32>(p.out, at + e, out[e]);
+                    else if (p.out_dt == MECHA_F16) store1<MECHA_F16>(p.out, at + e, out[e]);
+                    else store1<MECHA_BF16>(p.out, at + e, out[e]);
+                }
+        }
+        nan |= poison_in != 0.0f;
+        if (p.flags && (nan || poison != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
     }
 }
 
-// 8 contiguous columns of one output row where rows start 16-byte aligned and base has the result's type
-template <int OUT_DT, bool BASE>
-__device__ __forceinline__ void store_row8(const ProductParams &p, int64_t i, const float (&acc)[8]) {
-    float r[8], poison_in = 0.0f;
-    if constexpr (BASE) {
-        float b[8];
-        load8<OUT_DT>(p.base, i, b);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            poison_in = __builtin_fmaf(b[j], 0.0f, poison_in);
-            r[j] = __builtin_fmaf(acc[j], p.alpha, b[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) r[j] = acc[j] * p.alpha;
-    }
-    store8<OUT_DT>(p.out, i, r);
-    if (p.flags) {
-        float poison = 0.0f;
-        bool nan = poison_in != 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) { poison = __builtin_fmaf(r[j], 0.0f, poison); nan |= r[j] != r[j]; }
-        if (nan || poison != 0.0f) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
-    }
+template <int MODE, int AI, int BI>
+int launch_direct(ProductParams p, hipStream_t s) {
+    auto *const kernel = &product_direct_kernel<MODE, AI, BI>;
+    constexpr int bytes = DIRECT_WAVES * 16 * AI * (16 * BI + 4) * (int)sizeof(float);
+    if (bytes > 64 * 1024) MECHA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    p.tiles_m = (int)((p.m + 16 * AI - 1) / (16 * AI));
+    p.tiles_n = (int)((p.n + 16 * BI - 1) / (16 * BI));
+    MECHA_LAUNCH(MK_BLOCKS_PRODUCT, kernel, dim3((unsigned)p.tiles_m * (unsigned)p.tiles_n), dim3(DIRECT_THREADS), bytes, s, p);
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+template <int MODE>
+int launch_direct(int shape, const ProductParams &p, hipStream_t s) {
+    if (shape == 0) return launch_direct<MODE, 1, 1>(p, s);
+    if (shape == 1) return launch_direct<MODE, 1, 2>(p, s);
+    if (shape == 2) return launch_direct<MODE, 2, 2>(p, s);
+    return launch_direct<MODE, 2, 4>(p, s);
 }
 
 // ---------------------------------------------------------------------------------------------------- large products
-// 256 x 256 outputs by 8 waves of 128 x 64, one workgroup a CU that goes on from tile to tile.  A K step is one block of 128: 64 KiB of
-// codes in one of two LDS stages, 32 matrix instructions a wave.  The next step's codes -- the next tile's at a tile's end -- are on their
-// way while this one is multiplied, also over the epilogue; so are the scales of the next BIG_CH words of blocks.  One barrier a
-// step: behind it every wave's part of this stage has landed and the other stage has been read.
+// 32 MI x 256 outputs by 8 waves of 16 MI x 64, one workgroup a CU that goes on from tile to tile.  A K step is one block of 128: up to
+// 64 KiB of codes in one of two LDS stages, 4 MI matrix instructions a wave (16 MI for float32 results).  The next step's codes -- the next
+// tile's at a tile's end -- are on their way while this one is multiplied, also over the epilogue; so are the scales of the next BIG_CH
+// words of blocks.  One barrier a step: behind it every wave's part of this stage has landed and the other stage has been read.
 // Workgroups go round the 8 XCDs, each with its own L2: an XCD gets a run of tiles, ordered so that the 32 at work at a time are 8 x 4
-// tiles (2 MiB of a and 1 MiB of b at k = 1024).
-constexpr int BIG = 256, BIG_THREADS = 512, BIG_CH = 4, BIG_CUS = 256, BIG_BAND = 8;
+// tiles (2 MiB of a and 1 MiB of b at k = 1024, MI = 8).
+constexpr int BIG_N = 256, BIG_M = 256, BIG_THREADS = 512, BIG_CH = 4, BIG_CUS = 256, BIG_BAND = 8;
 struct BigLds {
-    uint8_t stage[2][2][BIG * 128];               // [stage][a, b][row][128]
-    uint32_t scale[2][2][BIG_CH][BIG];            // [parity of the chunk][a, b][word][row]
+    uint8_t stage[2][2][BIG_M * 128];             // [stage][a, b][row][128]
+    uint32_t scale[2][2][BIG_CH][BIG_M];          // [parity of the chunk][a, b][word][row]
 };
 
 __device__ __forceinline__ void lds_barrier() {
@@ -331,60 +517,80 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-
-template <int MODE, int OUT_DT, bool B_UNIFORM, bool BASE>
+// 1 KiB, as dma4
+__device__ __forceinline__ void dma1(const uint8_t *base, uint32_t off, uint32_t dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(base), "s"(dst) : "memory");
+}
+__device__ __forceinline__ uint32_t from_pair(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true); }   // lane ^ 1's
+// Lanes 2 q and 2 q + 1 hold two 16-byte pieces of rows 2 q and 2 q + 1 each; afterwards lane 2 q holds the first pieces of both
+// rows and lane 2 q + 1 the second ones (and back again: the exchange is its own inverse).
+__device__ __forceinline__ void exchange(u32x4 &c0, u32x4 &c1, bool odd) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t got = from_pair(odd ? c0[j] : c1[j]);
+        c0[j] = odd ? got : c0[j];
+        c1[j] = odd ? c1[j] : got;
+    }
+}
+template <int MODE, bool B_UNIFORM, int MI, bool BF16, bool BASE>
 __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[];
     BigLds &lds = *reinterpret_cast<BigLds *>(lds_raw);
-    constexpr int PER = MODE == HW_SCALES ? 4 * BIG_CH : BIG_CH;                 // blocks a chunk of scales
+    constexpr bool EXACT = MODE == EXACT_F32 || MODE == EXACT_E8M0;              // float32 results
+    constexpr int ROWS = 32 * MI, PER = MODE == HW_SCALES ? 4 * BIG_CH : BIG_CH; // rows of a tile; blocks a chunk of scales
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int g = lane >> 4, r = lane & 15;
-    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
+    const int wm = (wave & 1) * (16 * MI), wn = (wave >> 1) * 64;
     const int n_kb = (int)((p.k + SCALE_BLOCK - 1) / SCALE_BLOCK);
     const int tail = (int)(p.k - (int64_t)(n_kb - 1) * SCALE_BLOCK);
 
     // this workgroup's tiles: every (gridDim / 8)-th of its XCD's run
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    const int xcd = blockIdx.x & 7, per_xcd = gridDim.x >> 3;
-    const int64_t run0 = tiles * xcd / 8, run1 = tiles * (xcd + 1) / 8;
-    int64_t tile = run0 + (blockIdx.x >> 3);
+    const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;             // < 2^24
+    const uint32_t xcd = blockIdx.x & 7, per_xcd = gridDim.x >> 3;
+    const uint32_t run0 = tiles * xcd / 8, run1 = tiles * (xcd + 1) / 8;
+    uint32_t tile = run0 + (blockIdx.x >> 3);
     if (tile >= run1) return;
     // bands of BIG_BAND rows of tiles, down the band first
-    auto place = [&](int64_t i, int64_t &m0, int64_t &n0) {
-        const int band_tiles = BIG_BAND * p.tiles_n;
-        const int band = (int)(i / band_tiles), in = (int)(i - (int64_t)band * band_tiles);
-        const int high = p.tiles_m - band * BIG_BAND < BIG_BAND ? p.tiles_m - band * BIG_BAND : BIG_BAND;
-        m0 = (int64_t)(band * BIG_BAND + in % high) * BIG;
-        n0 = (int64_t)(in / high) * BIG;
+    auto place = [&](uint32_t i, uint32_t &m0, uint32_t &n0) {
+        const uint32_t band_tiles = BIG_BAND * (uint32_t)p.tiles_n, band = i / band_tiles, in = i - band * band_tiles;
+        const uint32_t left = (uint32_t)p.tiles_m - band * BIG_BAND, high = left < BIG_BAND ? left : BIG_BAND;
+        n0 = in / high * BIG_N;
+        m0 = (band * BIG_BAND + in % high) * ROWS;
     };
 
-    // DMA: wave w brings rows 32 w .. + 31 of each side, 8 an instruction; rows behind the last one read the last one
-    uint32_t oa[4], ob[4];
+    // b's rows of fragment f: 16-bit results: 8 contiguous columns a lane and pair of fragments; float32: 4 a fragment
+    auto b_at = [](int f, int rr) { return EXACT ? 16 * f + rr : b_row(f) + 8 * (rr >> 2) + (rr & 3); };
+    auto swz_n = [](int row) { return EXACT ? swz_a(row) : swz_b(row); };
+
+    // DMA: wave w brings rows 8 w .. + 7 of every 64 of each side, 1 KiB a piece; rows behind the last one read the last one
+    constexpr int PIECES = 4 + (ROWS + 63) / 64;
+    const int bring_row = 8 * wave + (lane >> 3);
+    const uint32_t part_a = 16u * (uint32_t)((lane & 7) ^ swz_a(bring_row)), part_b = 16u * (uint32_t)((lane & 7) ^ swz_n(bring_row));
+    int last_a, last_b;
     const uint8_t *ga, *gb;
-    auto aim = [&](int64_t m0, int64_t n0) {
-        const int la = p.m - 1 - m0 < BIG ? (int)(p.m - 1 - m0) : BIG, lb = p.n - 1 - n0 < BIG ? (int)(p.n - 1 - n0) : BIG;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = 32 * wave + 8 * i + (lane >> 3), slot = lane & 7;
-            oa[i] = (uint32_t)(row < la ? row : la) * (uint32_t)p.a_pitch + 16u * (uint32_t)(slot ^ swz_a(row));
-            ob[i] = (uint32_t)(row < lb ? row : lb) * (uint32_t)p.b_pitch + 16u * (uint32_t)(slot ^ swz_b(row));
-        }
-        ga = p.a + m0 * p.a_pitch;
-        gb = p.b + n0 * p.b_pitch;
+    auto aim = [&](uint32_t m0, uint32_t n0) {
+        last_a = p.m - 1 - m0 < BIG_M ? (int)(p.m - 1 - m0) : BIG_M;
+        last_b = p.n - 1 - n0 < BIG_N ? (int)(p.n - 1 - n0) : BIG_N;
+        ga = p.a + (int64_t)m0 * p.a_pitch;
+        gb = p.b + (int64_t)n0 * p.b_pitch;
     };
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte *)lds_raw) + (uint32_t)wave * 4096u;
-    auto issue = [&](int kb, int to) {
-        const uint32_t dst = lds0 + (uint32_t)to * (2 * BIG * 128);
-        dma4(ga + (int64_t)kb * SCALE_BLOCK, oa[0], oa[1], oa[2], oa[3], dst);
-        dma4(gb + (int64_t)kb * SCALE_BLOCK, ob[0], ob[1], ob[2], ob[3], dst + BIG * 128);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte *)lds_raw) + (uint32_t)wave * 1024u;
+    auto issue = [&](int kb, int to, int x) {                                     // piece x: b's four, then a's
+        if (x >= PIECES) return;
+        const bool of_b = x < 4;
+        const int y = of_b ? x : x - 4, row = 64 * y + bring_row, end = of_b ? last_b : last_a;
+        dma1((of_b ? gb : ga) + (int64_t)kb * SCALE_BLOCK, (uint32_t)(row < end ? row : end) * (uint32_t)(of_b ? p.b_pitch : p.a_pitch) + (of_b ? part_b : part_a),
+             lds0 + (uint32_t)to * (2 * BIG_M * 128) + (of_b ? BIG_M * 128 : 0) + 8192u * y);
     };
     // scales: thread (side, row) holds the words of a chunk between load and store
     uint32_t held[BIG_CH];
     const int side = __builtin_amdgcn_readfirstlane(t >> 8), srow = t & 255;
-    auto load_scales = [&](int64_t m0, int64_t n0, int kb0) {
+    auto load_scales = [&](uint32_t m0, uint32_t n0, int kb0) {
         const void *s = side ? p.sb : p.sa;
         const int64_t rows = side ? p.n : p.m, pitch = side ? p.sb_pitch : p.sa_pitch;
-        int64_t row = (side ? n0 : m0) + srow;
+        int64_t row = (int64_t)(side ? n0 : m0) + srow;
         if (row >= rows) row = rows - 1;
         if (side ? p.b_tile : p.a_tile) row /= SCALE_BLOCK;
         if constexpr (MODE == HW_SCALES) {                                        // four bytes at a time, at the end the row's last four
@@ -397,41 +603,53 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                 held[w] = v >> (8 * ((kb - from) & 3));
             }
         } else {
-            const float *at = static_cast<const float *>(s) + row * pitch;
 #pragma unroll
-            for (int w = 0; w < BIG_CH; w++) held[w] = __float_as_uint(at[kb0 + w < n_kb ? kb0 + w : n_kb - 1]);
+            for (int w = 0; w < BIG_CH; w++) {
+                const int64_t at = row * pitch + (kb0 + w < n_kb ? kb0 + w : n_kb - 1);
+                if constexpr (MODE == EXACT_E8M0) held[w] = static_cast<const uint8_t *>(s)[at];
+                else held[w] = __float_as_uint(static_cast<const float *>(s)[at]);
+            }
         }
     };
     auto put_scales = [&](int to) {
 #pragma unroll
-        for (int w = 0; w < BIG_CH; w++) lds.scale[to][side][w][srow] = held[w];
+        for (int w = 0; w < BIG_CH; w++) lds.scale[to][side][w][srow] = MODE == EXACT_E8M0 ? held[w] << 23 : held[w];
     };
 
     // fragment addresses inside a stage and a row of scales
-    uint32_t fa_at[2], fb_at[2];                                                  // of fragment 0; the others are 16 rows (a), 4 rows (b) on, in the same slots
-    const int ra0 = wm + r, rb0 = wn + 16 * (r >> 2) + (r & 3);
+    uint32_t fa_at[2], fb_at[2];                                                  // of fragment 0; the others lie whole rows on, in the same slots
+    const int ra0 = wm + r, rb0 = wn + b_at(0, r);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        fa_at[h] = (uint32_t)(ra0 * 128 + 16 * ((2 * g + h) ^ swz_a(ra0)));
-        fb_at[h] = (uint32_t)(rb0 * 128 + 16 * ((2 * g + h) ^ swz_b(rb0)));
+        fa_at[h] = (uint32_t)(ra0 * 128 + 16 * ((g + 4 * h) ^ swz_a(ra0)));
+        fb_at[h] = (uint32_t)(rb0 * 128 + 16 * ((g + 4 * h) ^ swz_n(rb0)));
     }
 
-    f32x4v acc[8][4];                                                             // [a fragment][b fragment]
+    f32x4v acc[MI][4];                                                            // [a fragment][b fragment]
     auto clear = [&]() {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < MI; i++)
 #pragma unroll
             for (int f = 0; f < 4; f++) acc[i][f] = f32x4v{0, 0, 0, 0};
     };
-    int64_t m0, n0, nm0 = 0, nn0 = 0;
+    uint32_t m0, n0, nm0 = 0, nn0 = 0;
     place(tile, m0, n0);
     aim(m0, n0);
-    issue(0, 0);
+#pragma unroll
+    for (int x = 0; x < PIECES; x++) issue(0, 0, x);
     load_scales(m0, n0, 0);
     put_scales(0);
     clear();
     wait_vm0();
     int stage = 0, chunk = 0, kb = 0;
+    // 16-bit results: fragment i + 2 of a is read while fragment i is multiplied, and a step's last fragment is multiplied behind the next
+    // barrier, while the next step's first ones come from LDS.
+    constexpr int SLOTS = MI == 4 ? 4 : 3;                                        // the carried fragment keeps its slot while fragment 0 is read
+    static_assert((MI - 1) % SLOTS != 0, "slots");
+    i32x8 fa[SLOTS], fb[4];
+    uint32_t sa[SLOTS], sb[4];                                                        // sb: the matrix unit's
+    f32x4v sbf[4];
+    float sb1 = 0.0f;
 #pragma clang loop unroll(disable)
     while (true) {
         const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
@@ -442,7 +660,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             for (int c = 0; c < 8; c++) {
                 const int sd = c >> 2, piece = 4 * (t & 1) + (c & 3), left = tail - 16 * piece;
                 if (left < 16) {
-                    u32x4 *at = reinterpret_cast<u32x4 *>(&lds.stage[stage][sd][row * 128 + 16 * (piece ^ (sd ? swz_b(row) : swz_a(row)))]);
+                    u32x4 *at = reinterpret_cast<u32x4 *>(&lds.stage[stage][sd][row * 128 + 16 * (piece ^ (sd ? swz_n(row) : swz_a(row)))]);
                     *at = first_bytes(*at, left);
                 }
             }
@@ -454,59 +672,137 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         }
         const int next_kb = last ? 0 : kb + 1;
         const bool refill = last ? more : next_kb % PER == 0;
-        if (!last || more) issue(next_kb, stage ^ 1);
         if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
-        {
-            const uint8_t *la = &lds.stage[stage][0][0], *lb = &lds.stage[stage][1][0];
-            i32x8 fb[4];
+
+        const uint8_t *la = &lds.stage[stage][0][0], *lb = &lds.stage[stage][1][0];
+        const int w = MODE == HW_SCALES ? (kb / 4) & (BIG_CH - 1) : kb & (BIG_CH - 1), sh = 8 * (kb & 3);
+        const uint32_t *sa_row = &lds.scale[chunk][0][w][ra0], *sb_row = &lds.scale[chunk][1][w][0];
+        auto read_a = [&](int i) { return join(*reinterpret_cast<const u32x4 *>(la + fa_at[0] + 2048 * i), *reinterpret_cast<const u32x4 *>(la + fa_at[1] + 2048 * i)); };
+        auto read_b = [&](int f) {
+            const int on = 128 * (b_at(f, 0) - b_at(0, 0));
+            return join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + on), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + on));
+        };
+        auto bring = [&](int x) { issue(next_kb, stage ^ 1, x); };
+        if constexpr (MODE == EXACT_E8M0) {
+            // the scales go into the conversion: code * 2^e is a bfloat16
+            bf16x8 bq[4][4];                                                      // b's, [fragment][quarter]
+            fa[0] = read_a(0);
+            sa[0] = sa_row[0];
 #pragma unroll
-            for (int f = 0; f < 4; f++)
-                fb[f] = join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + 512 * f), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + 512 * f));
-            // fragment i + 1 of a is read while fragment i is multiplied
-            const int w = MODE == HW_SCALES ? (kb / 4) & (BIG_CH - 1) : kb & (BIG_CH - 1), sh = 8 * (kb & 3);
-            auto read_a = [&](int i) { return join(*reinterpret_cast<const u32x4 *>(la + fa_at[0] + 2048 * i), *reinterpret_cast<const u32x4 *>(la + fa_at[1] + 2048 * i)); };
-            const uint32_t *sa_row = &lds.scale[chunk][0][w][ra0], *sb_row = &lds.scale[chunk][1][w][0];
-            uint32_t sb[4];                                                       // matrix unit's scales of b
-            f32x4v sbf[4];
-            float sb1 = 0.0f;
-            if constexpr (MODE == HW_SCALES) {
+            for (int f = 0; f < 4; f++) {
+                const i32x8 fb = read_b(f);
+                const float sb = __uint_as_float(sb_row[rb0 + 16 * f]);
 #pragma unroll
-                for (int f = 0; f < (B_UNIFORM ? 1 : 4); f++) sb[f] = sb_row[B_UNIFORM ? wn : rb0 + 4 * f] >> sh;
-            } else if constexpr (B_UNIFORM) sb1 = __uint_as_float(sb_row[wn]);
-            else {
-#pragma unroll
-                for (int f = 0; f < 4; f++) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * g + 4 * f]);
+                for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(fb[2 * q], fb[2 * q + 1], sb);
             }
-            i32x8 fa = read_a(0);
-            uint32_t sa = sa_row[0];
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                i32x8 fa_next = fa;
-                uint32_t sa_next = sa;
-                if (i < 7) { fa_next = read_a(i + 1); sa_next = sa_row[16 * (i + 1)]; }
-                __builtin_amdgcn_sched_barrier(0);
-                if constexpr (MODE == HW_SCALES) {
-                    const uint32_t sah = sa >> sh;
+            for (int i = 0; i < MI; i++) {
+                if (i + 1 < MI) { fa[(i + 1) & 1] = read_a(i + 1); sa[(i + 1) & 1] = sa_row[16 * (i + 1)]; }
+                bring(2 * i);
+                bring(2 * i + 1);
 #pragma unroll
-                    for (int f = 0; f < 4; f++)
-                        acc[i][f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa, acc[i][f], 0, 0, 0, (int)sb[B_UNIFORM ? 0 : f], 0, (int)sah);
-                } else {
-                    const float sf = __uint_as_float(sa) * (B_UNIFORM ? sb1 : 1.0f);
-                    f32x4v d[4];
+                for (int q = 0; q < 4; q++) {
+                    const bf16x8 aq = codes_to_bf16(fa[i & 1][2 * q], fa[i & 1][2 * q + 1], __uint_as_float(sa[i & 1]));
 #pragma unroll
-                    for (int f = 0; f < 4; f++)
-                        d[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa, f32x4v{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-#pragma unroll
-                    for (int f = 0; f < 4; f++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[f][e], B_UNIFORM ? sf : sf * sbf[f][e], acc[i][f][e]);
+                    for (int f = 0; f < 4; f++) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq, acc[i][f], 0, 0, 0);
                 }
-                // (nothing is executed here: the sums of this fragment are made at this point, not sunk to where they are stored)
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++)                                          // (nothing is executed here: the sums are made at this point, not sunk to the stores)
+                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
+        } else if constexpr (EXACT) {
+            bf16x8 bq[4][4];                                                      // b's codes as bfloat16, [fragment][quarter]
+            if constexpr (B_UNIFORM) sb1 = __uint_as_float(sb_row[wn]);
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const i32x8 fb = read_b(f);
+                if constexpr (!B_UNIFORM) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * f + 4 * g]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(fb[2 * q], fb[2 * q + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                const i32x8 fa = read_a(i);
+                bring(2 * i);
+                bring(2 * i + 1);
+                const float sa = __uint_as_float(sa_row[16 * i]) * (B_UNIFORM ? sb1 : 1.0f);
+                f32x4v d[4];
+#pragma unroll
+                for (int f = 0; f < 4; f++) d[f] = f32x4v{0, 0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const bf16x8 aq = codes_to_bf16(fa[2 * q], fa[2 * q + 1]);
+#pragma unroll
+                    for (int f = 0; f < 4; f++) d[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq, d[f], 0, 0, 0);
+                }
+#pragma unroll
+                for (int f = 0; f < 4; f++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[f][e], B_UNIFORM ? sa : sa * sbf[f][e], acc[i][f][e]);
+                // (nothing is executed here: the sums are made at this point, not sunk to where they are stored)
+                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
+            }
+        } else {
+            // One 16 x 16 x 128 product; shift: the byte of the scales' words that belongs to the step (HW_SCALES).
+            auto multiply = [&](int i, int f, int shift) {
+                if constexpr (MODE == HW_SCALES) {
+                    acc[i][f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i % SLOTS], acc[i][f], 0, 0, 0, (int)sb[f], 0, (int)(sa[i % SLOTS] >> shift));
+                } else {
+                    const f32x4v d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[f], fa[i % SLOTS], f32x4v{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    const float sf = __uint_as_float(sa[i % SLOTS]) * (B_UNIFORM ? sb1 : 1.0f);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[e], B_UNIFORM ? sf : sf * sbf[f][e], acc[i][f][e]);
+                }
+            };
+            auto pin = [&](int i) {                                               // (nothing is executed here: the sums are made at this point, not sunk to the stores)
                 asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
                 __builtin_amdgcn_sched_barrier(0);
-                fa = fa_next;
-                sa = sa_next;
+            };
+            auto fetch_a = [&](int i) { fa[i % SLOTS] = read_a(i); sa[i % SLOTS] = sa_row[16 * i]; };
+            auto fetch_b = [&](int f) {
+                if constexpr (MODE == HW_SCALES) sb[f] = sb_row[rb0 + b_row(f)] >> sh;
+                if constexpr (MODE == F32_SCALES && !B_UNIFORM) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + b_row(f) + 8 * g]);
+                fb[f] = read_b(f);
+            };
+            constexpr int Z = MI - 1;                                             // the fragment carried over
+            // The next stage is asked for in pieces between the products: the memory pipeline takes 1600 cycles for 64 KiB, and a wave that asks
+            // for more than it takes stands still.  Short steps need all the time there is for it.
+            constexpr int EARLY = MI == 4 ? PIECES : 2;
+            fetch_a(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kb > 0) {
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    multiply(Z, f, (sh - 8) & 31);
+                    asm volatile("" : "+v"(acc[Z][f]));
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_b(f);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+#pragma unroll
+                for (int f = 0; f < 4; f++) fetch_b(f);
+            }
+            if constexpr (B_UNIFORM) sb1 = __uint_as_float(sb_row[wn]);
+            fetch_a(1);
+#pragma unroll
+            for (int x = 0; x < EARLY; x++) bring(x);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < Z; i++) {
+                if (i + 2 < MI) fetch_a(i + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    multiply(i, f, sh);
+                    if (f % 2) bring(EARLY + 2 * i + f / 2);
+                }
+                pin(i);
+            }
+            if (last) {
+#pragma unroll
+                for (int f = 0; f < 4; f++) multiply(Z, f, sh);
+                pin(Z);
             }
         }
         wait_vm0();                                                               // the next stage; before the stores, which the same counter counts
@@ -514,26 +810,129 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         stage ^= 1;
         kb = next_kb;
         if (last) {
-            const int64_t n = n0 + wn + 16 * g;
+            // 16-byte pieces of two rows change places between two lanes, so that 8 lanes store a row's 128 bytes with one instruction;
+            // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280: 121 -> 103 us).
+            {
+                constexpr int EACH = EXACT ? 4 : 8, ESIZE = EXACT ? 4 : 2;        // elements of a piece, bytes of one
+                const bool odd = lane & 1;
+                const int64_t row0 = (int64_t)m0 + wm + (r & ~1), line = p.n * ESIZE;
+                const int rows = p.m - row0 < BIG_M ? (int)(p.m - row0) : BIG_M;
+                int64_t at0 = (row0 * p.n + n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g)) * ESIZE;
+                const int64_t cols = p.n - ((int64_t)n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g));
+                bool nan = false;
+                float poison_in = 0.0f, poison_out = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int64_t m = m0 + wm + 16 * i + r;
+                for (int i = 0; i < MI; i++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float row[8];
+                    for (int pair = 0; pair < (EXACT ? 2 : 1); pair++) {
+                        // this lane's pieces in memory: number 0 (even lane) or 1 (odd) of the pair
+                        const int64_t at = at0 + (EXACT ? 32 * ESIZE * pair : 0);
+                        const bool in = cols > (EXACT ? 32 * pair : 0), here = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
+                        u32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                        if constexpr (BASE) {
+                            if (here) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at));
+                            if (below) c[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at + line));
+                            exchange(c[0], c[1], odd);
+                        }
 #pragma unroll
-                    for (int f = 0; f < 2; f++)
+                        for (int h = 0; h < 2; h++) {
+                            float v[EACH];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) row[4 * f + e] = acc[i][2 * h + f][e];
-                    if (m < p.m && n + 8 * h < p.n) store_row8<OUT_DT, BASE>(p, m * p.n + n + 8 * h, row);
+                            for (int j = 0; j < EACH; j++) {
+                                const float sum = EXACT ? acc[i][2 * pair + h][j & 3] : acc[i][2 * h + (j >> 2)][j & 3];
+                                if constexpr (BASE) {
+                                    const uint32_t word = EXACT ? c[h][j & 3] : c[h][j >> 1];
+                                    const uint32_t half = j & 1 ? word >> 16 : word & 0xffffu;
+                                    const float bb = EXACT ? __uint_as_float(word) : BF16 ? bf16_bits_to_f32(half) : f16_bits_to_f32(half);
+                                    v[j] = __builtin_fmaf(sum, p.alpha, bb);
+                                    poison_in = __builtin_fmaf(bb, 0.0f, poison_in);
+                                } else v[j] = sum * p.alpha;
+                            }
+                            // (rows and columns behind the last ones are computed from the last ones: what is not finite there is so here)
+                            if (p.flags) {
+#pragma unroll
+                                for (int j = 0; j < EACH; j++) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
+                            }
+                            if constexpr (EXACT) c[h] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                            else {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) c[h][j] = BF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : pack_f16(v[2 * j], v[2 * j + 1]);
+                            }
+                        }
+                        exchange(c[0], c[1], odd);
+                        if (here) __builtin_nontemporal_store(c[0], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at));
+                        if (below) __builtin_nontemporal_store(c[1], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at + line));
+                    }
+                    at0 += 16 * line;
+                    asm volatile("" : "+v"(at0));                                 // (addresses one after the other, not all at once)
+                    if (i % 2) __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                nan |= poison_in != 0.0f;
+                if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
             }
             if (!more) break;
             tile += per_xcd; m0 = nm0; n0 = nn0;
             clear();
         }
     }
+}
+
+template <int MODE, bool B_UNIFORM, int MI>
+int launch_big(ProductParams p, hipStream_t s) {
+    p.tiles_m = (int)((p.m + 32 * MI - 1) / (32 * MI));
+    p.tiles_n = (int)((p.n + BIG_N - 1) / BIG_N);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, grid = tiles < BIG_CUS ? (tiles + 7) / 8 * 8 : BIG_CUS;
+    auto go = [&](auto bf16, auto base) -> int {
+        auto *const kernel = &product_big_kernel<MODE, B_UNIFORM, MI, decltype(bf16)::value, decltype(base)::value>;
+        MECHA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BigLds)));
+        MECHA_LAUNCH(MK_BLOCKS_PRODUCT, kernel, dim3((unsigned)grid), dim3(BIG_THREADS), sizeof(BigLds), s, p);
+        MECHA_CHECK_HIP(hipGetLastError());
+        return MECHA_OK;
+    };
+    auto with_base = [&](auto bf16) { return p.base ? go(bf16, std::true_type{}) : go(bf16, std::false_type{}); };
+    if constexpr (MODE == HW_SCALES || MODE == F32_SCALES) {
+        if (p.out_dt == MECHA_F16) return with_base(std::false_type{});
+    }
+    return with_base(std::true_type{});
+}
+template <int MODE, bool B_UNIFORM>
+int launch_big(int mi, const ProductParams &p, hipStream_t s) {
+    if constexpr (MODE == HW_SCALES || MODE == F32_SCALES) {
+        if (mi == 8) return launch_big<MODE, B_UNIFORM, 8>(p, s);
+        if (mi == 6) return launch_big<MODE, B_UNIFORM, 6>(p, s);
+    }
+    return launch_big<MODE, B_UNIFORM, 4>(p, s);
+}
+
+// ---------------------------------------------------------------------------------------------------- which kernel
+// The time each would take, in microseconds, from what it measured on 256 CUs (times fit within 20 % from 1 x 1280 x 1280 to
+// 16384 x 5120 x 640, all three kinds of sums):
+//   direct: a launch, plus the slower of one workgroup's reads (33 KB a us) and all reads together (5 TB/s);
+//   tiled:  rounds of tiles over the CUs, each n_kb steps and an epilogue.  128 x 128 tiles (two workgroups a CU) fill a few CUs more evenly:
+//           1024 x 1280 x 5120 36 us, 49 with 128 x 256 tiles; the larger ones share more: 8192 x 1280 x 5120 57 us (192 x 256), 80 with
+//           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 82 (128 x 256).
+struct Choice { int direct = -1, mi = 0; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
+Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
+    static const double step[3][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.57, 1.82, 0.0, 0.0}};    // 128 x 128, MI = 4, 6, 8
+    const double *us = step[mode == HW_SCALES ? 0 : mode == F32_SCALES ? 1 : 2];
+    const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
+    auto up = [](int64_t a, int64_t b) { return (double)((a + b - 1) / b); };
+    const double mid_tiles = up(m, 128) * up(n, 128) / BIG_CUS;
+    double best = 1.5 + (mid_tiles > 1.0 ? mid_tiles : 1.0) * (n_kb * us[0] + 1.0);
+    Choice c;
+    if (large_ok) {
+        for (int mi = 4; mi <= (us[2] > 0.0 ? 8 : 4); mi += 2) {
+            const double rounds = up((int64_t)(up(m, 32 * mi) * up(n, BIG_N)), BIG_CUS), t = 1.5 + rounds * (n_kb * us[mi / 2 - 1] + 0.25 * mi);
+            if (t < best) { best = t; c.mi = mi; }
+        }
+    }
+    static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
+    for (int d = 0; d < 4; d++) {
+        const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * (double)k, one = bytes / 33e3, all = blocks * bytes / 5e6;
+        const double t = 2.5 + (one > all ? one : all);
+        if (t < best) { best = t; c.mi = 0; c.direct = d; }
+    }
+    return c;
 }
 
 }  // namespace
@@ -559,28 +958,21 @@ int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, in
                     b_scale_pitch, b_tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
-    const int64_t bm = (m + BIG - 1) / BIG, bn = (n + BIG - 1) / BIG;
-    const bool big = out_dtype != MECHA_F32 && bm * bn >= 64 && k > 3 * SCALE_BLOCK && n % 8 == 0 && mecha_aligned16(out)
-                     && (base == nullptr || (base_dtype == out_dtype && mecha_aligned16(base)));
-    if (big) { p.tiles_m = (int)bm; p.tiles_n = (int)bn; }
-    int rc = MECHA_OK;
+    // The large kernel stores and reads base in 16-byte pieces of the result's type, and reads scales four blocks at a time.
+    const bool wide = out_dtype == MECHA_F32;
+    const bool large_ok = k > 3 * SCALE_BLOCK && n % (wide ? 4 : 8) == 0 && mecha_aligned16(out) && (base == nullptr || (base_dtype == out_dtype && mecha_aligned16(base)));
+    const Choice c = choose(m, n, k, wide ? EXACT_F32 : e8m0 ? HW_SCALES : F32_SCALES, large_ok);
+    if (c.direct >= 0) {
+        if (wide) return e8m0 ? launch_direct<EXACT_E8M0>(c.direct, p, s) : launch_direct<EXACT_F32>(c.direct, p, s);
+        return e8m0 ? launch_direct<HW_SCALES>(c.direct, p, s) : launch_direct<F32_SCALES>(c.direct, p, s);
+    }
+    if (c.mi) {
+        if (wide) return e8m0 ? launch_big<EXACT_E8M0, false>(c.mi, p, s) : launch_big<EXACT_F32, false>(c.mi, p, s);
+        if (e8m0) return launch_big<HW_SCALES, false>(c.mi, p, s);
+        return b_tile ? launch_big<F32_SCALES, true>(c.mi, p, s) : launch_big<F32_SCALES, false>(c.mi, p, s);
+    }
     auto go = [&](auto mode, auto dt) {
         constexpr int MODE = decltype(mode)::value, DT = decltype(dt)::value;
-        if constexpr (DT != MECHA_F32) {
-            if (big) {
-                auto large = [&](auto uniform, auto based) {
-                    constexpr bool U = decltype(uniform)::value, B = decltype(based)::value;
-                    auto *const kernel = &product_big_kernel<MODE, DT, U, B>;
-                    const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BigLds));
-                    if (room != hipSuccess) { mecha_set_error("%zu bytes of LDS: %s", sizeof(BigLds), hipGetErrorString(room)); rc = MECHA_ERR_HIP; return; }
-                    const int64_t grid = bm * bn < BIG_CUS ? (bm * bn + 7) / 8 * 8 : BIG_CUS;
-                    MECHA_LAUNCH(MK_BLOCKS_PRODUCT, kernel, dim3((unsigned)grid), dim3(BIG_THREADS), sizeof(BigLds), s, p);
-                };
-                auto with_base = [&](auto uniform) { if (base) large(uniform, std::true_type{}); else large(uniform, std::false_type{}); };
-                if (b_tile) with_base(std::true_type{}); else with_base(std::false_type{});
-                return;
-            }
-        }
         MECHA_LAUNCH(MK_BLOCKS_PRODUCT, (product_kernel<MODE, DT>), dim3((unsigned)(tm * tn)), dim3(MECHA_BLOCK), 0, s, p);
     };
     auto with_mode = [&](auto power, auto real, auto dt) { if (e8m0) go(power, dt); else go(real, dt); };
@@ -591,7 +983,6 @@ int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, in
         case MECHA_F16: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_F16>{}); break;
         default: with_mode(Hw{}, F32{}, std::integral_constant<int, MECHA_BF16>{}); break;
     }
-    if (rc) return rc;
     MECHA_CHECK_HIP(hipGetLastError());
     return MECHA_OK;
 }

@@ -239,6 +239,18 @@ def test_product_extreme_scales():
                 assert torch.equal(amd.block_product(a, b, out_dtype=dtype), want.float().to(dtype)), (m, ea, eb, dtype)
 
 
+def test_product_scales_that_are_not_a_number():
+    """A NaN scale of either kind makes its row, and only that, NaN."""
+    import sd_mecha_amd as amd
+    for m, n, k in ((2, 64, 300), (40, 56, 300), (2100, 2056, 1100)):
+        for scales in ("e8m0", "fp32"):
+            a, b = matrix(m, k, "rows", scales, 1), matrix(n, k, "tile", scales, 2)
+            a.scales.view(torch.uint8 if scales == "e8m0" else torch.int32)[1, -1] = 255 if scales == "e8m0" else 0x7FC00000
+            for dtype in (torch.float32, torch.bfloat16):
+                got = amd.block_product(a, b, out_dtype=dtype, check_finite=False)
+                assert bool(got[1].isnan().all()) and int(got.isnan().sum()) == n, (m, scales, dtype)
+
+
 def test_product_mixed_scales_base_types_and_shapes():
     import sd_mecha_amd as amd
     a, b = matrix(70, 200, "rows", "e8m0", 1), matrix(90, 200, "tile", "fp32", 2)
