@@ -2,11 +2,11 @@
 //
 //   g = grad * clip;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g g
 //   p = p (1 - lr wd[key]) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// in float32, every product, sum, quotient and root rounded by itself, whatever the storage types.
+// in float32, whatever the storage types.
 //
-// HBM-bound: 28 bytes an element with float32 throughout, 10 with 16-bit weights and gradients and 8-bit states.  One vector of
-// 8 elements a thread on a flat grid; a vector lies in one key (offsets are multiples of 8), its key is found by a search
-// over the segment table that a wave does once.
+// HBM-bound: 28 bytes an element with float32 throughout, 10 with 16-bit weights and gradients and 8-bit states.  One vector a
+// thread on a flat grid, 4 elements with float32 states and 8 with 8-bit ones; a vector lies in one key (offsets are multiples of
+// 8), its key is found by a search over the segment table that a wave does once, behind the loads.
 //
 // 8-bit states: e4m3 codes and a power-of-two scale for every 128 elements of the arena (segment offsets are multiples of 128, so
 // a block belongs to one key; 16 lanes own it).  The second moment is kept as its ROOT: e4m3 spans 2^18 between its largest and its
@@ -60,17 +60,59 @@ __device__ __forceinline__ int find_segment_wave(const mecha_segment *segs, int 
     return lo - 1;
 }
 
-// (segment or -1, elements of [i, i + 8) inside it).  i is a multiple of 8; every lane of the wave calls this.
-__device__ __forceinline__ int locate8(const mecha_segment *segs, int n, int64_t total, int64_t i, int64_t wave_i, int &valid) {
+// (segment or -1, elements of [i, i + N) inside it, elements from i to its end); a vector of N lies in one key.  Every lane of the wave
+// calls this.
+template <int N>
+__device__ __forceinline__ int locate(const mecha_segment *segs, int n, int64_t total, int64_t i, int64_t wave_i, int &valid, int64_t &left) {
     int s = find_segment_wave(segs, n, wave_i);
     while (s + 1 < n && segs[s + 1].offset <= i) s++;
     valid = 0;
+    left = INT64_MIN;
     if (s >= 0) {
-        int64_t left = segs[s].offset + segs[s].numel - i;
+        left = segs[s].offset + segs[s].numel - i;
         left = left < total - i ? left : total - i;
-        valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+        valid = left >= N ? N : left > 0 ? (int)left : 0;
     }
     return s;
+}
+
+// N consecutive elements of any type as float32: 4 (16 bytes of float32) or 8 (16 bytes of the 16-bit types), read or written once
+template <int DT, int N>
+__device__ __forceinline__ void load_n(const void *base, int64_t i, float (&v)[N]) {
+    if constexpr (N == 8) load8<DT, true>(base, i, v);
+    else if constexpr (DT == MECHA_F32) {
+        const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + i));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(base) + i));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t h = j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu;
+            v[j] = DT == MECHA_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+        }
+    }
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_n(void *base, int64_t i, const float (&v)[N]) {
+    if constexpr (N == 8) store8<DT, true>(base, i, v);
+    else if constexpr (DT == MECHA_F32)
+        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(static_cast<float *>(base) + i));
+    else {
+        u32x2 x;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            x[j] = DT == MECHA_BF16 ? f32_to_bf16_bits(v[2 * j]) | f32_to_bf16_bits(v[2 * j + 1]) << 16 : f32_to_f16_bits(v[2 * j]) | f32_to_f16_bits(v[2 * j + 1]) << 16;
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(base) + i));
+    }
+}
+
+// The square root to one unit in the last place, v_sqrt_f32's own error: float32's rounded root takes ten instructions more, and the code
+// or the weight that comes of it moves by far less than its rounding.  Under 2^-96 (where the instruction would take subnormals
+// for zeros) the root of 2^64 v.
+__device__ __forceinline__ float root_of(float v) {
+    const bool small = v < 1.262177448e-29f;
+    const float r = __builtin_amdgcn_sqrtf(small ? v * 18446744073709551616.0f : v);
+    return small ? r * 2.3283064365386963e-10f : r;
 }
 
 // 32 bits for an element: multiplications by odd constants (the first 32 fractional bits of the golden ratio and of the square roots
@@ -85,72 +127,41 @@ __device__ __forceinline__ uint32_t dither32(int64_t i, uint32_t key) {
 }
 __device__ __forceinline__ uint32_t dither_key(uint32_t step, uint32_t seed) { return step * 0x3C6EF373u + seed * 0x6A09E667u; }
 
-// |y| <= 448 down to a code or up to the next one: floor(|y| / distance + u / 2^16).  A float's top 12 bits below the sign are its
-// e4m3 code but for the exponent's bias, and the 20 below them its part of the distance: adding u << 4 carries with the right
-// probability.  Under 2^-6 the codes are 2^-9 apart like those of the next binade, so |y| + 2^-6 is rounded there instead.
-__device__ __forceinline__ uint32_t dithered_code(float y, uint32_t u) {
-    const float size = fabsf(y);
-    const bool small = size < 0.015625f;
-    const uint32_t bits = __float_as_uint(small ? size + 0.015625f : size);
-    uint32_t code = ((bits + (u << 4)) >> 20) - (small ? 968u : 960u);
-    code = nonfinite_f32(y) ? 0x7fu : code;
-    return code | ((__float_as_uint(y) >> 24) & 0x80u);
-}
-
 template <int P_DT, int G_DT, bool BITS8, bool VEC>
 __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
-    const int64_t i = ((int64_t)blockIdx.x * MECHA_BLOCK + threadIdx.x) * 8;
-    const int64_t wave_i = i - 8 * (threadIdx.x & 63);
+    constexpr int N = BITS8 ? 8 : 4;                          // elements a thread: 16 bytes of the arrays that weigh most
+    const int64_t i = ((int64_t)blockIdx.x * MECHA_BLOCK + threadIdx.x) * N;
+    const int64_t wave_i = i - N * (int)(threadIdx.x & 63);
     if (wave_i >= a.total) return;
+    float p[N], g[N], m[N], v[N];
+    u32x2 mc = {0, 0}, vc = {0, 0};
+    uint32_t ms = 0, vs = 0;
+    // what a whole vector of the arenas holds is on its way before the segment is known
+    const bool inside = i + N <= a.total;
+    if (VEC && inside) {
+        load_n<P_DT, N>(a.p, i, p);
+        load_n<G_DT, N>(a.g, i, g);
+        if constexpr (!BITS8) {
+            load_n<MECHA_F32, N>(a.m, i, m);
+            load_n<MECHA_F32, N>(a.v, i, v);
+        }
+    }
+    if constexpr (BITS8) {
+        if (inside) {                                         // (always: total is a multiple of 128)
+            mc = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(a.m) + i));
+            vc = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(a.v) + i));
+            ms = a.ms[i >> 7];
+            vs = a.vs[i >> 7];
+        }
+    }
+    int valid;
+    int64_t left;
+    const int s = locate<N>(a.segs, a.n_segs, a.total, i, wave_i, valid, left);
+    const float keep = 1.0f - a.lr * (a.decay ? (s >= 0 ? a.decay[s] : 0.0f) : a.decay_all);
     float clip = 1.0f;
     if (a.clip) {
         clip = a.clip[1];
         if (!(clip >= 0.0f)) return;                          // a gradient is inf or NaN: the step is left out
-    }
-    int valid;
-    const int s = locate8(a.segs, a.n_segs, a.total, i, wave_i, valid);
-    if constexpr (!BITS8) { if (valid == 0) return; }
-    const bool whole = VEC && valid == 8;
-    float p[8], g[8], m[8], v[8];
-    auto load = [&](auto dt, const void *from, float (&to)[8]) {
-        constexpr int DT = decltype(dt)::value;
-        if (whole) load8<DT, true>(from, i, to);
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) to[j] = j < valid ? load1<DT>(from, i + j) : 0.0f;
-        }
-    };
-    auto store = [&](auto dt, void *to, const float (&from)[8]) {
-        constexpr int DT = decltype(dt)::value;
-        if (whole) store8<DT, true>(to, i, from);
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < valid) store1<DT>(to, i + j, from[j]);
-        }
-    };
-    load(std::integral_constant<int, P_DT>{}, a.p, p);
-    load(std::integral_constant<int, G_DT>{}, a.g, g);
-    if constexpr (BITS8) {
-        if (valid) {                                          // a block's codes are all there, also behind its key's last element
-            const u32x2 mc = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(a.m) + i);
-            const u32x2 vc = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(a.v) + i);
-            const float sm = e8m0_to_f32(a.ms[i >> 7]), sv = e8m0_to_f32(a.vs[i >> 7]);
-            unpack_e4m3x4(mc.x, m); unpack_e4m3x4(mc.y, m + 4);
-            unpack_e4m3x4(vc.x, v); unpack_e4m3x4(vc.y, v + 4);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                m[j] = j < valid ? m[j] * sm : 0.0f;
-                const float root = j < valid ? v[j] * sv : 0.0f;
-                v[j] = root * root;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) m[j] = v[j] = 0.0f;
-        }
-    } else {
-        load(std::integral_constant<int, MECHA_F32>{}, a.m, m);
-        load(std::integral_constant<int, MECHA_F32>{}, a.v, v);
     }
     float size = a.size, root_size = a.root_size;
     uint32_t key = a.key;
@@ -165,18 +176,55 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         root_size = (float)(1.0 / sqrt(1.0 - w2));
         key = dither_key((uint32_t)t, a.seed);
     }
-    const float keep = 1.0f - a.lr * (a.decay ? (s >= 0 ? a.decay[s] : 0.0f) : a.decay_all);
-    bool bad_in = false, bad_out = false;
-    float root[8];
+    if (!BITS8 && valid == 0) return;
+    const bool whole = VEC && valid == N;
+    if (!VEC || !inside) {                                    // arenas that are not 16-byte aligned, an arena's last elements
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        bad_in |= nonfinite_f32(g[j]) || nonfinite_f32(p[j]);
+        for (int j = 0; j < N; j++) {
+            const bool in = j < valid;
+            p[j] = in ? load1<P_DT>(a.p, i + j) : 0.0f;
+            g[j] = in ? load1<G_DT>(a.g, i + j) : 0.0f;
+            if constexpr (!BITS8) {
+                m[j] = in ? load1<MECHA_F32>(a.m, i + j) : 0.0f;
+                v[j] = in ? load1<MECHA_F32>(a.v, i + j) : 0.0f;
+            }
+        }
+    }
+    auto store = [&](auto dt, void *to, const float (&from)[N]) {
+        constexpr int DT = decltype(dt)::value;
+        if (whole) store_n<DT, N>(to, i, from);
+        else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (j < valid) store1<DT>(to, i + j, from[j]);
+        }
+    };
+    if constexpr (BITS8) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {                      // two codes an instruction, the scale with them
+            const uint32_t mw = mc[j / 4], vw = vc[j / 4];
+            const f32x2 x = j & 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(mw, scale_bits(ms), true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(mw, scale_bits(ms), false);
+            const f32x2 y = j & 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(vw, scale_bits(vs), true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(vw, scale_bits(vs), false);
+            m[j] = x.x; m[j + 1] = x.y;
+            v[j] = y.x * y.x; v[j + 1] = y.y * y.y;
+        }
+        if (valid < 8) {                                      // what lies between the keys takes no part in a scale, and its codes become 0
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j >= valid) m[j] = v[j] = g[j] = 0.0f;
+        }
+    }
+    float poison_in = 0.0f, poison_out = 0.0f, root[N];       // fma(x, 0, poison) stays 0 while every x is finite
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        if (a.seg_flags && j < valid) poison_in = __builtin_fmaf(g[j], 0.0f, __builtin_fmaf(p[j], 0.0f, poison_in));
         const float gj = g[j] * clip;
-        m[j] = m[j] * a.b1 + gj * a.c1;
-        v[j] = v[j] * a.b2 + gj * gj * a.c2;
-        root[j] = __builtin_sqrtf(v[j]);
-        p[j] = p[j] * keep - m[j] / (root[j] * root_size + a.eps) * size;
-        bad_out |= nonfinite_f32(p[j]);
+        m[j] = __builtin_fmaf(gj, a.c1, m[j] * a.b1);
+        v[j] = __builtin_fmaf(gj * gj, a.c2, v[j] * a.b2);
+        root[j] = root_of(v[j]);
+        const float den = __builtin_fmaf(root[j], root_size, a.eps);
+        p[j] = __builtin_fmaf(m[j] * __builtin_amdgcn_rcpf(den), -size, p[j] * keep);
+        if (a.seg_flags && j < valid) poison_out = __builtin_fmaf(p[j], 0.0f, poison_out);
     }
     if (valid) {
         store(std::integral_constant<int, P_DT>{}, a.p, p);
@@ -189,35 +237,47 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
     if constexpr (BITS8) {
         float mm = 0.0f, vm = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            mm = fmaxf(mm, nonfinite_f32(m[j]) ? 0.0f : fabsf(m[j]));
-            vm = fmaxf(vm, nonfinite_f32(root[j]) ? 0.0f : root[j]);
-        }
+        for (int j = 0; j < 8; j++) { mm = fmaxf(mm, fabsf(m[j])); vm = fmaxf(vm, root[j]); }
         const int em = block_exponent(max16(mm)), ev = block_exponent(max16(vm));
-        const float im = pow2f(-em), iv = pow2f(-ev);
-        uint32_t mc[8], vc[8];
+        const float sm = scale_bits(em + 127), sv = scale_bits(ev + 127);
+        int mw[2] = {0, 0}, vw[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t u = dither32(i + j, key);
-            mc[j] = dithered_code(m[j] * im, u & 0xffffu);
-            const float y = root[j] * iv;
-            const uint32_t c = dithered_code(y, u >> 16);
-            vc[j] = y > 0.0f && c == 0u ? 1u : c;
+        for (int w = 0; w < 2; w++) {
+            // gfx950's stochastic conversion of x / 2^e: floor(|x| / distance + random / 2^32) for every code, subnormal ones too (checked on
+            // 2^22 numbers against the definition)
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[j] = dither32(i + 4 * w + j, key);
+            mw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(mw[w], m[4 * w], u[0] << 16, sm, 0);
+            mw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(mw[w], m[4 * w + 1], u[1] << 16, sm, 1);
+            mw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(mw[w], m[4 * w + 2], u[2] << 16, sm, 2);
+            mw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(mw[w], m[4 * w + 3], u[3] << 16, sm, 3);
+            // no root that is not zero goes under the smallest code: under it, it is raised to it, and not a random part further
+            const float least = sv * 0.001953125f;
+            float rr[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = root[4 * w + j];
+                const bool tiny = x > 0.0f && x < least;
+                rr[j] = tiny ? least : x;
+                u[j] = tiny ? 0u : u[j] & 0xffff0000u;
+            }
+            vw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(vw[w], rr[0], u[0], sv, 0);
+            vw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(vw[w], rr[1], u[1], sv, 1);
+            vw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(vw[w], rr[2], u[2], sv, 2);
+            vw[w] = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(vw[w], rr[3], u[3], sv, 3);
         }
-        if (valid) {
-            auto pack = [](const uint32_t (&c)[8]) {
-                return u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-            };
-            *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.m) + i) = pack(mc);
-            *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.v) + i) = pack(vc);
-            if ((threadIdx.x & 15) == 0) { a.ms[i >> 7] = (uint8_t)(em + 127); a.vs[i >> 7] = (uint8_t)(ev + 127); }
+        if (left > -(i & 127)) {                              // the key reaches into this block: its codes are all written
+            __builtin_nontemporal_store(u32x2{(uint32_t)mw[0], (uint32_t)mw[1]}, reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.m) + i));
+            __builtin_nontemporal_store(u32x2{(uint32_t)vw[0], (uint32_t)vw[1]}, reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.v) + i));
         }
+        if ((threadIdx.x & 15) == 0 && valid) { a.ms[i >> 7] = (uint8_t)(em + 127); a.vs[i >> 7] = (uint8_t)(ev + 127); }
     } else {
         store(std::integral_constant<int, MECHA_F32>{}, a.m, m);
         store(std::integral_constant<int, MECHA_F32>{}, a.v, v);
     }
-    if ((bad_in || bad_out) && valid && a.seg_flags)
-        atomicOr(a.seg_flags + s, (bad_in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+    if (a.seg_flags && valid && (poison_in != 0.0f || poison_out != 0.0f))
+        atomicOr(a.seg_flags + s, (poison_in != 0.0f ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
 }
 
 // ------------------------------------------------------------------------------------------------------- gradient norm
@@ -226,25 +286,46 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
 constexpr int NORM_GRID = 2048;
 
 template <int G_DT, bool VEC>
-__global__ __launch_bounds__(MECHA_BLOCK) void norm_partial_kernel(const void *g, const mecha_segment *segs, int n_segs, int64_t total, int64_t per_block,
+__global__ __launch_bounds__(MECHA_BLOCK) void norm_partial_kernel(const void *g, const mecha_segment *segs, int n_segs, int64_t total, int64_t per_wave,
                                                                    double *partial) {
     __shared__ double fold[MECHA_BLOCK];
-    const int64_t begin = blockIdx.x * per_block, end = begin + per_block < total ? begin + per_block : total;
+    constexpr int AHEAD = 4;                                  // vectors in flight a lane
+    const int lane = threadIdx.x & 63;
+    const int64_t begin = ((int64_t)blockIdx.x * (MECHA_BLOCK / 64) + (threadIdx.x >> 6)) * per_wave;
+    const int64_t end = begin + per_wave < total ? begin + per_wave : total;
     double sum = 0.0;
-    for (int64_t at = begin; at < end; at += 8 * MECHA_BLOCK) {
-        const int64_t i = at + 8 * threadIdx.x, wave_i = i - 8 * (threadIdx.x & 63);
-        if (wave_i >= end) break;
-        int valid;
-        locate8(segs, n_segs, total, i, wave_i, valid);
-        if (i >= end) valid = 0;
-        float v[8];
-        if (VEC && valid == 8) load8<G_DT, true>(g, i, v);
-        else {
+    int64_t key_begin = 0, key_end = 0;                       // a key's elements, the same for the whole wave
+    for (int64_t at = begin; at < end; at += 512 * AHEAD) {
+        float v[AHEAD][8];
+        const bool fast = VEC && at + 512 * AHEAD <= end;
+        if (fast) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = j < valid ? load1<G_DT>(g, i + j) : 0.0f;
+            for (int x = 0; x < AHEAD; x++) load8<G_DT, true>(g, at + 512 * x + 8 * lane, v[x]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum += (double)v[j] * (double)v[j];
+        for (int x = 0; x < AHEAD; x++) {
+            const int64_t wave_i = at + 512 * x, i = wave_i + 8 * lane;
+            if (wave_i >= end) break;
+            int valid = 8;
+            if (wave_i < key_begin || wave_i + 512 > key_end) {
+                int s = find_segment_wave(segs, n_segs, wave_i);
+                key_begin = s >= 0 ? segs[s].offset : 0;
+                key_end = s >= 0 ? segs[s].offset + segs[s].numel : 0;
+                key_end = key_end < total ? key_end : total;
+                int64_t left;
+                if (wave_i + 512 > key_end) locate<8>(segs, n_segs, total, i, wave_i, valid, left);
+                if (i >= end) valid = 0;
+            }
+            if (!fast) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[x][j] = j < valid && i < end ? load1<G_DT>(g, i + j) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double d = j < valid ? (double)v[x][j] : 0.0;
+                sum = __builtin_fma(d, d, sum);
+            }
+        }
     }
     fold[threadIdx.x] = sum;
     __syncthreads();
@@ -276,7 +357,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void norm_finish_kernel(const double *
 int check_arena(const mecha_segment *segs, int n_segs, int64_t total) {
     MECHA_REQUIRE(n_segs > 0 && segs != nullptr, "batched call needs a device segment table");
     MECHA_REQUIRE(total >= 0, "total_elems must be >= 0 (got %lld)", (long long)total);
-    MECHA_REQUIRE((total + 7) / 8 < (1ll << 32) - MECHA_BLOCK, "total_elems %lld is beyond one launch (2^35)", (long long)total);
+    MECHA_REQUIRE((total + 3) / 4 < (1ll << 32) - MECHA_BLOCK, "total_elems %lld is beyond one launch (2^34)", (long long)total);
     return MECHA_OK;
 }
 
@@ -310,16 +391,16 @@ int mecha_batched_grad_norm(const void *grad_arena, const mecha_segment *segment
         return MECHA_ERR_WORKSPACE;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t unit = 8 * MECHA_BLOCK, units = (total_elems + unit - 1) / unit;
-    const int64_t per_block = (units + NORM_GRID - 1) / NORM_GRID * unit;
-    const int grid = per_block ? (int)((total_elems + per_block - 1) / per_block) : 0;
+    const int64_t waves = NORM_GRID * (MECHA_BLOCK / 64), units = (total_elems + 2047) / 2048;
+    const int64_t per_wave = (units + waves - 1) / waves * 2048;                  // whole rounds of a wave
+    const int grid = per_wave ? (int)((total_elems + 4 * per_wave - 1) / (4 * per_wave)) : 0;
     double *partial = static_cast<double *>(workspace);
     const bool vec = mecha_aligned16(grad_arena);
     if (grid > 0)
         with_dtype(grad_dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
-            if (vec) MECHA_LAUNCH(MK_ADAMW, (norm_partial_kernel<DT, true>), dim3(grid), dim3(MECHA_BLOCK), 0, s, grad_arena, segments, n_segments, total_elems, per_block, partial);
-            else MECHA_LAUNCH(MK_ADAMW, (norm_partial_kernel<DT, false>), dim3(grid), dim3(MECHA_BLOCK), 0, s, grad_arena, segments, n_segments, total_elems, per_block, partial);
+            if (vec) MECHA_LAUNCH(MK_ADAMW, (norm_partial_kernel<DT, true>), dim3(grid), dim3(MECHA_BLOCK), 0, s, grad_arena, segments, n_segments, total_elems, per_wave, partial);
+            else MECHA_LAUNCH(MK_ADAMW, (norm_partial_kernel<DT, false>), dim3(grid), dim3(MECHA_BLOCK), 0, s, grad_arena, segments, n_segments, total_elems, per_wave, partial);
         });
     MECHA_LAUNCH(MK_ADAMW, norm_finish_kernel, dim3(1), dim3(MECHA_BLOCK), 0, s, partial, grid, max_norm, norm_out);
     MECHA_CHECK_HIP(hipGetLastError());
@@ -361,7 +442,7 @@ int mecha_batched_adamw(void *param_arena, const void *grad_arena, void *exp_avg
     }
     const bool vec = mecha_aligned16(param_arena) && mecha_aligned16(grad_arena) && (state_bits == 8 || (mecha_aligned16(exp_avg) && mecha_aligned16(exp_avg_sq)))
                      && (copy_arena == nullptr || mecha_aligned16(copy_arena));
-    const int64_t blocks = ((total_elems + 7) / 8 + MECHA_BLOCK - 1) / MECHA_BLOCK;
+    const int64_t each = (state_bits == 8 ? 8 : 4) * MECHA_BLOCK, blocks = (total_elems + each - 1) / each;
     hipStream_t s = static_cast<hipStream_t>(stream);
     with_dtype(param_dtype, [&](auto pd) {
         with_dtype(grad_dtype, [&](auto gd) {

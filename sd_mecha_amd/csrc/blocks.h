@@ -12,8 +12,8 @@ __device__ __forceinline__ int block_exponent(float amax) {
     const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -127 ? -127 : e;
 }
-// 2^e for -126 <= e <= 127; a block's -e is in -120..127
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 2^(byte - 127) as gfx950's scaled conversions take it: only the exponent's byte counts, 0 being 2^-127 and 255 NaN
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
 // 2^(byte - 127); byte 0 is 2^-127, a subnormal; byte 255 is NaN
 __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
     return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
@@ -24,11 +24,12 @@ __device__ __forceinline__ void unpack_e4m3x4(uint32_t w, float *v) {
     v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
 }
 
-// max over the 16 lanes that share a block of 128 (8 elements each); every lane gets it
+// max over the 16 lanes that share a block of 128 (8 elements each), by rotations within a row of lanes; every lane gets it.  NaN is left out.
 __device__ __forceinline__ float max16(float v) {
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 16));
-    return v;
+    v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x128, 0xf, 0xf, true)));
+    v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x124, 0xf, 0xf, true)));
+    v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x122, 0xf, 0xf, true)));
+    return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x121, 0xf, 0xf, true)));
 }
 
 // the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept

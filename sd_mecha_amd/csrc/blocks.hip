@@ -78,8 +78,6 @@ __device__ __forceinline__ int exponent_of_mag(uint32_t m) {
     else if constexpr (DT == MECHA_BF16) return block_exponent(__uint_as_float(m << 16));
     else return block_exponent(f16_bits_to_f32(m));
 }
-// 2^e as the conversions take it: only the exponent's byte counts, 0 being 2^-127
-__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // codes of two elements into half `HI` of r
 template <int DT, bool HI>
 __device__ __forceinline__ s16x2 codes2(s16x2 r, uint32_t lo, uint32_t hi, float scale) {     // 16-bit types: both elements in lo
@@ -145,7 +143,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
         m = one_mag<DT>(mag8<DT>(v));
     }
     const int e = exponent_of_mag<DT>(max_mag16<DT>(m));
-    u32x2 codes = codes8<DT>(v, scale_of(e));
+    u32x2 codes = codes8<DT>(v, scale_bits(e + 127));
     if (nan) codes = with_nan(codes, nan);
     *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = codes;
     if (l == 0) p.s[row * p.s_pitch + kb] = (uint8_t)(e + 127);
@@ -251,7 +249,7 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
     if (p.q) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            u32x2 codes = codes8<DT>(v[i], scale_of(re[i]));
+            u32x2 codes = codes8<DT>(v[i], scale_bits(re[i] + 127));
             if (bad) codes = with_nan(codes, nan[i >> 2] >> (8 * (i & 3)));
             if (row0 + i < p.rows) *reinterpret_cast<u32x2 *>(p.q + (row0 + i) * p.q_pitch + c) = codes;
         }
@@ -259,7 +257,7 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
     if (p.qt) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float scale = scale_of(ce[j]);
+            const float scale = scale_bits(ce[j] + 127);
             u32x2 codes;
 #pragma unroll
             for (int h = 0; h < 2; h++) {

@@ -82,7 +82,7 @@ def adamw(p, g, m, v, t, lr, b1, b2, eps, decay, coef=1.0):
     # roundings of u each: m: the constants, both products, the sum, g's own; v: the same and the square
     em = U * (4 * np.abs(b1 * m) + 5 * np.abs((1 - b1) * g)) * 1.01
     ev = U * 7 * v2 * 1.01
-    # root: half of v's and its own; denominator: root, the constant, product, sum; quotient, constant, product: 13 in all; p: constant's
-    # three, product, sum of both terms
-    ep = (5 * U * np.abs(p) + size * (em + 13 * U * np.abs(m2)) / den + 2 * U * np.abs(size * m2 / den)) * 1.01
+    # in units of u: root: half of v's 7 and 2 of its own (one unit in the last place); denominator: root, the constant, product, sum;
+    # reciprocal 2, product, constant, product: 13.5 in all; p: constant's three, product, sum of both terms
+    ep = (5 * U * np.abs(p) + size * (em + 13.5 * U * np.abs(m2)) / den + 2 * U * np.abs(size * m2 / den)) * 1.01
     return p2, m2, v2, ep, em, ev

@@ -140,6 +140,27 @@ def test_8bit_roots_never_vanish_and_zeros_stay():
     assert bool(p.isfinite().all()) and float(p.abs().max()) < 1e-2 and not p[100:].any()
 
 
+def test_8bit_codes_between_the_keys():
+    """A key's last block of 128 is written whole, zeros behind its last element; blocks that no key reaches into stay as they were."""
+    import sd_mecha_amd as amd
+    offsets, numels, n = [0, 640, 1024], [130, 1, 384], 1536
+    seg = torch.tensor([[o, c] for o, c in zip(offsets, numels)], device="cuda")
+    st = amd.adamw_state(n, "cuda", 8)
+    for t in st.values():
+        t.view(torch.uint8).fill_(0x51)
+    p, g = torch.full((n,), 5.0, device="cuda"), torch.ones(n, device="cuda")
+    amd.adamw_step(p, g, segments=seg, step=1, **st)
+    used, keys = torch.zeros(n, dtype=torch.bool), torch.zeros(n, dtype=torch.bool)
+    for o, c in zip(offsets, numels):
+        used[o:o + (c + 127) // 128 * 128] = True
+        keys[o:o + c] = True
+    for name in ("exp_avg", "exp_avg_sq"):
+        codes, scales = st[name].view(torch.uint8).cpu(), st[f"{name}_scales"].view(torch.uint8).cpu()
+        assert bool((codes[~used] == 0x51).all()) and bool((scales[~used[::128]] == 0x51).all())
+        assert not codes[used & ~keys].any() and bool((codes[keys] != 0).all())
+    assert bool((p.cpu()[~keys] == 5.0).all())
+
+
 def test_8bit_second_moment_decays_like_float32():
     """Without gradients the root shrinks by sqrt(beta2) a step.  Rounded to nearest it would never move; here its mean over a key follows."""
     import sd_mecha_amd as amd
