@@ -442,51 +442,69 @@ int64_t mecha_host_parse_safetensors_header(const char *json, int64_t len, int64
                                             int32_t *dtype_code, int32_t *ndim, int64_t *shape, int64_t *offsets, int64_t *metadata_span);
 
 /* ------------------------------------------------------------------ 8-bit weights
- * A block-scaled matrix: e4m3 codes [rows][pitch bytes] (16-byte aligned; `pitch` a multiple of 128, at least the columns rounded up to 128, and
- * all of that readable in every row) and a scale for each block of 128: `tile` == 0: scales [rows][ceil(cols / 128)], one for 128
- * columns of a row; `tile` != 0: scales [ceil(rows / 128)][ceil(cols / 128)], one for a 128 x 128 square.  `scale_pitch`: scales from one
- * row of them to the next.  value = code * scale.  Scales are float32 or a power of two in one byte, 2^(byte - 127) (255: NaN).
+ * A block-scaled matrix (the struct is the HOST's, what it points to the DEVICE's): e4m3 codes [rows][pitch bytes], 16-byte aligned, `pitch` a
+ * multiple of 128, at least the columns rounded up to 128, and all of that readable in every row; and a scale for each block of 128:
+ * `tile` == 0: scales [rows][ceil(cols / 128)], one for 128 columns of a row; `tile` != 0: scales [ceil(rows / 128)][ceil(cols / 128)], one
+ * for a 128 x 128 square.  `scale_pitch`: scales from one row of them to the next.  value = code * scale.  Scales are float32 or a
+ * power of two in one byte, 2^(byte - 127) (255: NaN).
  * No counterpart in the reference, which keeps keys in 16 and 32 bits (streaming.py:395-425). */
 #define MECHA_SCALE_BLOCK 128
 #define MECHA_SCALE_F32 0
 #define MECHA_SCALE_E8M0 1
+typedef struct mecha_block_matrix {
+    void *codes;
+    void *scales;
+    int64_t rows;
+    int64_t cols;
+    int64_t pitch;
+    int64_t scale_pitch;
+    int32_t tile;
+    int32_t scale_dtype;
+} mecha_block_matrix;
 
-/* A matrix [rows][cols] with `row_stride` elements from row to row into codes with power-of-two scales: the smallest 2^e with
+/* A matrix of `in_dtype`, `row_stride` elements from row to row, into codes with power-of-two scales: the smallest 2^e with
  * max|x| <= 448 * 2^e (e >= -127), codes to nearest even; the bytes of a row behind the last column, up to a multiple of 128, become 0.
- * `codes` / `codes_t` (either may be NULL): of the matrix, and of its transpose [cols][rows] -- with tile == 0 the latter has scales
- * of its own, for 128 original rows of one column.  inf and NaN become the NaN code, take no part in a scale, and set bit 0 of flags. */
-int mecha_cast_blocks(const void *a, int64_t rows, int64_t cols, int64_t row_stride, int in_dtype, int tile, void *codes, int64_t pitch,
-                      void *scales, int64_t scale_pitch, void *codes_t, int64_t pitch_t, void *scales_t, int64_t scale_pitch_t,
+ * `straight` [rows][cols] / `transposed` [cols][rows] (either may be NULL, their scales MECHA_SCALE_E8M0 and both of the same `tile`): where the
+ * codes go of the matrix, and of its transpose -- with tile == 0 that has scales of its own, for 128 original rows of one column.  inf and
+ * NaN become the NaN code, take no part in a scale, and set bit 0 of flags. */
+int mecha_cast_blocks(const void *a, int64_t row_stride, int in_dtype, const mecha_block_matrix *straight, const mecha_block_matrix *transposed,
                       uint32_t *flags, void *stream);
-/* codes * scales in float32, then rounded to out_dtype; out is contiguous [rows][cols].  NaN codes and non-finite scales set bit 0 of flags. */
-int mecha_uncast_blocks(const void *codes, int64_t pitch, const void *scales, int64_t scale_pitch, int scale_dtype, int tile, int64_t rows,
-                        int64_t cols, void *out, int out_dtype, uint32_t *flags, void *stream);
+/* codes * scales in float32, then rounded to out_dtype; out is contiguous [rows][cols].  NaN codes and non-finite scales set bit 0 of
+ * flags, non-finite results bit 1. */
+int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, uint32_t *flags, void *stream);
 
-/* out[m][n] = base[m][n] + alpha * sum_k a[m][k] b[n][k], a and b block-scaled along k, both with scales of `scale_dtype`; base (may be
- * NULL: zeros) and out contiguous, out may be base.  Sums in float32, one rounding to out_dtype; for a 16-bit
- * out_dtype the products of 8 neighbouring k are first cut off under 2^-13 of the largest of them (the 8-bit matrix instructions).  bit 0 of flags: a NaN came out or
- * base holds inf / NaN; bit 1: an output is inf / NaN. */
-int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, int64_t a_scale_pitch, int a_tile, const void *b, int64_t b_pitch,
-                        const void *b_scales, int64_t b_scale_pitch, int b_tile, int scale_dtype, const void *base, void *out, int64_t m,
-                        int64_t n, int64_t k, int base_dtype, int out_dtype, float alpha, uint32_t *flags, void *stream);
+/* out[m][n] = base[m][n] + alpha * sum_k a[m][k] b[n][k], a and b block-scaled along k, both with scales of one type; base (may be
+ * NULL: zeros) and out contiguous, out may be base.  Sums in float32, one rounding to out_dtype; for a 16-bit out_dtype the products of 8
+ * neighbouring k are first cut off under 2^-13 of the largest of them (the 8-bit matrix instructions).  bit 0 of flags: a NaN came out
+ * or base holds inf / NaN; bit 1: an output is inf / NaN. */
+int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
+                        float alpha, uint32_t *flags, void *stream);
 
 /* ------------------------------------------------------------------ training step
  * One AdamW step (decoupled weight decay) for every key of the arenas, in place, in one launch:
  *   g = grad * clip;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p = p (1 - lr * decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  t = step (from 1)
- * in float32.  param / grad / copy arenas in any of the three dtypes; copy_arena (may be NULL) receives the new weights once more.
- * state_bits 32: exp_avg = m, exp_avg_sq = v, float32.  state_bits 8: exp_avg = e4m3 codes of m, exp_avg_sq = e4m3 codes of sqrt(v), with
- * power-of-two scales [total_elems / 128] in *_scales; segment offsets and total_elems must be multiples of 128, and the codes
- * behind a key's last element, up to a multiple of 128, become 0.  The codes are rounded up or down by a hash of (offset, step, seed).
- * Elements outside the segments are left as they are.  key_weight_decay (may be NULL: weight_decay for all): DEVICE float[n_segments].
- * step_dev (may be NULL): DEVICE int64, read instead of `step` when the kernel runs (for captured graphs).  clip (may be NULL): DEVICE
- * float[2] of mecha_batched_grad_norm; if its coefficient is NaN the step changes nothing.
- * seg_flags: bit 0: a gradient or weight was inf / NaN, bit 1: a new weight is. */
-int mecha_batched_adamw(void *param_arena, const void *grad_arena, void *exp_avg, void *exp_avg_sq, void *exp_avg_scales,
-                        void *exp_avg_sq_scales, void *copy_arena, const mecha_segment *segments, int n_segments, int64_t total_elems,
-                        int param_dtype, int grad_dtype, int copy_dtype, int state_bits, double lr, double beta1, double beta2, double eps,
-                        double weight_decay, const float *key_weight_decay, int64_t step, const int64_t *step_dev, uint32_t seed,
-                        const float *clip, uint32_t *seg_flags, void *stream);
+ * in float32.  The struct is the HOST's, what it points to the DEVICE's. */
+typedef struct mecha_adamw {
+    void *params;                     /* arenas in any of the three dtypes */
+    const void *grads;
+    void *exp_avg;                    /* state_bits 32: m and v, float32; 8: e4m3 codes of m and of sqrt(v), 8-byte aligned, with */
+    void *exp_avg_sq;                 /*   power-of-two scales [total_elems / 128] in *_scales; the codes are rounded up or down by a hash */
+    void *exp_avg_scales;             /*   of (offset, step, seed).  Segment offsets and total_elems are multiples of 128 then, and the */
+    void *exp_avg_sq_scales;          /*   codes behind a key's last element, up to a multiple of 128, become 0 */
+    void *copy;                       /* arena that receives the new weights once more, may be NULL */
+    const mecha_segment *segments;    /* sorted; elements outside them are left as they are */
+    const float *key_weight_decay;    /* float[n_segments], may be NULL: weight_decay for all */
+    const int64_t *step_dev;          /* read instead of `step` when the kernel runs (for captured graphs), may be NULL */
+    const float *clip;                /* float[2] of mecha_batched_grad_norm, may be NULL; with a NaN coefficient the step changes nothing */
+    uint32_t *seg_flags;              /* uint32[n_segments], may be NULL: bit 0: a gradient or weight was inf / NaN, bit 1: a new weight is */
+    int64_t total_elems;
+    int64_t step;
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t n_segments, param_dtype, grad_dtype, copy_dtype, state_bits;
+    uint32_t seed;
+} mecha_adamw;
+int mecha_batched_adamw(const mecha_adamw *args, void *stream);
 /* norm_out (DEVICE float[2]) = [2-norm of every key's gradient together, min(1, max_norm / (norm + 1e-6))], the second NaN if the norm is
  * not finite.  Sums in float64, in the same order every time. */
 size_t mecha_batched_grad_norm_workspace_bytes(int64_t total_elems);

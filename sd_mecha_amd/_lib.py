@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 
 _HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libmecha_hip.so"
@@ -37,14 +38,19 @@ class LoraNet(ctypes.Structure):
                 ("weight", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
+# mecha_block_matrix and mecha_adamw as packed bytes (a call passes them by address; packing takes a tenth of filling a ctypes structure)
+BLOCK_MATRIX = struct.Struct("=QQqqqqii")
+ADAMW = struct.Struct("=12Q2q5d5iI")
+
+
 class MechaError(RuntimeError):
     """A libmecha_hip entry point returned a negative status."""
 
 
 _lib = None
 
-c_p, c_i, c_i64, c_f, c_d, c_sz, c_u64, c_u32 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
-                                                 ctypes.c_double, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_uint32)
+c_p, c_i, c_i64, c_f, c_d, c_sz, c_u64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
+                                          ctypes.c_double, ctypes.c_size_t, ctypes.c_uint64)
 
 # name -> (restype, argtypes); every symbol include/mecha_hip.h declares
 SIGNATURES = {
@@ -110,12 +116,10 @@ SIGNATURES = {
     "mecha_batched_ties_workspace_bytes": (c_sz, [c_i, c_i, c_i64]),
     "mecha_batched_add_difference_ties": (c_i, [c_p, c_p, c_i, c_p, c_p, c_p, c_i, c_i64, c_i, c_i, c_d, c_f, c_i,
                                                 c_p, c_p, c_sz, c_p, c_p]),
-    "mecha_cast_blocks": (c_i, [c_p, c_i64, c_i64, c_i64, c_i, c_i, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p]),
-    "mecha_uncast_blocks": (c_i, [c_p, c_i64, c_p, c_i64, c_i, c_i, c_i64, c_i64, c_p, c_i, c_p, c_p]),
-    "mecha_block_product": (c_i, [c_p, c_i64, c_p, c_i64, c_i, c_p, c_i64, c_p, c_i64, c_i, c_i, c_p, c_p, c_i64, c_i64, c_i64, c_i, c_i, c_f,
-                                  c_p, c_p]),
-    "mecha_batched_adamw": (c_i, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_i64, c_i, c_i, c_i, c_i, c_d, c_d, c_d, c_d, c_d, c_p, c_i64, c_p,
-                                  c_u32, c_p, c_p, c_p]),
+    "mecha_cast_blocks": (c_i, [c_p, c_i64, c_i, c_p, c_p, c_p, c_p]),
+    "mecha_uncast_blocks": (c_i, [c_p, c_p, c_i, c_p, c_p]),
+    "mecha_block_product": (c_i, [c_p, c_p, c_p, c_i, c_p, c_i, c_f, c_p, c_p]),
+    "mecha_batched_adamw": (c_i, [c_p, c_p]),
     "mecha_batched_grad_norm_workspace_bytes": (c_sz, [c_i64]),
     "mecha_batched_grad_norm": (c_i, [c_p, c_p, c_i, c_i64, c_i, c_d, c_p, c_p, c_sz, c_p]),
 }

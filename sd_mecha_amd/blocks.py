@@ -41,7 +41,7 @@ class BlockScaled:
 
     The kernels read rows in whole blocks of 128 bytes: ``cast_blocks`` lays rows a multiple of 128 bytes apart (``pitch``), with zeros
     behind the last column.  Values that lie otherwise (a stored tensor whose columns are no multiple of 128) are laid out so here, once."""
-    __slots__ = ("values", "scales", "rows", "cols", "tile", "pitch", "scale_pitch", "scale_code")
+    __slots__ = ("values", "scales", "rows", "cols", "tile", "pitch", "scale_pitch", "scale_code", "_packed")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor):
@@ -74,6 +74,7 @@ class BlockScaled:
 
     def _set(self, *of):
         self.values, self.scales, self.rows, self.cols, self.tile, self.pitch, self.scale_pitch, self.scale_code = of
+        self._packed = _lib.BLOCK_MATRIX.pack(self.values.data_ptr(), self.scales.data_ptr(), *of[2:4], *of[5:7], of[4], of[7])
 
     @property
     def shape(self) -> torch.Size:
@@ -91,7 +92,7 @@ def _empty(rows: int, cols: int, tile: bool, device) -> BlockScaled:
     s_rows = _blocks(rows) if tile else rows
     q = BlockScaled.__new__(BlockScaled)
     q._set(codes if cols == width else codes[:, :cols], torch.empty((s_rows, s_cols), dtype=torch.float8_e8m0fnu, device=device), rows, cols,
-           s_rows != rows, width, s_cols, SCALE_E8M0)
+           tile, width, s_cols, SCALE_E8M0)
     return q
 
 
@@ -140,11 +141,8 @@ def cast_blocks(a, *, tile: bool = False, sides: str = "straight", key=None, fla
     if rows and cols:
         with _on(device):
             word, fl = _flags(device, flags, check_finite)
-            _lib.check(_lib.lib().mecha_cast_blocks(
-                a.data_ptr(), rows, cols, stride, _DT[a.dtype], tile,
-                *((q.values.data_ptr(), q.pitch, q.scales.data_ptr(), q.scale_pitch) if q is not None else (None, 0, None, 0)),
-                *((qt.values.data_ptr(), qt.pitch, qt.scales.data_ptr(), qt.scale_pitch) if qt is not None else (None, 0, None, 0)),
-                word, _stream(device)), "mecha_cast_blocks")
+            _lib.check(_lib.lib().mecha_cast_blocks(a.data_ptr(), stride, _DT[a.dtype], q._packed if q is not None else None,
+                                                    qt._packed if qt is not None else None, word, _stream(device)), "mecha_cast_blocks")
             if fl is not None:
                 fl.finish(key)
     return q if qt is None else qt if q is None else (q, qt)
@@ -161,8 +159,7 @@ def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check
     if rows and cols:
         with _on(device):
             word, fl = _flags(device, flags, check_finite)
-            _lib.check(_lib.lib().mecha_uncast_blocks(q.values.data_ptr(), q.pitch, q.scales.data_ptr(), q.scale_pitch, q.scale_code, q.tile,
-                                                      rows, cols, out.data_ptr(), _DT[dtype], word, _stream(device)), "mecha_uncast_blocks")
+            _lib.check(_lib.lib().mecha_uncast_blocks(q._packed, out.data_ptr(), _DT[dtype], word, _stream(device)), "mecha_uncast_blocks")
             if fl is not None:
                 fl.finish(key)
     return out
@@ -210,16 +207,12 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         return out
     if k == 0:
         return out.zero_() if base is None else out if out is base else out.copy_(cast(base, out.dtype, key=key, flags=flags, check_finite=check_finite))
-    sa, sb, code = a.scales, b.scales, a.scale_code
-    sa_pitch, sb_pitch = a.scale_pitch, b.scale_pitch
-    if code != b.scale_code:
-        sa, sb, code = sa.to(torch.float32).contiguous(), sb.to(torch.float32).contiguous(), SCALE_F32
-        sa_pitch, sb_pitch = sa.shape[1], sb.shape[1]
+    if a.scale_code != b.scale_code:
+        a, b = (q if q.scale_code == SCALE_F32 else BlockScaled(q.values, q.scales.to(torch.float32)) for q in (a, b))
     with _on(device):
         word, fl = _flags(device, flags, check_finite)
         _lib.check(_lib.lib().mecha_block_product(
-            a.values.data_ptr(), a.pitch, sa.data_ptr(), sa_pitch, a.tile, b.values.data_ptr(), b.pitch, sb.data_ptr(), sb_pitch, b.tile, code,
-            base.data_ptr() if base is not None else None, out.data_ptr(), m, n, k, _DT[base.dtype] if base is not None else _lib.F32,
+            a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),
             _DT[out.dtype], alpha, word, _stream(device)), "mecha_block_product")
         if fl is not None:
             fl.finish(key)

@@ -125,7 +125,7 @@ __device__ __forceinline__ uint32_t dither32(int64_t i, uint32_t key) {
     x *= 0xBB67AE85u;
     return x ^ (x >> 16);
 }
-__device__ __forceinline__ uint32_t dither_key(uint32_t step, uint32_t seed) { return step * 0x3C6EF373u + seed * 0x6A09E667u; }
+__host__ __device__ __forceinline__ uint32_t dither_key(uint32_t step, uint32_t seed) { return step * 0x3C6EF373u + seed * 0x6A09E667u; }
 
 template <int P_DT, int G_DT, bool BITS8, bool VEC>
 __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
@@ -407,50 +407,48 @@ int mecha_batched_grad_norm(const void *grad_arena, const mecha_segment *segment
     return MECHA_OK;
 }
 
-int mecha_batched_adamw(void *param_arena, const void *grad_arena, void *exp_avg, void *exp_avg_sq, void *exp_avg_scales,
-                        void *exp_avg_sq_scales, void *copy_arena, const mecha_segment *segments, int n_segments, int64_t total_elems,
-                        int param_dtype, int grad_dtype, int copy_dtype, int state_bits, double lr, double beta1, double beta2, double eps,
-                        double weight_decay, const float *key_weight_decay, int64_t step, const int64_t *step_dev, uint32_t seed,
-                        const float *clip, uint32_t *seg_flags, void *stream) {
-    const int st = check_arena(segments, n_segments, total_elems);
+int mecha_batched_adamw(const mecha_adamw *args, void *stream) {
+    MECHA_REQUIRE(args != nullptr, "no arguments");
+    const mecha_adamw &x = *args;
+    const int st = check_arena(x.segments, x.n_segments, x.total_elems);
     if (st) return st;
-    MECHA_REQUIRE(mecha_valid_dtype(param_dtype) && mecha_valid_dtype(grad_dtype) && (copy_arena == nullptr || mecha_valid_dtype(copy_dtype)),
-                  "unknown dtype code (param %d, grad %d, copy %d)", param_dtype, grad_dtype, copy_dtype);
-    MECHA_REQUIRE(state_bits == 32 || state_bits == 8, "states are held in 32 or 8 bits (got %d)", state_bits);
-    MECHA_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "betas must be in [0, 1) (got %g, %g)", beta1, beta2);
-    MECHA_REQUIRE(eps >= 0.0 && lr >= 0.0, "lr and eps must be >= 0 (got %g, %g)", lr, eps);
-    MECHA_REQUIRE(step_dev != nullptr || step >= 1, "steps count from 1 (got %lld)", (long long)step);
-    if (total_elems == 0) return MECHA_OK;
-    MECHA_REQUIRE(param_arena && grad_arena && exp_avg && exp_avg_sq, "an arena is NULL");
-    if (state_bits == 8) {
-        MECHA_REQUIRE(exp_avg_scales && exp_avg_sq_scales, "8-bit states need their scales");
-        MECHA_REQUIRE(total_elems % SCALE_BLOCK == 0, "8-bit states: total_elems %lld must be a multiple of 128", (long long)total_elems);
-        MECHA_REQUIRE((reinterpret_cast<uintptr_t>(exp_avg) & 7u) == 0 && (reinterpret_cast<uintptr_t>(exp_avg_sq) & 7u) == 0, "8-bit states must be 8-byte aligned");
+    MECHA_REQUIRE(mecha_valid_dtype(x.param_dtype) && mecha_valid_dtype(x.grad_dtype) && (x.copy == nullptr || mecha_valid_dtype(x.copy_dtype)),
+                  "unknown dtype code (param %d, grad %d, copy %d)", x.param_dtype, x.grad_dtype, x.copy_dtype);
+    MECHA_REQUIRE(x.state_bits == 32 || x.state_bits == 8, "states are held in 32 or 8 bits (got %d)", x.state_bits);
+    MECHA_REQUIRE(x.beta1 >= 0.0 && x.beta1 < 1.0 && x.beta2 >= 0.0 && x.beta2 < 1.0, "betas must be in [0, 1) (got %g, %g)", x.beta1, x.beta2);
+    MECHA_REQUIRE(x.eps >= 0.0 && x.lr >= 0.0, "lr and eps must be >= 0 (got %g, %g)", x.lr, x.eps);
+    MECHA_REQUIRE(x.step_dev != nullptr || x.step >= 1, "steps count from 1 (got %lld)", (long long)x.step);
+    if (x.total_elems == 0) return MECHA_OK;
+    MECHA_REQUIRE(x.params && x.grads && x.exp_avg && x.exp_avg_sq, "an arena is NULL");
+    if (x.state_bits == 8) {
+        MECHA_REQUIRE(x.exp_avg_scales && x.exp_avg_sq_scales, "8-bit states need their scales");
+        MECHA_REQUIRE(x.total_elems % SCALE_BLOCK == 0, "8-bit states: total_elems %lld must be a multiple of 128", (long long)x.total_elems);
+        MECHA_REQUIRE((reinterpret_cast<uintptr_t>(x.exp_avg) & 7u) == 0 && (reinterpret_cast<uintptr_t>(x.exp_avg_sq) & 7u) == 0, "8-bit states must be 8-byte aligned");
     }
     AdamParams a{};
-    a.p = param_arena; a.g = grad_arena; a.m = exp_avg; a.v = exp_avg_sq;
-    a.ms = static_cast<uint8_t *>(exp_avg_scales); a.vs = static_cast<uint8_t *>(exp_avg_sq_scales);
-    a.copy = copy_arena; a.copy_dt = copy_dtype;
-    a.segs = segments; a.n_segs = n_segments; a.total = total_elems;
-    a.decay = key_weight_decay; a.decay_all = (float)weight_decay;
-    a.lr = (float)lr; a.b1 = (float)beta1; a.b2 = (float)beta2; a.c1 = (float)(1.0 - beta1); a.c2 = (float)(1.0 - beta2); a.eps = (float)eps;
-    a.lrd = lr; a.b1d = beta1; a.b2d = beta2; a.seed = seed; a.step_dev = step_dev; a.clip = clip; a.seg_flags = seg_flags;
-    if (step_dev == nullptr) {
-        a.size = (float)(lr / (1.0 - pow(beta1, (double)step)));
-        a.root_size = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-        a.key = (uint32_t)step * 0x3C6EF373u + seed * 0x6A09E667u;
+    a.p = x.params; a.g = x.grads; a.m = x.exp_avg; a.v = x.exp_avg_sq;
+    a.ms = static_cast<uint8_t *>(x.exp_avg_scales); a.vs = static_cast<uint8_t *>(x.exp_avg_sq_scales);
+    a.copy = x.copy; a.copy_dt = x.copy_dtype;
+    a.segs = x.segments; a.n_segs = x.n_segments; a.total = x.total_elems;
+    a.decay = x.key_weight_decay; a.decay_all = (float)x.weight_decay;
+    a.lr = (float)x.lr; a.b1 = (float)x.beta1; a.b2 = (float)x.beta2; a.c1 = (float)(1.0 - x.beta1); a.c2 = (float)(1.0 - x.beta2); a.eps = (float)x.eps;
+    a.lrd = x.lr; a.b1d = x.beta1; a.b2d = x.beta2; a.seed = x.seed; a.step_dev = x.step_dev; a.clip = x.clip; a.seg_flags = x.seg_flags;
+    if (x.step_dev == nullptr) {
+        a.size = (float)(x.lr / (1.0 - pow(x.beta1, (double)x.step)));
+        a.root_size = (float)(1.0 / sqrt(1.0 - pow(x.beta2, (double)x.step)));
+        a.key = dither_key((uint32_t)x.step, x.seed);
     }
-    const bool vec = mecha_aligned16(param_arena) && mecha_aligned16(grad_arena) && (state_bits == 8 || (mecha_aligned16(exp_avg) && mecha_aligned16(exp_avg_sq)))
-                     && (copy_arena == nullptr || mecha_aligned16(copy_arena));
-    const int64_t each = (state_bits == 8 ? 8 : 4) * MECHA_BLOCK, blocks = (total_elems + each - 1) / each;
+    const bool vec = mecha_aligned16(x.params) && mecha_aligned16(x.grads) && (x.state_bits == 8 || (mecha_aligned16(x.exp_avg) && mecha_aligned16(x.exp_avg_sq)))
+                     && (x.copy == nullptr || mecha_aligned16(x.copy));
+    const int64_t each = (x.state_bits == 8 ? 8 : 4) * MECHA_BLOCK, blocks = (x.total_elems + each - 1) / each;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    with_dtype(param_dtype, [&](auto pd) {
-        with_dtype(grad_dtype, [&](auto gd) {
+    with_dtype(x.param_dtype, [&](auto pd) {
+        with_dtype(x.grad_dtype, [&](auto gd) {
             auto go = [&](auto b8, auto v) {
                 MECHA_LAUNCH(MK_ADAMW, (adamw_kernel<decltype(pd)::value, decltype(gd)::value, decltype(b8)::value, decltype(v)::value>),
                              dim3((unsigned)blocks), dim3(MECHA_BLOCK), 0, s, a);
             };
-            if (state_bits == 8) { if (vec) go(std::true_type{}, std::true_type{}); else go(std::true_type{}, std::false_type{}); }
+            if (x.state_bits == 8) { if (vec) go(std::true_type{}, std::true_type{}); else go(std::true_type{}, std::false_type{}); }
             else { if (vec) go(std::false_type{}, std::true_type{}); else go(std::false_type{}, std::false_type{}); }
         });
     });

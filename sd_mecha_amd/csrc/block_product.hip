@@ -939,23 +939,25 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
 
 extern "C" {
 
-int mecha_block_product(const void *a, int64_t a_pitch, const void *a_scales, int64_t a_scale_pitch, int a_tile, const void *b, int64_t b_pitch,
-                        const void *b_scales, int64_t b_scale_pitch, int b_tile, int scale_dtype, const void *base, void *out, int64_t m,
-                        int64_t n, int64_t k, int base_dtype, int out_dtype, float alpha, uint32_t *flags, void *stream) {
-    MECHA_REQUIRE(m >= 0 && n >= 0 && k >= 1, "bad product: %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
+int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
+                        float alpha, uint32_t *flags, void *stream) {
+    MECHA_REQUIRE(a != nullptr && b != nullptr, "a matrix is NULL");
     MECHA_REQUIRE(mecha_valid_dtype(out_dtype) && (base == nullptr || mecha_valid_dtype(base_dtype)), "unknown dtype code (base %d, out %d)", base_dtype, out_dtype);
-    MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
+    int st = mecha_check_blocks("a", *a);
+    if (st) return st;
+    st = mecha_check_blocks("b", *b);
+    if (st) return st;
+    MECHA_REQUIRE(a->scale_dtype == b->scale_dtype, "scales of two types (%d, %d)", a->scale_dtype, b->scale_dtype);
+    const int64_t m = a->rows, n = b->rows, k = a->cols;
+    MECHA_REQUIRE(k >= 1 && b->cols == k, "a has %lld columns, b %lld: they must be the same, and some", (long long)k, (long long)b->cols);
     if (m == 0 || n == 0) return MECHA_OK;
     MECHA_REQUIRE(out != nullptr, "out is NULL");
-    int st = mecha_check_blocks("a", a, m, k, a_pitch, a_scales, a_scale_pitch);
-    if (st) return st;
-    st = mecha_check_blocks("b", b, n, k, b_pitch, b_scales, b_scale_pitch);
-    if (st) return st;
-    MECHA_REQUIRE(a_pitch <= (1 << 24) && b_pitch <= (1 << 24), "rows of more than 2^24 bytes (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
+    MECHA_REQUIRE(a->pitch <= (1 << 24) && b->pitch <= (1 << 24), "rows of more than 2^24 bytes (%lld, %lld)", (long long)a->pitch, (long long)b->pitch);
     const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128;
-    MECHA_REQUIRE(tm * tn < (1ll << 24), "%lld x %lld outputs are beyond one launch", (long long)m, (long long)n);
-    ProductParams p{static_cast<const uint8_t *>(a), a_pitch, a_scales, a_scale_pitch, a_tile, static_cast<const uint8_t *>(b), b_pitch, b_scales,
-                    b_scale_pitch, b_tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
+    MECHA_REQUIRE(m < (1ll << 31) && n < (1ll << 31) && tm * tn < (1ll << 24), "%lld x %lld outputs are beyond one launch", (long long)m, (long long)n);
+    ProductParams p{static_cast<const uint8_t *>(a->codes), a->pitch, a->scales, a->scale_pitch, a->tile, static_cast<const uint8_t *>(b->codes), b->pitch,
+                    b->scales, b->scale_pitch, b->tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
+    const int b_tile = b->tile, scale_dtype = a->scale_dtype;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
     // The large kernel stores and reads base in 16-byte pieces of the result's type, and reads scales four blocks at a time.

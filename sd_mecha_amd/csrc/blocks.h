@@ -33,12 +33,15 @@ __device__ __forceinline__ float max16(float v) {
 }
 
 // the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept
-static inline int mecha_check_blocks(const char *what, const void *q, int64_t rows, int64_t cols, int64_t pitch, const void *s, int64_t s_pitch) {
-    MECHA_REQUIRE(q != nullptr && s != nullptr, "%s: codes or scales are NULL", what);
-    MECHA_REQUIRE(mecha_aligned16(q), "%s: codes must be 16-byte aligned", what);
-    MECHA_REQUIRE(pitch % SCALE_BLOCK == 0 && pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK,
-                  "%s: the row pitch %lld must be a multiple of 128 and hold %lld columns rounded up to 128", what, (long long)pitch, (long long)cols);
-    MECHA_REQUIRE(s_pitch >= (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, "%s: a row of scales holds %lld, %lld are needed", what, (long long)s_pitch,
-                  (long long)((cols + SCALE_BLOCK - 1) / SCALE_BLOCK));
+static inline int mecha_check_blocks(const char *what, const mecha_block_matrix &q) {
+    const int64_t blocks = (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK;
+    MECHA_REQUIRE(q.rows >= 0 && q.cols >= 0, "%s: bad matrix %lld x %lld", what, (long long)q.rows, (long long)q.cols);
+    MECHA_REQUIRE(q.scale_dtype == MECHA_SCALE_F32 || q.scale_dtype == MECHA_SCALE_E8M0, "%s: unknown scale dtype %d", what, q.scale_dtype);
+    if (q.rows == 0 || q.cols == 0) return MECHA_OK;
+    MECHA_REQUIRE(q.codes != nullptr && q.scales != nullptr, "%s: codes or scales are NULL", what);
+    MECHA_REQUIRE(mecha_aligned16(q.codes), "%s: codes must be 16-byte aligned", what);
+    MECHA_REQUIRE(q.pitch % SCALE_BLOCK == 0 && q.pitch >= blocks * SCALE_BLOCK, "%s: the row pitch %lld must be a multiple of 128 and hold %lld columns rounded up to 128",
+                  what, (long long)q.pitch, (long long)q.cols);
+    MECHA_REQUIRE(q.scale_pitch >= blocks, "%s: a row of scales holds %lld, %lld are needed", what, (long long)q.scale_pitch, (long long)blocks);
     return MECHA_OK;
 }

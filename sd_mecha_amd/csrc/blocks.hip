@@ -329,21 +329,30 @@ __global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, i
 
 extern "C" {
 
-int mecha_cast_blocks(const void *a, int64_t rows, int64_t cols, int64_t row_stride, int in_dtype, int tile, void *codes, int64_t pitch,
-                      void *scales, int64_t scale_pitch, void *codes_t, int64_t pitch_t, void *scales_t, int64_t scale_pitch_t,
+int mecha_cast_blocks(const void *a, int64_t row_stride, int in_dtype, const mecha_block_matrix *straight, const mecha_block_matrix *transposed,
                       uint32_t *flags, void *stream) {
-    MECHA_REQUIRE(rows >= 0 && cols >= 0 && mecha_valid_dtype(in_dtype), "bad matrix: %lld x %lld, dtype %d", (long long)rows, (long long)cols, in_dtype);
-    MECHA_REQUIRE(codes != nullptr || codes_t != nullptr, "neither codes nor transposed codes are asked for");
+    MECHA_REQUIRE(straight != nullptr || transposed != nullptr, "neither codes nor transposed codes are asked for");
+    MECHA_REQUIRE(mecha_valid_dtype(in_dtype), "unknown dtype code %d", in_dtype);
+    const int64_t rows = straight ? straight->rows : transposed->cols, cols = straight ? straight->cols : transposed->rows;
+    const int tile = straight ? straight->tile : transposed->tile;
+    for (const mecha_block_matrix *q : {straight, transposed}) {
+        if (!q) continue;
+        const int st = mecha_check_blocks(q == straight ? "codes" : "transposed codes", *q);
+        if (st) return st;
+        MECHA_REQUIRE(q->scale_dtype == MECHA_SCALE_E8M0, "a cast makes power-of-two scales");
+    }
+    if (straight && transposed)
+        MECHA_REQUIRE(transposed->rows == cols && transposed->cols == rows && !transposed->tile == !tile, "the transposed matrix is %lld x %lld, not %lld x %lld of the same form",
+                      (long long)transposed->rows, (long long)transposed->cols, (long long)cols, (long long)rows);
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(a != nullptr && row_stride >= cols, "a is NULL or its rows overlap (stride %lld, %lld columns)", (long long)row_stride, (long long)cols);
-    if (codes) { const int st = mecha_check_blocks("codes", codes, rows, cols, pitch, scales, scale_pitch); if (st) return st; }
-    if (codes_t) { const int st = mecha_check_blocks("transposed codes", codes_t, cols, rows, pitch_t, scales_t, scale_pitch_t); if (st) return st; }
-    CastParams p{a, rows, cols, row_stride, static_cast<uint8_t *>(codes), pitch, static_cast<uint8_t *>(scales), scale_pitch,
-                 static_cast<uint8_t *>(codes_t), pitch_t, static_cast<uint8_t *>(scales_t), scale_pitch_t, flags};
+    CastParams p{a, rows, cols, row_stride, nullptr, 0, nullptr, 0, nullptr, 0, nullptr, 0, flags};
+    if (straight) { p.q = static_cast<uint8_t *>(straight->codes); p.q_pitch = straight->pitch; p.s = static_cast<uint8_t *>(straight->scales); p.s_pitch = straight->scale_pitch; }
+    if (transposed) { p.qt = static_cast<uint8_t *>(transposed->codes); p.qt_pitch = transposed->pitch; p.st = static_cast<uint8_t *>(transposed->scales); p.st_pitch = transposed->scale_pitch; }
     const bool vec = mecha_aligned16(a) && (row_stride * (int64_t)mecha_dtype_size(in_dtype)) % 16 == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t bc = (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, br = (rows + SCALE_BLOCK - 1) / SCALE_BLOCK;
-    const bool flat = codes_t == nullptr && !tile;
+    const bool flat = transposed == nullptr && !tile;
     const int64_t blocks = flat ? (rows * bc + MECHA_BLOCK / 16 - 1) / (MECHA_BLOCK / 16) : br * bc;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
     dim3 grid((unsigned)blocks), block(MECHA_BLOCK);
@@ -364,24 +373,23 @@ int mecha_cast_blocks(const void *a, int64_t rows, int64_t cols, int64_t row_str
     return MECHA_OK;
 }
 
-int mecha_uncast_blocks(const void *codes, int64_t pitch, const void *scales, int64_t scale_pitch, int scale_dtype, int tile, int64_t rows,
-                        int64_t cols, void *out, int out_dtype, uint32_t *flags, void *stream) {
-    MECHA_REQUIRE(rows >= 0 && cols >= 0 && mecha_valid_dtype(out_dtype), "bad matrix: %lld x %lld, dtype %d", (long long)rows, (long long)cols, out_dtype);
-    MECHA_REQUIRE(scale_dtype == MECHA_SCALE_F32 || scale_dtype == MECHA_SCALE_E8M0, "unknown scale dtype %d", scale_dtype);
+int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, uint32_t *flags, void *stream) {
+    MECHA_REQUIRE(q != nullptr && mecha_valid_dtype(out_dtype), "no matrix, or unknown dtype code %d", out_dtype);
+    const int st = mecha_check_blocks("codes", *q);
+    if (st) return st;
+    const int64_t rows = q->rows, cols = q->cols;
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(out != nullptr, "out is NULL");
-    const int st = mecha_check_blocks("codes", codes, rows, cols, pitch, scales, scale_pitch);
-    if (st) return st;
     const int64_t vec_per_row = (cols + 7) / 8, blocks = (rows * vec_per_row + MECHA_BLOCK - 1) / MECHA_BLOCK;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
     const bool vec = mecha_aligned16(out) && (cols * (int64_t)mecha_dtype_size(out_dtype)) % 16 == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto dt, auto e8, auto v) {
         MECHA_LAUNCH(MK_BLOCKS_CAST, (uncast_kernel<decltype(dt)::value, decltype(e8)::value, decltype(v)::value>), dim3((unsigned)blocks), dim3(MECHA_BLOCK), 0, s,
-                     static_cast<const uint8_t *>(codes), pitch, scales, scale_pitch, tile, rows, cols, vec_per_row, out, flags);
+                     static_cast<const uint8_t *>(q->codes), q->pitch, q->scales, q->scale_pitch, q->tile, rows, cols, vec_per_row, out, flags);
     };
     auto with_vec = [&](auto dt, auto e8) { if (vec) go(dt, e8, std::true_type{}); else go(dt, e8, std::false_type{}); };
-    auto with_scale = [&](auto dt) { if (scale_dtype == MECHA_SCALE_E8M0) with_vec(dt, std::true_type{}); else with_vec(dt, std::false_type{}); };
+    auto with_scale = [&](auto dt) { if (q->scale_dtype == MECHA_SCALE_E8M0) with_vec(dt, std::true_type{}); else with_vec(dt, std::false_type{}); };
     switch (out_dtype) {
         case MECHA_F32: with_scale(std::integral_constant<int, MECHA_F32>{}); break;
         case MECHA_F16: with_scale(std::integral_constant<int, MECHA_F16>{}); break;

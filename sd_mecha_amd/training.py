@@ -3,7 +3,7 @@
 reference, which merges checkpoints and does not train them."""
 from __future__ import annotations
 
-from typing import Optional, Sequence, Union
+from typing import Optional, Union
 
 import torch
 
@@ -30,13 +30,16 @@ def adamw_state(total_elems: Union[int, ArenaLayout], device, bits: int = 32) ->
     return state
 
 
-def _arena(t, name: str, dtypes: Sequence[torch.dtype], n: int, device) -> None:
+def _arena(t, name: str, dtypes, n: int, device) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"adamw_step: {name} is {type(t).__name__}, expected a torch.Tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"adamw_step: {name} is of {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != 1 or t.numel() != n or t.device != device or not t.is_contiguous():
+    if t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"adamw_step: {name} must be a flat tensor of {n} elements on {device}, got {tuple(t.shape)} on {t.device}")
+
+
+_F32_STATE, _CODES, _SCALES = (torch.float32,), (CODES,), (torch.float8_e8m0fnu,)
 
 
 def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, segments: torch.Tensor, *,
@@ -64,16 +67,16 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
             raise TypeError(f"adamw_step: {name} is {type(t).__name__}, expected a torch.Tensor")
     device, n = params.device, params.numel()
     bits8 = exp_avg_scales is not None or exp_avg_sq_scales is not None
-    states = (CODES,) if bits8 else (torch.float32,)
+    states = _CODES if bits8 else _F32_STATE
     for t, name, dtypes in ((params, "params", _DT), (grads, "grads", _DT), (exp_avg, "exp_avg", states), (exp_avg_sq, "exp_avg_sq", states)):
-        _arena(t, name, tuple(dtypes), n, device)
+        _arena(t, name, dtypes, n, device)
     if bits8:
         if n % SCALE_BLOCK:
             raise ValueError(f"adamw_step: an arena with 8-bit states holds a multiple of {SCALE_BLOCK} elements, got {n}")
         for t, name in ((exp_avg_scales, "exp_avg_scales"), (exp_avg_sq_scales, "exp_avg_sq_scales")):
-            _arena(t, name, (torch.float8_e8m0fnu,), n // SCALE_BLOCK, device)
+            _arena(t, name, _SCALES, n // SCALE_BLOCK, device)
     if copy is not None:
-        _arena(copy, "copy", tuple(_DT), n, device)
+        _arena(copy, "copy", _DT, n, device)
     if segments.dtype != torch.int64 or segments.dim() != 2 or segments.shape[1] != 2 or segments.device != device or not segments.is_contiguous():
         raise ValueError(f"adamw_step: segments must be the layout's device_segments: contiguous int64 [keys, 2] on {device}")
     keys = segments.shape[0]
@@ -106,12 +109,11 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
             _lib.check(L.mecha_batched_grad_norm(grads.data_ptr(), segments.data_ptr(), keys, n, _DT[grads.dtype], float(max_norm), norm.data_ptr(),
                                                  ws.data_ptr(), size, stream), "mecha_batched_grad_norm")
         on_device = isinstance(step, torch.Tensor)
-        _lib.check(L.mecha_batched_adamw(
-            params.data_ptr(), grads.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
-            exp_avg_scales.data_ptr() if bits8 else None, exp_avg_sq_scales.data_ptr() if bits8 else None,
-            copy.data_ptr() if copy is not None else None, segments.data_ptr(), keys, n, _DT[params.dtype], _DT[grads.dtype],
-            _DT[copy.dtype] if copy is not None else _lib.F32, 8 if bits8 else 32, float(lr), float(betas[0]), float(betas[1]), float(eps),
-            0.0 if per_key else float(weight_decay), weight_decay.data_ptr() if per_key else None,
-            0 if on_device else int(step), step.data_ptr() if on_device else None, int(seed) & 0xFFFFFFFF,
-            norm.data_ptr() if norm is not None else None, flags.data_ptr() if flags is not None else None, stream), "mecha_batched_adamw")
+        _lib.check(L.mecha_batched_adamw(_lib.ADAMW.pack(
+            params.data_ptr(), grads.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg_scales.data_ptr() if bits8 else 0,
+            exp_avg_sq_scales.data_ptr() if bits8 else 0, copy.data_ptr() if copy is not None else 0, segments.data_ptr(),
+            weight_decay.data_ptr() if per_key else 0, step.data_ptr() if on_device else 0, norm.data_ptr() if norm is not None else 0,
+            flags.data_ptr() if flags is not None else 0, n, 0 if on_device else int(step), lr, betas[0], betas[1], eps,
+            0.0 if per_key else weight_decay, keys, _DT[params.dtype], _DT[grads.dtype], _DT[copy.dtype] if copy is not None else _lib.F32,
+            8 if bits8 else 32, int(seed) & 0xFFFFFFFF), stream), "mecha_batched_adamw")
     return norm[:1] if norm is not None else None

@@ -135,29 +135,41 @@ def test_c_entries_refuse_before_any_launch():
     from sd_mecha_amd import _lib
     L = _lib.lib()
     at = 4096                                                               # an address that is never read
-    cast = lambda **k: L.mecha_cast_blocks(*[k.get(n, d) for n, d in (                                         # noqa: E731
-        ("a", at), ("rows", 4), ("cols", 100), ("ld", 100), ("dt", _lib.F32), ("tile", 0), ("q", at), ("pitch", 128), ("s", at), ("sp", 1),
-        ("qt", None), ("pt", 0), ("st", None), ("spt", 0), ("flags", None), ("stream", None))])
-    for bad in (dict(rows=-1), dict(dt=7), dict(q=None), dict(ld=99), dict(pitch=100), dict(pitch=0), dict(sp=0), dict(s=None), dict(q=at + 8),
-                dict(a=None), dict(qt=at, pt=100, st=at, spt=1)):
+
+    def packed(of, fields, change):
+        return of.pack(*[change.get(n, d) for n, d in fields])
+
+    def matrix(**k):
+        return packed(_lib.BLOCK_MATRIX, (("codes", at), ("scales", at), ("rows", 4), ("cols", 100), ("pitch", 128), ("sp", 1), ("tile", 0), ("sdt", 1)), k)
+
+    def cast(q=matrix(), qt=None, a=at, ld=100, dt=_lib.F32):
+        return L.mecha_cast_blocks(a, ld, dt, q, qt, None, None)
+    for bad in (dict(q=matrix(rows=-1)), dict(dt=7), dict(q=None), dict(ld=99), dict(q=matrix(pitch=100)), dict(q=matrix(pitch=0)), dict(q=matrix(sp=0)),
+                dict(q=matrix(scales=0)), dict(q=matrix(codes=at + 8)), dict(a=None), dict(q=matrix(sdt=0)), dict(qt=matrix(rows=100, cols=4, pitch=100)),
+                dict(qt=matrix(rows=100, cols=5)), dict(qt=matrix(rows=100, cols=4, tile=1)), dict(qt=matrix())):
         assert cast(**bad) < 0 and L.mecha_last_error(), bad
-    un = lambda **k: L.mecha_uncast_blocks(*[k.get(n, d) for n, d in (                                         # noqa: E731
-        ("q", at), ("pitch", 128), ("s", at), ("sp", 1), ("sdt", 0), ("tile", 0), ("rows", 4), ("cols", 100), ("out", at), ("dt", 0), ("flags", None), ("stream", None))])
-    for bad in (dict(q=None), dict(pitch=64), dict(sdt=5), dict(dt=9), dict(out=None), dict(cols=-1)):
+
+    def un(q=matrix(), out=at, dt=0):
+        return L.mecha_uncast_blocks(q, out, dt, None, None)
+    for bad in (dict(q=None), dict(q=matrix(codes=0)), dict(q=matrix(pitch=64)), dict(q=matrix(sdt=5)), dict(dt=9), dict(out=None), dict(q=matrix(cols=-1))):
         assert un(**bad) < 0, bad
-    prod = lambda **k: L.mecha_block_product(*[k.get(n, d) for n, d in (                                       # noqa: E731
-        ("a", at), ("ap", 128), ("sa", at), ("sap", 1), ("at", 0), ("b", at), ("bp", 128), ("sb", at), ("sbp", 1), ("bt", 0), ("sdt", 1),
-        ("base", None), ("out", at), ("m", 4), ("n", 4), ("k", 100), ("bdt", 0), ("odt", 0), ("alpha", 1.0), ("flags", None), ("stream", None))])
-    for bad in (dict(m=-1), dict(k=0), dict(odt=3), dict(base=at, bdt=4), dict(sdt=2), dict(out=None), dict(a=None), dict(bp=127), dict(sap=0),
-                dict(ap=1 << 25), dict(b=at + 4), dict(m=1 << 20, n=1 << 30)):
+
+    def prod(a=matrix(), b=matrix(), base=None, bdt=0, out=at, odt=0):
+        return L.mecha_block_product(a, b, base, bdt, out, odt, 1.0, None, None)
+    for bad in (dict(a=matrix(rows=-1)), dict(a=matrix(cols=0), b=matrix(cols=0)), dict(a=matrix(cols=99)), dict(odt=3), dict(base=at, bdt=4), dict(a=matrix(sdt=2)),
+                dict(a=matrix(sdt=0)), dict(out=None), dict(a=None), dict(b=None), dict(a=matrix(codes=0)), dict(b=matrix(pitch=127)), dict(a=matrix(sp=0)),
+                dict(a=matrix(pitch=1 << 25)), dict(b=matrix(codes=at + 4)), dict(a=matrix(rows=1 << 20), b=matrix(rows=1 << 30)), dict(a=matrix(rows=1 << 31))):
         assert prod(**bad) < 0, bad
-    ad = lambda **k: L.mecha_batched_adamw(*[k.get(n, d) for n, d in (                                         # noqa: E731
-        ("p", at), ("g", at), ("m", at), ("v", at), ("ms", None), ("vs", None), ("copy", None), ("segs", at), ("n", 1), ("total", 256), ("pd", 0),
-        ("gd", 0), ("cd", 0), ("bits", 32), ("lr", 1e-3), ("b1", 0.9), ("b2", 0.999), ("eps", 1e-8), ("wd", 0.0), ("kwd", None), ("step", 1),
-        ("sd", None), ("seed", 0), ("clip", None), ("flags", None), ("stream", None))])
-    for bad in (dict(n=0), dict(segs=None), dict(total=-1), dict(total=1 << 36), dict(pd=5), dict(copy=at, cd=9), dict(bits=16), dict(b1=1.0),
-                dict(lr=-1.0), dict(eps=-1.0), dict(step=0), dict(p=None), dict(bits=8), dict(bits=8, ms=at, vs=at, total=130), dict(bits=8, ms=at, vs=at, m=at + 4)):
+
+    def ad(**k):
+        return L.mecha_batched_adamw(packed(_lib.ADAMW, (
+            ("p", at), ("g", at), ("m", at), ("v", at), ("ms", 0), ("vs", 0), ("copy", 0), ("segs", at), ("kwd", 0), ("sd", 0), ("clip", 0), ("flags", 0),
+            ("total", 256), ("step", 1), ("lr", 1e-3), ("b1", 0.9), ("b2", 0.999), ("eps", 1e-8), ("wd", 0.0), ("n", 1), ("pd", 0), ("gd", 0), ("cd", 0),
+            ("bits", 32), ("seed", 0)), k), None)
+    for bad in (dict(n=0), dict(segs=0), dict(total=-1), dict(total=1 << 36), dict(pd=5), dict(copy=at, cd=9), dict(bits=16), dict(b1=1.0),
+                dict(lr=-1.0), dict(eps=-1.0), dict(step=0), dict(p=0), dict(bits=8), dict(bits=8, ms=at, vs=at, total=130), dict(bits=8, ms=at, vs=at, m=at + 4)):
         assert ad(**bad) < 0, bad
+    assert L.mecha_batched_adamw(None, None) < 0
     norm = lambda **k: L.mecha_batched_grad_norm(*[k.get(n, d) for n, d in (                                   # noqa: E731
         ("g", at), ("segs", at), ("n", 1), ("total", 256), ("gd", 0), ("max", 1.0), ("out", at), ("ws", at), ("size", 1 << 20), ("stream", None))])
     for bad in (dict(g=None), dict(out=None), dict(max=-1.0), dict(ws=None), dict(size=8), dict(gd=4), dict(n=0)):
