@@ -512,11 +512,6 @@ struct BigLds {
     uint32_t scale[2][2][BIG_CH][BIG_M];          // [parity of the chunk][a, b][word][row]
 };
 
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 // 1 KiB, as dma4
 __device__ __forceinline__ void dma1(const uint8_t *base, uint32_t off, uint32_t dst) {
     unsigned keep;
@@ -565,7 +560,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     auto swz_n = [](int row) { return EXACT ? swz_a(row) : swz_b(row); };
 
     // DMA: wave w brings rows 8 w .. + 7 of every 64 of each side, 1 KiB a piece; rows behind the last one read the last one
-    constexpr int PIECES = 4 + (ROWS + 63) / 64;
+    constexpr int PIECES = 4 + (ROWS + 63) / 64;                                  // 6, 7 or 8
     const int bring_row = 8 * wave + (lane >> 3);
     const uint32_t part_a = 16u * (uint32_t)((lane & 7) ^ swz_a(bring_row)), part_b = 16u * (uint32_t)((lane & 7) ^ swz_n(bring_row));
     int last_a, last_b;
@@ -642,14 +637,16 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     clear();
     wait_vm0();
     int stage = 0, chunk = 0, kb = 0;
-    // 16-bit results: fragment i + 2 of a is read while fragment i is multiplied, and a step's last fragment is multiplied behind the next
-    // barrier, while the next step's first ones come from LDS.
+    // Fragment i + 2 of a is read while fragment i is multiplied (i + 1 is made a bfloat16 then, for float32 results), and a step's last
+    // fragment is multiplied behind the next barrier, while the next step's first ones come from LDS.
     constexpr int SLOTS = MI == 4 ? 4 : 3;                                        // the carried fragment keeps its slot while fragment 0 is read
     static_assert((MI - 1) % SLOTS != 0, "slots");
     i32x8 fa[SLOTS], fb[4];
     uint32_t sa[SLOTS], sb[4];                                                        // sb: the matrix unit's
     f32x4v sbf[4];
     float sb1 = 0.0f;
+    bf16x8 aq[2][4], bq[4][4];                                                    // float32 results: [fragment][quarter] of a and b as bfloat16
+    float sz = 0.0f;                                                              // and the carried fragment's scale
 #pragma clang loop unroll(disable)
     while (true) {
         const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
@@ -683,64 +680,73 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             return join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + on), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + on));
         };
         auto bring = [&](int x) { issue(next_kb, stage ^ 1, x); };
-        if constexpr (MODE == EXACT_E8M0) {
-            // the scales go into the conversion: code * 2^e is a bfloat16
-            bf16x8 bq[4][4];                                                      // b's, [fragment][quarter]
-            fa[0] = read_a(0);
-            sa[0] = sa_row[0];
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                const i32x8 fb = read_b(f);
-                const float sb = __uint_as_float(sb_row[rb0 + 16 * f]);
-#pragma unroll
-                for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(fb[2 * q], fb[2 * q + 1], sb);
-            }
-#pragma unroll
-            for (int i = 0; i < MI; i++) {
-                if (i + 1 < MI) { fa[(i + 1) & 1] = read_a(i + 1); sa[(i + 1) & 1] = sa_row[16 * (i + 1)]; }
-                bring(2 * i);
-                bring(2 * i + 1);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const bf16x8 aq = codes_to_bf16(fa[i & 1][2 * q], fa[i & 1][2 * q + 1], __uint_as_float(sa[i & 1]));
-#pragma unroll
-                    for (int f = 0; f < 4; f++) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq, acc[i][f], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MI; i++)                                          // (nothing is executed here: the sums are made at this point, not sunk to the stores)
-                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
-        } else if constexpr (EXACT) {
-            bf16x8 bq[4][4];                                                      // b's codes as bfloat16, [fragment][quarter]
-            if constexpr (B_UNIFORM) sb1 = __uint_as_float(sb_row[wn]);
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                const i32x8 fb = read_b(f);
-                if constexpr (!B_UNIFORM) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * f + 4 * g]);
-#pragma unroll
-                for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(fb[2 * q], fb[2 * q + 1]);
-            }
-#pragma unroll
-            for (int i = 0; i < MI; i++) {
-                const i32x8 fa = read_a(i);
-                bring(2 * i);
-                bring(2 * i + 1);
-                const float sa = __uint_as_float(sa_row[16 * i]) * (B_UNIFORM ? sb1 : 1.0f);
+        if constexpr (EXACT) {
+            constexpr int Z = MI - 1;                                             // the fragment carried over
+            static_assert(Z % 2 == 1, "the carried fragment keeps its place while fragment 0 is made");
+            // Quarter q of fragment i of a as bfloat16.  Power-of-two scales go into the conversion: code * 2^e is a bfloat16.
+            auto make_a = [&](int i, int q) { aq[i & 1][q] = codes_to_bf16(fa[i & 1][2 * q], fa[i & 1][2 * q + 1], MODE == EXACT_E8M0 ? __uint_as_float(sa[i & 1]) : 1.0f); };
+            auto fetch_a = [&](int i) { fa[i & 1] = read_a(i); sa[i & 1] = sa_row[16 * i]; };
+            // fragments f0 .. f0 + count - 1 of b with fragment i of a, quarter by quarter: one sum's instructions lie `count` apart
+            auto multiply = [&](int i, int f0, int count, float scale, auto between) {
                 f32x4v d[4];
 #pragma unroll
                 for (int f = 0; f < 4; f++) d[f] = f32x4v{0, 0, 0, 0};
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const bf16x8 aq = codes_to_bf16(fa[2 * q], fa[2 * q + 1]);
 #pragma unroll
-                    for (int f = 0; f < 4; f++) d[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq, d[f], 0, 0, 0);
+                    for (int x = 0; x < count; x++) {
+                        const int f = f0 + x;
+                        if constexpr (MODE == EXACT_E8M0) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq[i & 1][q], acc[i][f], 0, 0, 0);
+                        else d[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq[i & 1][q], d[x], 0, 0, 0);
+                    }
+                    between(q);
+                }
+                if constexpr (MODE == EXACT_F32) {
+#pragma unroll
+                    for (int x = 0; x < count; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][f0 + x][e] = __builtin_fmaf(d[x][e], scale * sbf[f0 + x][e], acc[i][f0 + x][e]);
+                }
+            };
+            auto nothing = [](int) {};
+            i32x8 raw[4];
+            uint32_t rawscale[4];
+#pragma unroll
+            for (int f = 0; f < 4; f++) { raw[f] = read_b(f); rawscale[f] = sb_row[rb0 + 16 * f]; }
+            fetch_a(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (kb > 0) multiply(Z, 2 * h, 2, sz, nothing);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 2 * h; f < 2 * h + 2; f++) {
+                    if constexpr (MODE == EXACT_F32) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * f + 4 * g]);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(raw[f][2 * q], raw[f][2 * q + 1], MODE == EXACT_E8M0 ? __uint_as_float(rawscale[f]) : 1.0f);
                 }
 #pragma unroll
-                for (int f = 0; f < 4; f++)
+                for (int x = 0; x < PIECES / 2; x++) bring(PIECES / 2 * h + x);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("" : "+v"(acc[Z][0]), "+v"(acc[Z][1]), "+v"(acc[Z][2]), "+v"(acc[Z][3]));
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[f][e], B_UNIFORM ? sa : sa * sbf[f][e], acc[i][f][e]);
-                // (nothing is executed here: the sums are made at this point, not sunk to where they are stored)
+            for (int q = 0; q < 4; q++) make_a(0, q);
+            float si = __uint_as_float(sa[0]);
+            fetch_a(1);
+#pragma unroll
+            for (int i = 0; i < Z; i++) {
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(i, 0, 4, si, [&](int q) { make_a(i + 1, q); });
+                si = __uint_as_float(sa[(i + 1) & 1]);
+                if (i + 2 < MI) fetch_a(i + 2);
+                // (nothing is executed here: the sums are made at this point, not sunk to the stores)
                 asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
+            }
+            sz = si;
+            if (last) {
+                multiply(Z, 0, 4, sz, nothing);
+                asm volatile("" : "+v"(acc[Z][0]), "+v"(acc[Z][1]), "+v"(acc[Z][2]), "+v"(acc[Z][3]));
             }
         } else {
             // One 16 x 16 x 128 product; shift: the byte of the scales' words that belongs to the step (HW_SCALES).

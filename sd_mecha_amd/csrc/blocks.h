@@ -32,6 +32,13 @@ __device__ __forceinline__ float max16(float v) {
     return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x121, 0xf, 0xf, true)));
 }
 
+// A barrier for what the waves exchange through LDS: unlike __syncthreads() it does not wait for stores to memory.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept
 static inline int mecha_check_blocks(const char *what, const mecha_block_matrix &q) {
     const int64_t blocks = (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK;

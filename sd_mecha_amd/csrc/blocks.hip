@@ -155,7 +155,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
 // waves, and an 8 x 8 square of codes turns over in registers; transposed codes go through 16 KiB of LDS to leave as whole
 // 128-byte lines.
 template <int DT, bool VEC, bool TILE>
-__global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
+__global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
     constexpr int W = WORDS<DT>;
     __shared__ uint32_t wave_max[4][16][W];
     __shared__ u32x2 turned[SCALE_BLOCK][16];
@@ -171,41 +171,45 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
             for (int j = 0; j < W; j++) v[i].w[j] = 0u;
         }
     }
-    uint32_t rmax[8], nan[2] = {0, 0}, all = 0;      // nan: 8 bits a row
-#pragma unroll
-    for (int i = 0; i < 8; i++) { rmax[i] = mag8<DT>(v[i]); all = max_mag<DT>(all, rmax[i]); }
-    const bool bad = one_mag<DT>(all) >= INF<DT>;
-    if (bad) {
+    // columns first: over this thread's rows, and from there whether anything is inf or NaN
+    uint32_t cmax[W], nan[2] = {0, 0}, all = 0;      // nan: 8 bits a row
+    auto columns = [&]() {
         all = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) { nan[i >> 2] |= take_out<DT>(v[i]) << (8 * (i & 3)); rmax[i] = mag8<DT>(v[i]); all = max_mag<DT>(all, rmax[i]); }
+        for (int j = 0; j < W; j++) {
+            cmax[j] = v[0].w[j] & MAG<DT>;
+#pragma unroll
+            for (int i = 1; i < 8; i++) cmax[j] = max_mag<DT>(cmax[j], v[i].w[j] & MAG<DT>);
+            all = max_mag<DT>(all, cmax[j]);
+        }
+    };
+    columns();
+    const bool bad = one_mag<DT>(all) >= INF<DT>;
+    if (bad) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) nan[i >> 2] |= take_out<DT>(v[i]) << (8 * (i & 3));
+        columns();
         if (p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
     }
-    int re[8], ce[8];                            // exponents of this thread's rows and columns
+    int tile_e = 0;
     if constexpr (TILE) {
-        uint32_t m = max_mag16<DT>(one_mag<DT>(all));
+        const uint32_t m = max_mag16<DT>(one_mag<DT>(all));
         if (tc == 0) wave_max[wave][tr & 3][0] = m;
-        __syncthreads();
-        m = 0;
+        lds_barrier();
+        uint32_t o = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) { const uint32_t o = wave_max[i >> 2][i & 3][0]; m = m > o ? m : o; }
-        const int e = exponent_of_mag<DT>(m);
-#pragma unroll
-        for (int i = 0; i < 8; i++) re[i] = ce[i] = e;
+        for (int i = 0; i < 16; i++) o = o > wave_max[i >> 2][i & 3][0] ? o : wave_max[i >> 2][i & 3][0];
+        tile_e = exponent_of_mag<DT>(o);
         if (t == 0) {
-            if (p.q) p.s[sr * p.s_pitch + sc] = (uint8_t)(e + 127);
-            if (p.qt) p.st[sc * p.st_pitch + sr] = (uint8_t)(e + 127);
+            if (p.q) p.s[sr * p.s_pitch + sc] = (uint8_t)(tile_e + 127);
+            if (p.qt) p.st[sc * p.st_pitch + sr] = (uint8_t)(tile_e + 127);
         }
     } else {
-        // columns: over this thread's rows, the wave's 4 row groups (lanes 16 and 32 apart), the 4 waves
-        uint32_t cmax[W];
+        // a column's maximum: the wave's 4 row groups (lanes 16 and 32 apart) here, the 4 waves behind the barrier
 #pragma unroll
         for (int j = 0; j < W; j++) {
-            uint32_t m = v[0].w[j] & MAG<DT>;
-#pragma unroll
-            for (int i = 1; i < 8; i++) m = max_mag<DT>(m, v[i].w[j] & MAG<DT>);
-            const auto x = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-            m = max_mag<DT>(x[0], x[1]);
+            const auto x = __builtin_amdgcn_permlane32_swap(cmax[j], cmax[j], false, false);
+            const uint32_t m = max_mag<DT>(x[0], x[1]);
             const auto y = __builtin_amdgcn_permlane16_swap(m, m, false, false);
             cmax[j] = max_mag<DT>(y[0], y[1]);
         }
@@ -213,7 +217,40 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
 #pragma unroll
             for (int j = 0; j < W; j++) wave_max[wave][lane][j] = cmax[j];
         }
-        __syncthreads();
+    }
+    // the straight codes leave while the columns' maxima meet
+    if (p.q) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            int e[2] = {tile_e, tile_e};
+            if constexpr (!TILE) {
+                if constexpr (DT == MECHA_F32) {
+                    e[0] = exponent_of_mag<DT>(max_mag16<DT>(mag8<DT>(v[i])));
+                    e[1] = exponent_of_mag<DT>(max_mag16<DT>(mag8<DT>(v[i + 1])));
+                } else {                             // two rows a word go round the lanes together
+                    const uint32_t m = max_mag16<DT>(one_mag<DT>(mag8<DT>(v[i])) | one_mag<DT>(mag8<DT>(v[i + 1])) << 16);
+                    e[0] = exponent_of_mag<DT>(m & 0xffffu);
+                    e[1] = exponent_of_mag<DT>(m >> 16);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int64_t row = row0 + i + h;
+                u32x2 codes = codes8<DT>(v[i + h], scale_bits(e[h] + 127));
+                if (bad) codes = with_nan(codes, nan[(i + h) >> 2] >> (8 * ((i + h) & 3)));
+                if (row < p.rows) {
+                    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = codes;
+                    if (!TILE && tc == 0) p.s[row * p.s_pitch + sc] = (uint8_t)(e[h] + 127);
+                }
+            }
+        }
+    }
+    int ce[8];                                       // exponents of this thread's columns
+    if constexpr (TILE) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) ce[j] = tile_e;
+    } else {
+        lds_barrier();
 #pragma unroll
         for (int j = 0; j < W; j++) {
             uint32_t m = wave_max[0][tc][j];
@@ -226,32 +263,6 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (c + j < p.cols) p.st[(c + j) * p.st_pitch + sr] = (uint8_t)(ce[j] + 127);
-        }
-        if (p.q) {
-            if constexpr (DT == MECHA_F32) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) re[i] = exponent_of_mag<DT>(max_mag16<DT>(rmax[i]));
-            } else {                             // two rows a word go round the lanes together
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const uint32_t m = max_mag16<DT>(one_mag<DT>(rmax[i]) | one_mag<DT>(rmax[i + 1]) << 16);
-                    re[i] = exponent_of_mag<DT>(m & 0xffffu);
-                    re[i + 1] = exponent_of_mag<DT>(m >> 16);
-                }
-            }
-            if (tc == 0) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (row0 + i < p.rows) p.s[(row0 + i) * p.s_pitch + sc] = (uint8_t)(re[i] + 127);
-            }
-        }
-    }
-    if (p.q) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            u32x2 codes = codes8<DT>(v[i], scale_bits(re[i] + 127));
-            if (bad) codes = with_nan(codes, nan[i >> 2] >> (8 * (i & 3)));
-            if (row0 + i < p.rows) *reinterpret_cast<u32x2 *>(p.q + (row0 + i) * p.q_pitch + c) = codes;
         }
     }
     if (p.qt) {
@@ -282,7 +293,7 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 4) void cast_squ
             // slot XOR the column's group: 16 lanes (columns 8 apart, 1 KiB) write to 16 different slots
             turned[8 * tc + j][tr ^ tc] = codes;
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int col = 16 * i + tr;
