@@ -16,6 +16,7 @@ from .merge_methods import _DT, _Flags, _resolve, cast
 CODES = torch.float8_e4m3fn
 _SCALE_DT = {torch.float32: SCALE_F32, torch.float8_e8m0fnu: SCALE_E8M0}
 SIDES = ("straight", "transposed", "both")
+_pack = _lib.BLOCK_MATRIX.pack
 
 
 def _blocks(n: int) -> int:
@@ -49,14 +50,13 @@ class BlockScaled:
         code = _SCALE_DT.get(scales.dtype)
         if values.dtype is not CODES or code is None:
             raise TypeError(f"BlockScaled: values of {values.dtype} (float8_e4m3fn) and scales of {scales.dtype} (float32, float8_e8m0fnu)")
-        shape, s_shape = values.shape, scales.shape
-        if len(shape) != 2 or len(s_shape) != 2 or values.device != scales.device:
-            raise ValueError(f"BlockScaled: values {tuple(shape)} on {values.device} and scales {tuple(s_shape)} on {scales.device} "
+        if values.dim() != 2 or scales.dim() != 2 or values.get_device() != scales.get_device():
+            raise ValueError(f"BlockScaled: values {tuple(values.shape)} on {values.device} and scales {tuple(scales.shape)} on {scales.device} "
                              "must be matrices on one device")
-        (rows, cols), (s_rows, s_cols) = shape, s_shape
-        if s_cols != _blocks(cols) or (s_rows != rows and s_rows != _blocks(rows)):
+        (rows, cols), (s_rows, s_cols) = values.shape, scales.shape
+        if s_cols != (cols + 127) // 128 or (s_rows != rows and s_rows != (rows + 127) // 128):
             raise ValueError(f"BlockScaled: values {rows} x {cols} take scales {rows} x {_blocks(cols)} or {_blocks(rows)} x {_blocks(cols)}, "
-                             f"got {tuple(s_shape)}")
+                             f"got {tuple(scales.shape)}")
         s_pitch, s_step = scales.stride()
         if (s_step != 1 and s_cols > 1) or (s_pitch < s_cols and s_rows > 1):
             scales, s_pitch = scales.contiguous(), s_cols
@@ -72,9 +72,10 @@ class BlockScaled:
             values, pitch = whole[:, :cols], width
         self._set(values, scales, rows, cols, s_rows != rows, pitch, s_pitch if s_rows > 1 else s_cols, code)
 
-    def _set(self, *of):
-        self.values, self.scales, self.rows, self.cols, self.tile, self.pitch, self.scale_pitch, self.scale_code = of
-        self._packed = _lib.BLOCK_MATRIX.pack(self.values.data_ptr(), self.scales.data_ptr(), *of[2:4], *of[5:7], of[4], of[7])
+    def _set(self, values, scales, rows, cols, tile, pitch, scale_pitch, scale_code):
+        self.values, self.scales, self.rows, self.cols = values, scales, rows, cols
+        self.tile, self.pitch, self.scale_pitch, self.scale_code = tile, pitch, scale_pitch, scale_code
+        self._packed = _pack(values.data_ptr(), scales.data_ptr(), rows, cols, pitch, scale_pitch, tile, scale_code)
 
     @property
     def shape(self) -> torch.Size:
@@ -170,7 +171,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
     """``base + alpha * a @ b.T`` (``base=None``: ``alpha * a @ b.T``) of two 8-bit matrices a [m, k], b [n, k], summed in float32 and rounded once to
     ``out_dtype`` (default float32; for 16-bit results the 8-bit matrix instructions first cut the products of 8 neighbouring k off under
     2^-13 of the largest, 1.5e-5 of a typical result) -- add_difference(base, product, alpha).  ``base``: m * n elements; the result has its shape.  ``out``: where
-    the result goes (contiguous, m * n elements, of the result's dtype); it may be ``base`` itself.
+    the result goes (contiguous, m * n elements, of the result's dtype); it may be ``base`` itself, and otherwise shares no memory with an input.
 
     A linear layer ``y = x @ w.T`` with w cast with ``tile=True, sides="both"`` to (w, wt), x and the output gradient g cast to (x, xt) and
     (g, gt): y = block_product(x, w), the input's gradient block_product(g, wt), the weight's block_product(gt, xt).
@@ -178,7 +179,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
     _check_blocks(a, "block_product")
     _check_blocks(b, "block_product")
     m, k, n, kb, device = a.rows, a.cols, b.rows, b.cols, a.values.device
-    if k != kb or b.values.device != device:
+    if k != kb or b.values.get_device() != device.index:
         raise ValueError(f"block_product: a {m} x {k} on {device} and b {n} x {kb} on {b.values.device} do not go together (a @ b.T)")
     if isinstance(alpha, torch.Tensor):
         if alpha.numel() != 1:
@@ -195,7 +196,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         if out_dtype is not None and out_dtype not in _DT:
             raise TypeError(f"block_product: unsupported out_dtype {out_dtype} (float32, float16, bfloat16)")
         out = torch.empty(shape, dtype=out_dtype or torch.float32, device=device)
-    elif out.device != device or out.numel() != m * n or not out.is_contiguous() or (out_dtype is not None and out.dtype != out_dtype):
+    elif not isinstance(out, torch.Tensor) or out.device != device or out.numel() != m * n or not out.is_contiguous() or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"block_product: out must be a contiguous tensor of {m} x {n} elements on {device}, of the out_dtype if that is given")
     if out.dtype not in _DT:
         raise TypeError(f"block_product: unsupported result dtype {out.dtype} (float32, float16, bfloat16)")

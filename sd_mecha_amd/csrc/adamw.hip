@@ -158,11 +158,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
     int64_t left;
     const int s = locate<N>(a.segs, a.n_segs, a.total, i, wave_i, valid, left);
     const float keep = 1.0f - a.lr * (a.decay ? (s >= 0 ? a.decay[s] : 0.0f) : a.decay_all);
-    float clip = 1.0f;
-    if (a.clip) {
-        clip = a.clip[1];
-        if (!(clip >= 0.0f)) return;                          // a gradient is inf or NaN: the step is left out
-    }
+    const float clip = a.clip ? a.clip[1] : 1.0f;
     float size = a.size, root_size = a.root_size;
     uint32_t key = a.key;
     if (a.step_dev) {
@@ -190,6 +186,16 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
             }
         }
     }
+    float poison_in = 0.0f, poison_out = 0.0f, root[N];       // fma(x, 0, poison) stays 0 while every x is finite
+    if (a.seg_flags) {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (j < valid) poison_in = __builtin_fmaf(g[j], 0.0f, __builtin_fmaf(p[j], 0.0f, poison_in));
+    }
+    if (!(clip >= 0.0f)) {                                    // the gradients' norm is inf or NaN: the step is left out
+        if (a.seg_flags && valid && poison_in != 0.0f) atomicOr(a.seg_flags + s, MECHA_FLAG_INPUT_NONFINITE);
+        return;
+    }
     auto store = [&](auto dt, void *to, const float (&from)[N]) {
         constexpr int DT = decltype(dt)::value;
         if (whole) store_n<DT, N>(to, i, from);
@@ -214,10 +220,8 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
                 if (j >= valid) m[j] = v[j] = g[j] = 0.0f;
         }
     }
-    float poison_in = 0.0f, poison_out = 0.0f, root[N];       // fma(x, 0, poison) stays 0 while every x is finite
 #pragma unroll
     for (int j = 0; j < N; j++) {
-        if (a.seg_flags && j < valid) poison_in = __builtin_fmaf(g[j], 0.0f, __builtin_fmaf(p[j], 0.0f, poison_in));
         const float gj = g[j] * clip;
         m[j] = __builtin_fmaf(gj, a.c1, m[j] * a.b1);
         v[j] = __builtin_fmaf(gj * gj, a.c2, v[j] * a.b2);
@@ -425,6 +429,13 @@ int mecha_batched_adamw(const mecha_adamw *args, void *stream) {
         MECHA_REQUIRE(x.total_elems % SCALE_BLOCK == 0, "8-bit states: total_elems %lld must be a multiple of 128", (long long)x.total_elems);
         MECHA_REQUIRE((reinterpret_cast<uintptr_t>(x.exp_avg) & 7u) == 0 && (reinterpret_cast<uintptr_t>(x.exp_avg_sq) & 7u) == 0, "8-bit states must be 8-byte aligned");
     }
+    const size_t n = (size_t)x.total_elems, state_bytes = x.state_bits == 8 ? n : 4 * n, scale_bytes = x.state_bits == 8 ? n / SCALE_BLOCK : 0;
+    const struct { const void *at; size_t bytes; } arenas[] = {
+        {x.params, n * mecha_dtype_size(x.param_dtype)}, {x.grads, n * mecha_dtype_size(x.grad_dtype)}, {x.exp_avg, state_bytes}, {x.exp_avg_sq, state_bytes},
+        {x.copy, x.copy ? n * mecha_dtype_size(x.copy_dtype) : 0}, {x.exp_avg_scales, scale_bytes}, {x.exp_avg_sq_scales, scale_bytes}};
+    for (int i = 0; i < 7; i++)
+        for (int j = 0; j < i; j++)
+            MECHA_REQUIRE(arenas[i].bytes == 0 || !mecha_overlap(arenas[i].at, arenas[i].bytes, arenas[j].at, arenas[j].bytes), "two arenas share memory");
     AdamParams a{};
     a.p = x.params; a.g = x.grads; a.m = x.exp_avg; a.v = x.exp_avg_sq;
     a.ms = static_cast<uint8_t *>(x.exp_avg_scales); a.vs = static_cast<uint8_t *>(x.exp_avg_sq_scales);

@@ -854,8 +854,8 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                                     poison_in = __builtin_fmaf(bb, 0.0f, poison_in);
                                 } else v[j] = sum * p.alpha;
                             }
-                            // (rows and columns behind the last ones are computed from the last ones: what is not finite there is so here)
-                            if (p.flags) {
+                            // (rows and columns behind the last ones are made from the last ones, but without their base)
+                            if (p.flags && row0 + 16 * i + odd < p.m && (int64_t)n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g) < p.n) {
 #pragma unroll
                                 for (int j = 0; j < EACH; j++) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
                             }
@@ -934,9 +934,9 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
     }
     static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
     for (int d = 0; d < 4; d++) {
-        const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * (double)k, one = bytes / 33e3, all = blocks * bytes / 5e6;
+        const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * bytes / 5e6;
         const double t = 2.5 + (one > all ? one : all);
-        if (t < best) { best = t; c.mi = 0; c.direct = d; }
+        if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.direct = d; }     // a launch's threads
     }
     return c;
 }
@@ -961,6 +961,12 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     MECHA_REQUIRE(a->pitch <= (1 << 24) && b->pitch <= (1 << 24), "rows of more than 2^24 bytes (%lld, %lld)", (long long)a->pitch, (long long)b->pitch);
     const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128;
     MECHA_REQUIRE(m < (1ll << 31) && n < (1ll << 31) && tm * tn < (1ll << 24), "%lld x %lld outputs are beyond one launch", (long long)m, (long long)n);
+    const size_t out_bytes = (size_t)m * n * mecha_dtype_size(out_dtype);
+    for (const mecha_block_matrix *q : {a, b})
+        MECHA_REQUIRE(!mecha_overlap(out, out_bytes, q->codes, mecha_codes_bytes(*q)) && !mecha_overlap(out, out_bytes, q->scales, mecha_scales_bytes(*q)),
+                      "out shares memory with a or b");
+    MECHA_REQUIRE(base == nullptr || (base == out && base_dtype == out_dtype) || !mecha_overlap(out, out_bytes, base, (size_t)m * n * mecha_dtype_size(base_dtype)),
+                  "out may be base itself, of the same dtype, but not overlap it otherwise");
     ProductParams p{static_cast<const uint8_t *>(a->codes), a->pitch, a->scales, a->scale_pitch, a->tile, static_cast<const uint8_t *>(b->codes), b->pitch,
                     b->scales, b->scale_pitch, b->tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
     const int b_tile = b->tile, scale_dtype = a->scale_dtype;

@@ -39,6 +39,19 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+static inline bool mecha_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && x < y + b_bytes && y < x + a_bytes;
+}
+// from a matrix's first code or scale to behind its last
+static inline size_t mecha_codes_bytes(const mecha_block_matrix &q) {
+    return q.rows && q.cols ? (size_t)(q.rows - 1) * q.pitch + (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK : 0;
+}
+static inline size_t mecha_scales_bytes(const mecha_block_matrix &q) {
+    const int64_t rows = q.tile ? (q.rows + SCALE_BLOCK - 1) / SCALE_BLOCK : q.rows;
+    return rows && q.cols ? ((size_t)(rows - 1) * q.scale_pitch + (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK) * (q.scale_dtype == MECHA_SCALE_F32 ? 4 : 1) : 0;
+}
+
 // the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept
 static inline int mecha_check_blocks(const char *what, const mecha_block_matrix &q) {
     const int64_t blocks = (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK;

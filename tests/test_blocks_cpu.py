@@ -170,6 +170,19 @@ def test_c_entries_refuse_before_any_launch():
                 dict(lr=-1.0), dict(eps=-1.0), dict(step=0), dict(p=0), dict(bits=8), dict(bits=8, ms=at, vs=at, total=130), dict(bits=8, ms=at, vs=at, m=at + 4)):
         assert ad(**bad) < 0, bad
     assert L.mecha_batched_adamw(None, None) < 0
+    # results that share memory with what they are made from: the addresses lie apart but for one byte
+    q, codes = dict(rows=4, cols=100, pitch=128), 4 * 128
+    far = [at * 16 * i for i in range(1, 8)]
+    one, two = matrix(**q, codes=far[0], scales=far[1]), matrix(**q, codes=far[2], scales=far[3])
+    for out in (far[0] + codes - 1, far[1] + 3, far[2] - 63, far[3] - 63):
+        assert prod(a=one, b=two, out=out) < 0 and b"shares memory" in L.mecha_last_error(), out
+    for more in (dict(bdt=2), dict(base=far[4] + 4), dict(base=far[4] - 63)):
+        assert prod(**{**dict(a=one, b=two, out=far[4], base=far[4]), **more}) < 0 and b"base itself" in L.mecha_last_error(), more
+    apart = dict(zip(("p", "g", "m", "v", "copy"), far))
+    for x in apart:
+        for y in set(apart) - {x}:
+            assert ad(**{**apart, x: apart[y] + 4 * 256 - 1}) < 0 and b"share memory" in L.mecha_last_error(), (x, y)
+    assert ad(**apart, bits=8, ms=far[5], vs=far[5] + 1) < 0 and b"share memory" in L.mecha_last_error()
     norm = lambda **k: L.mecha_batched_grad_norm(*[k.get(n, d) for n, d in (                                   # noqa: E731
         ("g", at), ("segs", at), ("n", 1), ("total", 256), ("gd", 0), ("max", 1.0), ("out", at), ("ws", at), ("size", 1 << 20), ("stream", None))])
     for bad in (dict(g=None), dict(out=None), dict(max=-1.0), dict(ws=None), dict(size=8), dict(gd=4), dict(n=0)):

@@ -211,8 +211,9 @@ def test_a_gradient_that_is_not_finite(bits):
         s = make(layout, bits=bits)
         before = {k: v.clone() for k, v in s.items()}
         s["grads"][layout.offsets[1] + 17] = value
-        norm = amd.adamw_step(**s, step=3, max_norm=1.0)
-        assert not bool(norm.isfinite())
+        flags = torch.zeros(3, dtype=torch.int32, device="cuda")
+        norm = amd.adamw_step(**s, step=3, max_norm=1.0, flags=flags)
+        assert not bool(norm.isfinite()) and flags.tolist() == [0, 1, 0]
         for k in ("params", "exp_avg", "exp_avg_sq"):
             assert torch.equal(s[k].view(torch.uint8), before[k].view(torch.uint8)), k
         flags = torch.zeros(3, dtype=torch.int32, device="cuda")

@@ -225,6 +225,55 @@ def test_product_large(m, n, k, scales, dtype):
         amd.block_product(amd.BlockScaled(v, a.scales), b, out_dtype=dtype)
 
 
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", LARGE)
+def test_product_large_float32(m, n, k, scales):
+    """Partial sums are multiples of 2^-6 (powers of two: 2^-3 on each side; whole scales: of 1) and no larger than the sum S of the products'
+    magnitudes: up to 2^24 of those units each is a float32 and the result exact.  Beyond (2049 x 2048: both sides are drawn alike, and the
+    diagonal holds squares) each of k additions is off by half a unit of S at most."""
+    import sd_mecha_amd as amd
+
+    def same(got, va, vb, alpha=1.0, base=None):
+        whole = va @ vb.t() * alpha
+        size = va.abs() @ vb.abs().t()
+        if base is not None:
+            whole = whole + base.double()
+        want, exact = whole.float(), size <= 2.0 ** (18 if scales == "e8m0" else 24)
+        assert bool(exact.float().mean() > 0.9)
+        return torch.equal(got[exact], want[exact]) and bool(((got.double() - whole).abs() <= (k + 2) * 2.0 ** -24 * abs(alpha) * (size + 64))[~exact].all())
+    for fa, fb in (("rows", "tile"), ("rows", "rows")):
+        a, b = matrix(m, k, fa, scales, m + 1, ints=True), matrix(n, k, fb, scales, n + 2, ints=True)
+        va, vb = torch.from_numpy(R.values(a)).cuda(), torch.from_numpy(R.values(b)).cuda()
+        assert same(amd.block_product(a, b), va, vb), (fa, fb)
+        base = torch.randint(-64, 64, (m, n), device="cuda").float()
+        assert same(amd.block_product(a, b, base, -2.0), va, vb, -2.0, base), (fa, fb)
+        assert same(amd.block_product(a, b, base, -2.0, out=base.clone()), va, vb, -2.0, base), (fa, fb)
+        out = base.clone()
+        assert same(amd.block_product(a, b, out, -2.0, out=out), va, vb, -2.0, base), (fa, fb)
+    a, b = matrix(m, k, "rows", scales, m + 3), matrix(n, k, "tile", scales, n + 4)
+    check_product(amd.block_product(a, b), a, b)
+
+
+# results of many tiles that are not whole 16-byte pieces, have a base of another type, or few k
+MIDDLE = [(2100, 1003, 700), (1500, 1501, 1700), (2100, 1000, 384), (1111, 2040, 200), (9000, 1100, 3), (70000, 200, 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", MIDDLE)
+def test_product_middle(m, n, k, scales, dtype):
+    import sd_mecha_amd as amd
+    a, b = matrix(m, k, "rows", scales, m + 1, ints=True), matrix(n, k, "tile", scales, n + 2, ints=True)
+    whole = torch.from_numpy(R.values(a)).cuda() @ torch.from_numpy(R.values(b)).cuda().t()
+    assert torch.equal(amd.block_product(a, b, alpha=2.0 ** -7, out_dtype=dtype), (whole * 2.0 ** -7).float().to(dtype))
+    base = torch.randint(-64, 64, (m, n), device="cuda")
+    want = (whole * 2.0 ** -7 + base.double()).float().to(dtype)
+    for base_dt in TYPES:
+        assert torch.equal(amd.block_product(a, b, base.to(base_dt), 2.0 ** -7, out_dtype=dtype), want), base_dt
+    room = torch.empty(m * n + 1, dtype=dtype, device="cuda")                       # 2 or 4 bytes off
+    assert torch.equal(amd.block_product(a, b, base.to(dtype), 2.0 ** -7, out=room[1:]).view(m, n), want)
+
+
 def test_product_extreme_scales():
     """Powers of two from 2^-127 on one side against large ones on the other."""
     import sd_mecha_amd as amd
@@ -329,6 +378,24 @@ def test_product_refusals_on_the_gpu():
     x = torch.zeros(40 * 50, device="cuda")
     with pytest.raises(ValueError):
         amd.block_product(a, b, x.view(torch.bfloat16)[:2000], out=x)
+    with pytest.raises(ValueError):
+        amd.block_product(a, b, out=[0.0] * 2000)
+    with pytest.raises(amd._lib.MechaError, match="shares memory"):
+        amd.block_product(a, b, out=torch.as_strided(a.values.view(torch.uint8), (8000,), (1,)).view(torch.float32))
+
+
+def test_product_flags_count_the_results_elements_only():
+    """What the tiles hold behind the last row and column is made from the last ones without their base, and may be infinite where the
+    result is not: 2^127 * 3 - 2^127 * 1.5."""
+    import sd_mecha_amd as amd
+    m, n, k = 2049, 2056, 700
+    ones = torch.ones(m, k, device="cuda").to(E4M3), torch.ones(n, k, device="cuda").to(E4M3)
+    a = amd.BlockScaled(ones[0], torch.full((m, 6), 2.0 ** 100, device="cuda"))
+    b = amd.BlockScaled(ones[1], torch.ones(n, 6, device="cuda"))
+    flags, alpha = torch.zeros(1, dtype=torch.int32, device="cuda"), 1.5 * 2.0 ** 28 / 700      # a @ b.T * alpha: 2^127 * 3, over the largest
+    base = torch.full((m, n), -1.5 * 2.0 ** 127, device="cuda")
+    got = amd.block_product(a, b, base, alpha, flags=flags, check_finite=False)
+    assert bool(got.isfinite().all()) and int(flags) == 0
 
 
 def test_product_outputs_past_two_to_the_31():
@@ -396,3 +463,29 @@ def test_same_result_every_time_on_any_stream_and_in_a_graph():
         eager = [call(f) for f in fresh]
         torch.cuda.synchronize()
         assert all(torch.equal(o, e) for o, e in zip(outs, eager))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+def test_large_products_in_a_graph_and_side_by_side(scales, dtype):
+    """Results of many tiles, of every kind of kernel, captured together and replayed next to the same products on another stream."""
+    import sd_mecha_amd as amd
+    pairs = [(matrix(m, k, "rows", scales, m), matrix(n, k, "tile", scales, n)) for m, n, k in ((2100, 2056, 1100), (2100, 1003, 700), (200, 640, 900))]
+    pairs = [(amd.BlockScaled(a.values, (a.scales.float() / 2.0 ** 17).to(a.scales.dtype)), b) for a, b in pairs]
+
+    def call():
+        return [amd.block_product(a, b, out_dtype=dtype, check_finite=False) for a, b in pairs]
+    want = call()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            eager = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) and torch.equal(e, w) for o, e, w in zip(outs, eager, want))
