@@ -495,8 +495,10 @@ template <int MODE>
 int launch_direct(int shape, const ProductParams &p, hipStream_t s) {
     if (shape == 0) return launch_direct<MODE, 1, 1>(p, s);
     if (shape == 1) return launch_direct<MODE, 1, 2>(p, s);
-    if (shape == 2) return launch_direct<MODE, 2, 2>(p, s);
-    return launch_direct<MODE, 2, 4>(p, s);
+    if constexpr (MODE != EXACT_F32) {
+        if (shape == 3) return launch_direct<MODE, 2, 4>(p, s);
+    }
+    return launch_direct<MODE, 2, 2>(p, s);
 }
 
 // ---------------------------------------------------------------------------------------------------- large products
@@ -630,125 +632,280 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     uint32_t m0, n0, nm0 = 0, nn0 = 0;
     place(tile, m0, n0);
     aim(m0, n0);
+    load_scales(m0, n0, 0);
 #pragma unroll
     for (int x = 0; x < PIECES; x++) issue(0, 0, x);
-    load_scales(m0, n0, 0);
     put_scales(0);
     clear();
     wait_vm0();
     int stage = 0, chunk = 0, kb = 0;
-    // Fragment i + 2 of a is read while fragment i is multiplied (i + 1 is made a bfloat16 then, for float32 results), and a step's last
-    // fragment is multiplied behind the next barrier, while the next step's first ones come from LDS.
-    constexpr int SLOTS = MI == 4 ? 4 : 3;                                        // the carried fragment keeps its slot while fragment 0 is read
-    static_assert((MI - 1) % SLOTS != 0, "slots");
-    i32x8 fa[SLOTS], fb[4];
-    uint32_t sa[SLOTS], sb[4];                                                        // sb: the matrix unit's
-    f32x4v sbf[4];
-    float sb1 = 0.0f;
-    bf16x8 aq[2][4], bq[4][4];                                                    // float32 results: [fragment][quarter] of a and b as bfloat16
-    float sz = 0.0f;                                                              // and the carried fragment's scale
+    auto cut_tail = [&]() {                                                       // bytes behind column k are not the matrix's
+        const int row = t >> 1;                                                   // thread: half of a row of each side
 #pragma clang loop unroll(disable)
-    while (true) {
-        const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
+        for (int c = 0; c < 8; c++) {
+            const int sd = c >> 2, piece = 4 * (t & 1) + (c & 3), left = tail - 16 * piece;
+            if (left < 16) {
+                u32x4 *at = reinterpret_cast<u32x4 *>(&lds.stage[stage][sd][row * 128 + 16 * (piece ^ (sd ? swz_n(row) : swz_a(row)))]);
+                *at = first_bytes(*at, left);
+            }
+        }
         lds_barrier();
-        if (last && tail < SCALE_BLOCK) {                                         // bytes behind column k are not the matrix's
-            const int row = t >> 1;                                               // thread: half of a row of each side
-#pragma clang loop unroll(disable)
-            for (int c = 0; c < 8; c++) {
-                const int sd = c >> 2, piece = 4 * (t & 1) + (c & 3), left = tail - 16 * piece;
-                if (left < 16) {
-                    u32x4 *at = reinterpret_cast<u32x4 *>(&lds.stage[stage][sd][row * 128 + 16 * (piece ^ (sd ? swz_n(row) : swz_a(row)))]);
-                    *at = first_bytes(*at, left);
+    };
+    auto finish = [&]() {
+        // 16-byte pieces of two rows change places between two lanes, so that 8 lanes store a row's 128 bytes with one instruction;
+        // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280: 121 -> 103 us).
+        constexpr int EACH = EXACT ? 4 : 8, ESIZE = EXACT ? 4 : 2;        // elements of a piece, bytes of one
+        const bool odd = lane & 1;
+        const int64_t row0 = (int64_t)m0 + wm + (r & ~1), line = p.n * ESIZE;
+        const int rows = p.m - row0 < BIG_M ? (int)(p.m - row0) : BIG_M;
+        int64_t at0 = (row0 * p.n + n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g)) * ESIZE;
+        const int64_t cols = p.n - ((int64_t)n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g));
+        bool nan = false;
+        float poison_in = 0.0f, poison_out = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MI; i++) {
+#pragma unroll
+            for (int pair = 0; pair < (EXACT ? 2 : 1); pair++) {
+                // this lane's pieces in memory: number 0 (even lane) or 1 (odd) of the pair
+                const int64_t at = at0 + (EXACT ? 32 * ESIZE * pair : 0);
+                const bool in = cols > (EXACT ? 32 * pair : 0), here = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
+                u32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                if constexpr (BASE) {
+                    if (here) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at));
+                    if (below) c[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at + line));
+                    exchange(c[0], c[1], odd);
                 }
-            }
-            lds_barrier();
-        }
-        if (last && more) {
-            place(tile + per_xcd, nm0, nn0);
-            aim(nm0, nn0);
-        }
-        const int next_kb = last ? 0 : kb + 1;
-        const bool refill = last ? more : next_kb % PER == 0;
-        if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
-
-        const uint8_t *la = &lds.stage[stage][0][0], *lb = &lds.stage[stage][1][0];
-        const int w = MODE == HW_SCALES ? (kb / 4) & (BIG_CH - 1) : kb & (BIG_CH - 1), sh = 8 * (kb & 3);
-        const uint32_t *sa_row = &lds.scale[chunk][0][w][ra0], *sb_row = &lds.scale[chunk][1][w][0];
-        auto read_a = [&](int i) { return join(*reinterpret_cast<const u32x4 *>(la + fa_at[0] + 2048 * i), *reinterpret_cast<const u32x4 *>(la + fa_at[1] + 2048 * i)); };
-        auto read_b = [&](int f) {
-            const int on = 128 * (b_at(f, 0) - b_at(0, 0));
-            return join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + on), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + on));
-        };
-        auto bring = [&](int x) { issue(next_kb, stage ^ 1, x); };
-        if constexpr (EXACT) {
-            constexpr int Z = MI - 1;                                             // the fragment carried over
-            static_assert(Z % 2 == 1, "the carried fragment keeps its place while fragment 0 is made");
-            // Quarter q of fragment i of a as bfloat16.  Power-of-two scales go into the conversion: code * 2^e is a bfloat16.
-            auto make_a = [&](int i, int q) { aq[i & 1][q] = codes_to_bf16(fa[i & 1][2 * q], fa[i & 1][2 * q + 1], MODE == EXACT_E8M0 ? __uint_as_float(sa[i & 1]) : 1.0f); };
-            auto fetch_a = [&](int i) { fa[i & 1] = read_a(i); sa[i & 1] = sa_row[16 * i]; };
-            // fragments f0 .. f0 + count - 1 of b with fragment i of a, quarter by quarter: one sum's instructions lie `count` apart
-            auto multiply = [&](int i, int f0, int count, float scale, auto between) {
-                f32x4v d[4];
 #pragma unroll
-                for (int f = 0; f < 4; f++) d[f] = f32x4v{0, 0, 0, 0};
+                for (int h = 0; h < 2; h++) {
+                    float v[EACH];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-#pragma unroll
-                    for (int x = 0; x < count; x++) {
-                        const int f = f0 + x;
-                        if constexpr (MODE == EXACT_E8M0) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq[i & 1][q], acc[i][f], 0, 0, 0);
-                        else d[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bq[f][q], aq[i & 1][q], d[x], 0, 0, 0);
+                    for (int j = 0; j < EACH; j++) {
+                        const float sum = EXACT ? acc[i][2 * pair + h][j & 3] : acc[i][2 * h + (j >> 2)][j & 3];
+                        if constexpr (BASE) {
+                            const uint32_t word = EXACT ? c[h][j & 3] : c[h][j >> 1];
+                            const uint32_t half = j & 1 ? word >> 16 : word & 0xffffu;
+                            const float bb = EXACT ? __uint_as_float(word) : BF16 ? bf16_bits_to_f32(half) : f16_bits_to_f32(half);
+                            v[j] = __builtin_fmaf(sum, p.alpha, bb);
+                            poison_in = __builtin_fmaf(bb, 0.0f, poison_in);
+                        } else v[j] = sum * p.alpha;
                     }
-                    between(q);
+                    // (rows and columns behind the last ones are made from the last ones, but without their base)
+                    if (p.flags && row0 + 16 * i + odd < p.m && (int64_t)n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g) < p.n) {
+#pragma unroll
+                        for (int j = 0; j < EACH; j++) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
+                    }
+                    if constexpr (EXACT) c[h] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) c[h][j] = BF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : pack_f16(v[2 * j], v[2 * j + 1]);
+                    }
                 }
-                if constexpr (MODE == EXACT_F32) {
+                exchange(c[0], c[1], odd);
+                if (here) __builtin_nontemporal_store(c[0], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at));
+                if (below) __builtin_nontemporal_store(c[1], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at + line));
+            }
+            at0 += 16 * line;
+            asm volatile("" : "+v"(at0));                                 // (addresses one after the other, not all at once)
+            if (i % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        nan |= poison_in != 0.0f;
+        if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+    };
+    if constexpr (EXACT) {
+        // Float32 results.  A step is four fragments of a, each multiplied a quarter of its k at a time: 4 instructions of 16 cycles.  The matrix unit
+        // leaves room for two other instructions beside each of its own, so the conversions to bfloat16 stand between them, one by one: the next
+        // fragment's of a, and, while the last one is multiplied, the next step's of b, each in the place of the quarter that was used last (the last
+        // quarter's in the next step).  Behind the second fragment all that is left of this stage is in registers: there the waves meet, the step
+        // after the next is asked for into this one's place, and the next step's codes are read.  A wave that is in its last fragment goes first, which
+        // keeps the two waves of a SIMD apart: 1280 x 5120 x 8269 102 us, 110 without.
+        static_assert(MI == 4, "fragments");
+        i32x8 fa[2], raw[4];
+        uint32_t sa[2], rawscale[4];
+        f32x4v sbf[4];
+        i32x4 aq[2][4], bq[4][4];                                                // [fragment][quarter] of a and b
+        int dkb = 0;                                                              // the step that was asked for last
+        uint32_t dtile = tile;
+        auto advance = [&]() {                                                    // (behind the last tile it stays, and fetches what nobody reads)
+            if (++dkb < n_kb) return;
+            dkb = 0;
+            if (dtile + per_xcd >= run1) return;
+            dtile += per_xcd;
+            uint32_t dm, dn;
+            place(dtile, dm, dn);
+            aim(dm, dn);
+        };
+        const uint8_t *la = nullptr, *lb = nullptr;
+        const uint32_t *sa_row = nullptr, *sb_row = nullptr;
+        auto look = [&](int at_kb) {                                              // at the codes and scales of a step
+            la = &lds.stage[stage][0][0]; lb = &lds.stage[stage][1][0];
+            sa_row = &lds.scale[chunk][0][at_kb & (BIG_CH - 1)][ra0]; sb_row = &lds.scale[chunk][1][at_kb & (BIG_CH - 1)][0];
+        };
+        auto fetch_a = [&](int i) {
+            fa[i & 1] = join(*reinterpret_cast<const u32x4 *>(la + fa_at[0] + 2048 * i), *reinterpret_cast<const u32x4 *>(la + fa_at[1] + 2048 * i));
+            sa[i & 1] = sa_row[16 * i];
+        };
+        auto fetch_b = [&]() {
 #pragma unroll
-                    for (int x = 0; x < count; x++)
+            for (int f = 0; f < 4; f++) {
+                raw[f] = join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + 2048 * f), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + 2048 * f));
+                if constexpr (MODE == EXACT_E8M0) rawscale[f] = sb_row[rb0 + 16 * f];
+            }
+        };
+        auto fetch_sb = [&]() {
+            if constexpr (MODE == EXACT_F32) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[i][f0 + x][e] = __builtin_fmaf(d[x][e], scale * sbf[f0 + x][e], acc[i][f0 + x][e]);
+                for (int f = 0; f < 4; f++) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * f + 4 * g]);
+            }
+        };
+        // Power-of-two scales go into the conversion: code * 2^e is a bfloat16.
+        auto code2 = [](const i32x8 &v, int q, int w, uint32_t scale) {           // codes 2 w, 2 w + 1 of quarter q
+            const float by = MODE == EXACT_E8M0 ? __uint_as_float(scale) : 1.0f;
+            const int from = v[2 * q + w / 2];
+            return __builtin_bit_cast(int, w & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(from, by, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(from, by, false));
+        };
+        // (the empty statements keep a conversion where it stands)
+        auto make_a = [&](int i, int q, int w) {
+            int v = code2(fa[i & 1], q, w, sa[i & 1]);
+            asm volatile("" : "+v"(v));
+            aq[i & 1][q][w] = v;
+        };
+        auto make_b = [&](int f, int q) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                int v = code2(raw[f], q, w, rawscale[f]);
+                asm volatile("" : "+v"(v));
+                bq[f][q][w] = v;
+            }
+        };
+        auto multiply = [&](int i, float scale, auto between) {
+            f32x4v d[4];
+#pragma unroll
+            for (int f = 0; f < 4; f++) d[f] = f32x4v{0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    const bf16x8 x = __builtin_bit_cast(bf16x8, bq[f][q]), y = __builtin_bit_cast(bf16x8, aq[i & 1][q]);
+                    if constexpr (MODE == EXACT_E8M0) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc[i][f], 0, 0, 0);
+                    else d[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, d[f], 0, 0, 0);
+                    between(q, f);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            };
-            auto nothing = [](int) {};
-            i32x8 raw[4];
-            uint32_t rawscale[4];
+            if constexpr (MODE == EXACT_F32) {
 #pragma unroll
-            for (int f = 0; f < 4; f++) { raw[f] = read_b(f); rawscale[f] = sb_row[rb0 + 16 * f]; }
-            fetch_a(0);
+                for (int f = 0; f < 4; f++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][f][e] = __builtin_fmaf(d[f][e], scale * sbf[f][e], acc[i][f][e]);
+            }
+            // (nothing is executed here: the sums are made at this point, not sunk to the stores)
+            asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
             __builtin_amdgcn_sched_barrier(0);
+        };
+        lds_barrier();
+        advance();
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (kb > 0) multiply(Z, 2 * h, 2, sz, nothing);
-                __builtin_amdgcn_sched_barrier(0);
+        for (int x = 0; x < PIECES; x++) issue(dkb, 1, x);
+        look(0);
+        fetch_b();
+        fetch_sb();
+        fetch_a(0);
 #pragma unroll
-                for (int f = 2 * h; f < 2 * h + 2; f++) {
-                    if constexpr (MODE == EXACT_F32) sbf[f] = *reinterpret_cast<const f32x4v *>(&sb_row[wn + 16 * f + 4 * g]);
+        for (int q = 0; q < 4; q++) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++) bq[f][q] = codes_to_bf16(raw[f][2 * q], raw[f][2 * q + 1], MODE == EXACT_E8M0 ? __uint_as_float(rawscale[f]) : 1.0f);
-                }
-#pragma unroll
-                for (int x = 0; x < PIECES / 2; x++) bring(PIECES / 2 * h + x);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int f = 0; f < 4; f++) {
+                if (q < 3) make_b(f, q);
+                make_a(0, q, f);
             }
-            asm volatile("" : "+v"(acc[Z][0]), "+v"(acc[Z][1]), "+v"(acc[Z][2]), "+v"(acc[Z][3]));
-#pragma unroll
-            for (int q = 0; q < 4; q++) make_a(0, q);
-            float si = __uint_as_float(sa[0]);
+        }
+        float si = __uint_as_float(sa[0]);
+        fetch_a(1);
+#pragma clang loop unroll(disable)
+        while (true) {
+            const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
+            if (last && more) place(tile + per_xcd, nm0, nn0);
+            const int next_kb = last ? 0 : kb + 1;
+            const bool refill = last ? more : next_kb % PER == 0;
+            if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
+            float next_si = __uint_as_float(sa[1]);
+            fetch_a(2);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
+            multiply(0, si, [&](int q, int f) {
+                if (q == 0) make_b(f, 3);
+                make_a(1, q, f);
+            });
+            si = next_si;
+            fetch_a(3);
+            __builtin_amdgcn_sched_barrier(0);
+            next_si = __uint_as_float(sa[0]);
+            multiply(1, si, [&](int q, int f) { make_a(2, q, f); });
+            si = next_si;
+            wait_vm0();                                                           // the next stage
+            if (refill) { put_scales(chunk ^ 1); chunk ^= 1; }
+            stage ^= 1;
+            lds_barrier();                                                        // everyone's part of it, and this one has been read
+            if (next_kb + 1 == n_kb && tail < SCALE_BLOCK) cut_tail();
+            look(next_kb);
+            fetch_b();
+            fetch_a(0);
+            advance();
+            __builtin_amdgcn_sched_barrier(0);
+            next_si = __uint_as_float(sa[1]);
+            multiply(2, si, [&](int q, int f) {
+                make_a(3, q, f);
+                if (f == 3 && q < 3) issue(dkb, stage ^ 1, q);
+            });
+            si = next_si;
             fetch_a(1);
-#pragma unroll
-            for (int i = 0; i < Z; i++) {
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(i, 0, 4, si, [&](int q) { make_a(i + 1, q); });
-                si = __uint_as_float(sa[(i + 1) & 1]);
-                if (i + 2 < MI) fetch_a(i + 2);
-                // (nothing is executed here: the sums are made at this point, not sunk to the stores)
-                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
-            }
-            sz = si;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            multiply(3, si, [&](int q, int f) {
+                if (q > 0) make_b(f, q - 1);
+                make_a(0, q, f);
+                if (f == 3 && q < 3) issue(dkb, stage ^ 1, 3 + q);
+            });
+            si = __uint_as_float(sa[0]);
+            fetch_sb();
             if (last) {
-                multiply(Z, 0, 4, sz, nothing);
-                asm volatile("" : "+v"(acc[Z][0]), "+v"(acc[Z][1]), "+v"(acc[Z][2]), "+v"(acc[Z][3]));
+                finish();
+                if (!more) break;
+                tile += per_xcd; m0 = nm0; n0 = nn0;
+                clear();
             }
-        } else {
+            kb = next_kb;
+        }
+        wait_vm0();                                                               // what nobody reads has landed, too
+    } else {
+        // Fragment i + 2 of a is read while fragment i is multiplied, and a step's last fragment is multiplied behind the next barrier, while
+        // the next step's first ones come from LDS.
+        constexpr int SLOTS = MI == 4 ? 4 : 3;                                        // the carried fragment keeps its slot while fragment 0 is read
+        static_assert((MI - 1) % SLOTS != 0, "slots");
+        i32x8 fa[SLOTS], fb[4];
+        uint32_t sa[SLOTS], sb[4];                                                    // sb: the matrix unit's
+        f32x4v sbf[4];
+        float sb1 = 0.0f;
+#pragma clang loop unroll(disable)
+        while (true) {
+            const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
+            lds_barrier();
+            if (last && tail < SCALE_BLOCK) cut_tail();
+            if (last && more) {
+                place(tile + per_xcd, nm0, nn0);
+                aim(nm0, nn0);
+            }
+            const int next_kb = last ? 0 : kb + 1;
+            const bool refill = last ? more : next_kb % PER == 0;
+            if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
+
+            const uint8_t *la = &lds.stage[stage][0][0], *lb = &lds.stage[stage][1][0];
+            const int w = MODE == HW_SCALES ? (kb / 4) & (BIG_CH - 1) : kb & (BIG_CH - 1), sh = 8 * (kb & 3);
+            const uint32_t *sa_row = &lds.scale[chunk][0][w][ra0], *sb_row = &lds.scale[chunk][1][w][0];
+            auto read_a = [&](int i) { return join(*reinterpret_cast<const u32x4 *>(la + fa_at[0] + 2048 * i), *reinterpret_cast<const u32x4 *>(la + fa_at[1] + 2048 * i)); };
+            auto read_b = [&](int f) {
+                const int on = 128 * (b_at(f, 0) - b_at(0, 0));
+                return join(*reinterpret_cast<const u32x4 *>(lb + fb_at[0] + on), *reinterpret_cast<const u32x4 *>(lb + fb_at[1] + on));
+            };
+            auto bring = [&](int x) { issue(next_kb, stage ^ 1, x); };
             // One 16 x 16 x 128 product; shift: the byte of the scales' words that belongs to the step (HW_SCALES).
             auto multiply = [&](int i, int f, int shift) {
                 if constexpr (MODE == HW_SCALES) {
@@ -810,75 +967,16 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                 for (int f = 0; f < 4; f++) multiply(Z, f, sh);
                 pin(Z);
             }
-        }
-        wait_vm0();                                                               // the next stage; before the stores, which the same counter counts
-        if (refill) { put_scales(chunk ^ 1); chunk ^= 1; }
-        stage ^= 1;
-        kb = next_kb;
-        if (last) {
-            // 16-byte pieces of two rows change places between two lanes, so that 8 lanes store a row's 128 bytes with one instruction;
-            // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280: 121 -> 103 us).
-            {
-                constexpr int EACH = EXACT ? 4 : 8, ESIZE = EXACT ? 4 : 2;        // elements of a piece, bytes of one
-                const bool odd = lane & 1;
-                const int64_t row0 = (int64_t)m0 + wm + (r & ~1), line = p.n * ESIZE;
-                const int rows = p.m - row0 < BIG_M ? (int)(p.m - row0) : BIG_M;
-                int64_t at0 = (row0 * p.n + n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g)) * ESIZE;
-                const int64_t cols = p.n - ((int64_t)n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g));
-                bool nan = false;
-                float poison_in = 0.0f, poison_out = 0.0f;
-#pragma unroll
-                for (int i = 0; i < MI; i++) {
-#pragma unroll
-                    for (int pair = 0; pair < (EXACT ? 2 : 1); pair++) {
-                        // this lane's pieces in memory: number 0 (even lane) or 1 (odd) of the pair
-                        const int64_t at = at0 + (EXACT ? 32 * ESIZE * pair : 0);
-                        const bool in = cols > (EXACT ? 32 * pair : 0), here = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
-                        u32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                        if constexpr (BASE) {
-                            if (here) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at));
-                            if (below) c[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at + line));
-                            exchange(c[0], c[1], odd);
-                        }
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float v[EACH];
-#pragma unroll
-                            for (int j = 0; j < EACH; j++) {
-                                const float sum = EXACT ? acc[i][2 * pair + h][j & 3] : acc[i][2 * h + (j >> 2)][j & 3];
-                                if constexpr (BASE) {
-                                    const uint32_t word = EXACT ? c[h][j & 3] : c[h][j >> 1];
-                                    const uint32_t half = j & 1 ? word >> 16 : word & 0xffffu;
-                                    const float bb = EXACT ? __uint_as_float(word) : BF16 ? bf16_bits_to_f32(half) : f16_bits_to_f32(half);
-                                    v[j] = __builtin_fmaf(sum, p.alpha, bb);
-                                    poison_in = __builtin_fmaf(bb, 0.0f, poison_in);
-                                } else v[j] = sum * p.alpha;
-                            }
-                            // (rows and columns behind the last ones are made from the last ones, but without their base)
-                            if (p.flags && row0 + 16 * i + odd < p.m && (int64_t)n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g) < p.n) {
-#pragma unroll
-                                for (int j = 0; j < EACH; j++) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
-                            }
-                            if constexpr (EXACT) c[h] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                            else {
-#pragma unroll
-                                for (int j = 0; j < 4; j++) c[h][j] = BF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : pack_f16(v[2 * j], v[2 * j + 1]);
-                            }
-                        }
-                        exchange(c[0], c[1], odd);
-                        if (here) __builtin_nontemporal_store(c[0], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at));
-                        if (below) __builtin_nontemporal_store(c[1], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at + line));
-                    }
-                    at0 += 16 * line;
-                    asm volatile("" : "+v"(at0));                                 // (addresses one after the other, not all at once)
-                    if (i % 2) __builtin_amdgcn_sched_barrier(0);
-                }
-                nan |= poison_in != 0.0f;
-                if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+            wait_vm0();                                                               // the next stage; before the stores, which the same counter counts
+            if (refill) { put_scales(chunk ^ 1); chunk ^= 1; }
+            stage ^= 1;
+            kb = next_kb;
+            if (last) {
+                finish();
+                if (!more) break;
+                tile += per_xcd; m0 = nm0; n0 = nn0;
+                clear();
             }
-            if (!more) break;
-            tile += per_xcd; m0 = nm0; n0 = nn0;
-            clear();
         }
     }
 }
@@ -919,7 +1017,7 @@ int launch_big(int mi, const ProductParams &p, hipStream_t s) {
 //           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 82 (128 x 256).
 struct Choice { int direct = -1, mi = 0; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
 Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
-    static const double step[3][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.57, 1.82, 0.0, 0.0}};    // 128 x 128, MI = 4, 6, 8
+    static const double step[3][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.57, 1.60, 0.0, 0.0}};    // 128 x 128, MI = 4, 6, 8
     const double *us = step[mode == HW_SCALES ? 0 : mode == F32_SCALES ? 1 : 2];
     const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
     auto up = [](int64_t a, int64_t b) { return (double)((a + b - 1) / b); };
@@ -933,7 +1031,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
         }
     }
     static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
-    for (int d = 0; d < 4; d++) {
+    for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 32 us, 16 without it)
         const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * bytes / 5e6;
         const double t = 2.5 + (one > all ? one : all);
         if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.direct = d; }     // a launch's threads
@@ -975,7 +1073,7 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     // The large kernel stores and reads base in 16-byte pieces of the result's type, and reads scales four blocks at a time.
     const bool wide = out_dtype == MECHA_F32;
     const bool large_ok = k > 3 * SCALE_BLOCK && n % (wide ? 4 : 8) == 0 && mecha_aligned16(out) && (base == nullptr || (base_dtype == out_dtype && mecha_aligned16(base)));
-    const Choice c = choose(m, n, k, wide ? EXACT_F32 : e8m0 ? HW_SCALES : F32_SCALES, large_ok);
+    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, large_ok);
     if (c.direct >= 0) {
         if (wide) return e8m0 ? launch_direct<EXACT_E8M0>(c.direct, p, s) : launch_direct<EXACT_F32>(c.direct, p, s);
         return e8m0 ? launch_direct<HW_SCALES>(c.direct, p, s) : launch_direct<F32_SCALES>(c.direct, p, s);
