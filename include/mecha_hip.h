@@ -476,9 +476,12 @@ int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, u
 /* out[m][n] = base[m][n] + alpha * sum_k a[m][k] b[n][k], a and b block-scaled along k, both with scales of one type; base (may be
  * NULL: zeros) and out contiguous, out may be base.  Sums in float32, one rounding to out_dtype; for a 16-bit out_dtype the products of 8
  * neighbouring k are first cut off under 2^-13 of the largest of them (the 8-bit matrix instructions).  bit 0 of flags: a NaN came out
- * or base holds inf / NaN; bit 1: an output is inf / NaN. */
+ * or base holds inf / NaN; bit 1: an output is inf / NaN.  out shares no memory with a, b or (but for out == base) base. */
 int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
-                        float alpha, uint32_t *flags, void *stream);
+                        float alpha, uint32_t *flags, void *workspace, size_t workspace_bytes, void *stream);
+/* What a product of m x n results over k can use (0 for most): float32 sums of parts of k, for results too few to fill the chip.  With
+ * less, or NULL, k is not shared out. */
+size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int out_dtype);
 
 /* ------------------------------------------------------------------ training step
  * One AdamW step (decoupled weight decay) for every key of the arenas, in place, in one launch:

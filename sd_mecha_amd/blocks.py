@@ -5,6 +5,7 @@ a ROCm device, works on the current stream and has no CPU path.  No counterpart 
 from __future__ import annotations
 
 from contextlib import nullcontext
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -166,6 +167,11 @@ def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check
     return out
 
 
+@lru_cache(maxsize=4096)
+def _product_workspace(m: int, n: int, k: int, scale_code: int, out_code: int) -> int:
+    return _lib.lib().mecha_block_product_workspace_bytes(m, n, k, scale_code, out_code)
+
+
 def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] = None, alpha: float = 1.0, *, out: Optional[torch.Tensor] = None,
                   key=None, out_dtype=None, flags=None, check_finite: bool = True) -> torch.Tensor:
     """``base + alpha * a @ b.T`` (``base=None``: ``alpha * a @ b.T``) of two 8-bit matrices a [m, k], b [n, k], summed in float32 and rounded once to
@@ -212,9 +218,11 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         a, b = (q if q.scale_code == SCALE_F32 else BlockScaled(q.values, q.scales.to(torch.float32)) for q in (a, b))
     with _on(device):
         word, fl = _flags(device, flags, check_finite)
+        size = _product_workspace(m, n, k, a.scale_code, _DT[out.dtype])
+        room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _lib.check(_lib.lib().mecha_block_product(
             a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),
-            _DT[out.dtype], alpha, word, _stream(device)), "mecha_block_product")
+            _DT[out.dtype], alpha, word, room.data_ptr() if size else None, size, _stream(device)), "mecha_block_product")
         if fl is not None:
             fl.finish(key)
     return out

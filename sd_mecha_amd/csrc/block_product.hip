@@ -34,6 +34,7 @@ struct ProductParams {
     float alpha;
     uint32_t *flags;
     int tiles_m, tiles_n;
+    int splits;                        // the large kernel: parts of k, each with a result of its own, m * n float32 behind the one before
 };
 
 // global -> LDS: lane l's 16 bytes at base + off go to dst + 16 l (dst wave-uniform).  Inline assembly because the compiler cannot tell
@@ -505,9 +506,15 @@ int launch_direct(int shape, const ProductParams &p, hipStream_t s) {
 // 32 MI x 256 outputs by 8 waves of 16 MI x 64, one workgroup a CU that goes on from tile to tile.  A K step is one block of 128: up to
 // 64 KiB of codes in one of two LDS stages, 4 MI matrix instructions a wave (16 MI for float32 results).  The next step's codes -- the next
 // tile's at a tile's end -- are on their way while this one is multiplied, also over the epilogue; so are the scales of the next BIG_CH
-// words of blocks.  One barrier a step: behind it every wave's part of this stage has landed and the other stage has been read.
+// words of blocks.  One barrier a step: behind it every wave's part of the next stage has landed and the other stage has been read.
 // Workgroups go round the 8 XCDs, each with its own L2: an XCD gets a run of tiles, ordered so that the 32 at work at a time are 8 x 4
 // tiles (2 MiB of a and 1 MiB of b at k = 1024, MI = 8).
+//
+// Measured (no base): 8192 x 8192 x 8192 457 us (2.4 PFLOP/s; the matrix unit's own rate is 4.3, and a plain per-tensor library product takes 421);
+// 8192 x 10240 x 1280 105 us (2.0 PFLOP/s, 168 MB of results at 1.6 TB/s; the library 108); 8269 x 1280 x 5120 58 us (float32 scales: 64).  A
+// 256 x 256 step takes 3900 cycles: 2048 of products at the unit's rate, and 1600 in which its 64 KiB come from L2 to LDS, which overlap
+// only in part: fewer or more of them asked for at a step's start, by four waves or by eight, made no difference.  Float32 results
+// multiply at bfloat16's rate (2.1 PFLOP/s): 1280 x 5120 x 8269 102 us (1.06 PFLOP/s on 200 of the 256 CUs).
 constexpr int BIG_N = 256, BIG_M = 256, BIG_THREADS = 512, BIG_CH = 4, BIG_CUS = 256, BIG_BAND = 8;
 struct BigLds {
     uint8_t stage[2][2][BIG_M * 128];             // [stage][a, b][row][128]
@@ -531,11 +538,13 @@ __device__ __forceinline__ void exchange(u32x4 &c0, u32x4 &c1, bool odd) {
         c1[j] = odd ? c1[j] : got;
     }
 }
-template <int MODE, bool B_UNIFORM, int MI, bool BF16, bool BASE>
+template <int MODE, bool B_UNIFORM, int MI, int OUT, bool BASE>
 __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[];
     BigLds &lds = *reinterpret_cast<BigLds *>(lds_raw);
-    constexpr bool EXACT = MODE == EXACT_F32 || MODE == EXACT_E8M0;              // float32 results
+    constexpr bool EXACT = MODE == EXACT_F32 || MODE == EXACT_E8M0;              // float32 results; else float32 (OUT) are the sums of a part of k
+    constexpr bool BF16 = OUT == MECHA_BF16;
+    const uint32_t splits = MI == 4 && OUT == MECHA_F32 && !BASE ? (uint32_t)p.splits : 1u;
     constexpr int ROWS = 32 * MI, PER = MODE == HW_SCALES ? 4 * BIG_CH : BIG_CH; // rows of a tile; blocks a chunk of scales
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int g = lane >> 4, r = lane & 15;
@@ -543,18 +552,29 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     const int n_kb = (int)((p.k + SCALE_BLOCK - 1) / SCALE_BLOCK);
     const int tail = (int)(p.k - (int64_t)(n_kb - 1) * SCALE_BLOCK);
 
-    // this workgroup's tiles: every (gridDim / 8)-th of its XCD's run
-    const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;             // < 2^24
+    // this workgroup's tiles: every (gridDim / 8)-th of its XCD's run (of the tiles of the first part of k, then the second, ...)
+    const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n, all_tiles = tiles * splits;                   // < 2^24
     const uint32_t xcd = blockIdx.x & 7, per_xcd = gridDim.x >> 3;
-    const uint32_t run0 = tiles * xcd / 8, run1 = tiles * (xcd + 1) / 8;
+    const uint32_t run0 = all_tiles * xcd / 8, run1 = all_tiles * (xcd + 1) / 8;
     uint32_t tile = run0 + (blockIdx.x >> 3);
     if (tile >= run1) return;
-    // bands of BIG_BAND rows of tiles, down the band first
-    auto place = [&](uint32_t i, uint32_t &m0, uint32_t &n0) {
+    // bands of BIG_BAND rows of tiles, down the band first; blocks k0 .. k0 + count - 1 of k
+    struct Place { uint32_t m0, n0, part; int k0, count; };
+    auto one = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };      // the same in every lane
+    auto place = [&](uint32_t i) {
+        Place at;
+        at.part = splits > 1 ? one(i / tiles) : 0u;
+        i -= at.part * tiles;
         const uint32_t band_tiles = BIG_BAND * (uint32_t)p.tiles_n, band = i / band_tiles, in = i - band * band_tiles;
         const uint32_t left = (uint32_t)p.tiles_m - band * BIG_BAND, high = left < BIG_BAND ? left : BIG_BAND;
-        n0 = in / high * BIG_N;
-        m0 = (band * BIG_BAND + in % high) * ROWS;
+        at.n0 = one(in / high * BIG_N);
+        at.m0 = one((band * BIG_BAND + in % high) * ROWS);
+        at.k0 = 0; at.count = n_kb;
+        if (splits > 1) {
+            at.k0 = (int)one((uint32_t)n_kb * at.part / splits);
+            at.count = (int)one((uint32_t)n_kb * (at.part + 1) / splits) - at.k0;
+        }
+        return at;
     };
 
     // b's rows of fragment f: 16-bit results: 8 contiguous columns a lane and pair of fragments; float32: 4 a fragment
@@ -567,11 +587,11 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     const uint32_t part_a = 16u * (uint32_t)((lane & 7) ^ swz_a(bring_row)), part_b = 16u * (uint32_t)((lane & 7) ^ swz_n(bring_row));
     int last_a, last_b;
     const uint8_t *ga, *gb;
-    auto aim = [&](uint32_t m0, uint32_t n0) {
-        last_a = p.m - 1 - m0 < BIG_M ? (int)(p.m - 1 - m0) : BIG_M;
-        last_b = p.n - 1 - n0 < BIG_N ? (int)(p.n - 1 - n0) : BIG_N;
-        ga = p.a + (int64_t)m0 * p.a_pitch;
-        gb = p.b + (int64_t)n0 * p.b_pitch;
+    auto aim = [&](const Place &at) {
+        last_a = p.m - 1 - at.m0 < BIG_M ? (int)(p.m - 1 - at.m0) : BIG_M;
+        last_b = p.n - 1 - at.n0 < BIG_N ? (int)(p.n - 1 - at.n0) : BIG_N;
+        ga = p.a + (int64_t)at.m0 * p.a_pitch + (int64_t)at.k0 * SCALE_BLOCK;
+        gb = p.b + (int64_t)at.n0 * p.b_pitch + (int64_t)at.k0 * SCALE_BLOCK;
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte *)lds_raw) + (uint32_t)wave * 1024u;
     auto issue = [&](int kb, int to, int x) {                                     // piece x: b's four, then a's
@@ -629,10 +649,9 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
 #pragma unroll
             for (int f = 0; f < 4; f++) acc[i][f] = f32x4v{0, 0, 0, 0};
     };
-    uint32_t m0, n0, nm0 = 0, nn0 = 0;
-    place(tile, m0, n0);
-    aim(m0, n0);
-    load_scales(m0, n0, 0);
+    Place here = place(tile), next = here;
+    aim(here);
+    load_scales(here.m0, here.n0, here.k0);
 #pragma unroll
     for (int x = 0; x < PIECES; x++) issue(0, 0, x);
     put_scales(0);
@@ -652,14 +671,25 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         lds_barrier();
     };
     auto finish = [&]() {
+        if constexpr (!EXACT && OUT == MECHA_F32) {                                // a part's sums; what joins the parts reads them from the caches
+            float *const out = static_cast<float *>(p.out) + (int64_t)here.part * p.m * p.n;
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    const int64_t m = (int64_t)here.m0 + wm + 16 * i + r, n = (int64_t)here.n0 + wn + b_row(f) + 8 * g;
+                    if (m < p.m && n < p.n) *reinterpret_cast<f32x4v *>(out + m * p.n + n) = acc[i][f];
+                }
+            return;
+        }
         // 16-byte pieces of two rows change places between two lanes, so that 8 lanes store a row's 128 bytes with one instruction;
         // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280: 121 -> 103 us).
         constexpr int EACH = EXACT ? 4 : 8, ESIZE = EXACT ? 4 : 2;        // elements of a piece, bytes of one
         const bool odd = lane & 1;
-        const int64_t row0 = (int64_t)m0 + wm + (r & ~1), line = p.n * ESIZE;
+        const int64_t row0 = (int64_t)here.m0 + wm + (r & ~1), line = p.n * ESIZE;
         const int rows = p.m - row0 < BIG_M ? (int)(p.m - row0) : BIG_M;
-        int64_t at0 = (row0 * p.n + n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g)) * ESIZE;
-        const int64_t cols = p.n - ((int64_t)n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g));
+        int64_t at0 = (((int64_t)here.part * p.m + row0) * p.n + here.n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g)) * ESIZE;
+        const int64_t cols = p.n - ((int64_t)here.n0 + wn + (EXACT ? 16 * odd + 4 * g : 32 * odd + 8 * g));
         bool nan = false;
         float poison_in = 0.0f, poison_out = 0.0f;
 #pragma unroll
@@ -668,10 +698,10 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             for (int pair = 0; pair < (EXACT ? 2 : 1); pair++) {
                 // this lane's pieces in memory: number 0 (even lane) or 1 (odd) of the pair
                 const int64_t at = at0 + (EXACT ? 32 * ESIZE * pair : 0);
-                const bool in = cols > (EXACT ? 32 * pair : 0), here = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
+                const bool in = cols > (EXACT ? 32 * pair : 0), above = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
                 u32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
                 if constexpr (BASE) {
-                    if (here) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at));
+                    if (above) c[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at));
                     if (below) c[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.base) + at + line));
                     exchange(c[0], c[1], odd);
                 }
@@ -690,7 +720,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                         } else v[j] = sum * p.alpha;
                     }
                     // (rows and columns behind the last ones are made from the last ones, but without their base)
-                    if (p.flags && row0 + 16 * i + odd < p.m && (int64_t)n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g) < p.n) {
+                    if (p.flags && row0 + 16 * i + odd < p.m && (int64_t)here.n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g) < p.n) {
 #pragma unroll
                         for (int j = 0; j < EACH; j++) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
                     }
@@ -701,7 +731,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                     }
                 }
                 exchange(c[0], c[1], odd);
-                if (here) __builtin_nontemporal_store(c[0], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at));
+                if (above) __builtin_nontemporal_store(c[0], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at));
                 if (below) __builtin_nontemporal_store(c[1], reinterpret_cast<u32x4 *>(static_cast<char *>(p.out) + at + line));
             }
             at0 += 16 * line;
@@ -723,16 +753,16 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         uint32_t sa[2], rawscale[4];
         f32x4v sbf[4];
         i32x4 aq[2][4], bq[4][4];                                                // [fragment][quarter] of a and b
-        int dkb = 0;                                                              // the step that was asked for last
+        int dkb = 0, dcount = here.count;                                         // the step that was asked for last
         uint32_t dtile = tile;
         auto advance = [&]() {                                                    // (behind the last tile it stays, and fetches what nobody reads)
-            if (++dkb < n_kb) return;
+            if (++dkb < dcount) return;
             dkb = 0;
             if (dtile + per_xcd >= run1) return;
             dtile += per_xcd;
-            uint32_t dm, dn;
-            place(dtile, dm, dn);
-            aim(dm, dn);
+            const Place to = place(dtile);
+            dcount = to.count;
+            aim(to);
         };
         const uint8_t *la = nullptr, *lb = nullptr;
         const uint32_t *sa_row = nullptr, *sb_row = nullptr;
@@ -821,11 +851,11 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         fetch_a(1);
 #pragma clang loop unroll(disable)
         while (true) {
-            const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
-            if (last && more) place(tile + per_xcd, nm0, nn0);
+            const bool last = kb + 1 == here.count, more = tile + per_xcd < run1;
+            if (last && more) next = place(tile + per_xcd);
             const int next_kb = last ? 0 : kb + 1;
             const bool refill = last ? more : next_kb % PER == 0;
-            if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
+            if (refill) load_scales(last ? next.m0 : here.m0, last ? next.n0 : here.n0, last ? next.k0 : here.k0 + next_kb);
             float next_si = __uint_as_float(sa[1]);
             fetch_a(2);
             __builtin_amdgcn_sched_barrier(0);
@@ -844,7 +874,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             if (refill) { put_scales(chunk ^ 1); chunk ^= 1; }
             stage ^= 1;
             lds_barrier();                                                        // everyone's part of it, and this one has been read
-            if (next_kb + 1 == n_kb && tail < SCALE_BLOCK) cut_tail();
+            if (next_kb + 1 == here.count && here.k0 + here.count == n_kb && tail < SCALE_BLOCK) cut_tail();
             look(next_kb);
             fetch_b();
             fetch_a(0);
@@ -869,7 +899,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             if (last) {
                 finish();
                 if (!more) break;
-                tile += per_xcd; m0 = nm0; n0 = nn0;
+                tile += per_xcd; here = next;
                 clear();
             }
             kb = next_kb;
@@ -886,16 +916,16 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         float sb1 = 0.0f;
 #pragma clang loop unroll(disable)
         while (true) {
-            const bool last = kb + 1 == n_kb, more = tile + per_xcd < run1;
+            const bool last = kb + 1 == here.count, more = tile + per_xcd < run1;
             lds_barrier();
-            if (last && tail < SCALE_BLOCK) cut_tail();
+            if (last && here.k0 + here.count == n_kb && tail < SCALE_BLOCK) cut_tail();
             if (last && more) {
-                place(tile + per_xcd, nm0, nn0);
-                aim(nm0, nn0);
+                next = place(tile + per_xcd);
+                aim(next);
             }
             const int next_kb = last ? 0 : kb + 1;
             const bool refill = last ? more : next_kb % PER == 0;
-            if (refill) load_scales(last ? nm0 : m0, last ? nn0 : n0, next_kb);
+            if (refill) load_scales(last ? next.m0 : here.m0, last ? next.n0 : here.n0, last ? next.k0 : here.k0 + next_kb);
 
             const uint8_t *la = &lds.stage[stage][0][0], *lb = &lds.stage[stage][1][0];
             const int w = MODE == HW_SCALES ? (kb / 4) & (BIG_CH - 1) : kb & (BIG_CH - 1), sh = 8 * (kb & 3);
@@ -974,38 +1004,94 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             if (last) {
                 finish();
                 if (!more) break;
-                tile += per_xcd; m0 = nm0; n0 = nn0;
+                tile += per_xcd; here = next;
                 clear();
             }
         }
     }
 }
 
-template <int MODE, bool B_UNIFORM, int MI>
-int launch_big(ProductParams p, hipStream_t s) {
+// The parts of k together: out = base + alpha * (part 0 + part 1 + ...), added in that order in float32.  4 elements a thread; the parts
+// come out of the caches, 6 TB/s and more.
+template <int DT, bool BASE>
+__global__ __launch_bounds__(MECHA_BLOCK) void join_kernel(const float *parts, int splits, int64_t count, const void *base, void *out, float alpha, uint32_t *flags) {
+    const int64_t i = ((int64_t)blockIdx.x * MECHA_BLOCK + threadIdx.x) * 4;
+    if (i >= count) return;
+    f32x4v sum = *reinterpret_cast<const f32x4v *>(parts + i);
+    const float *at = parts + i;
+#pragma unroll 4
+    for (int x = 1; x < splits; x++) {
+        at += count;
+        const f32x4v v = *reinterpret_cast<const f32x4v *>(at);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] += v[e];
+    }
+    float v[4], poison_in = 0.0f, poison_out = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float b = BASE ? load1<DT>(base, i + e) : 0.0f;
+        v[e] = BASE ? __builtin_fmaf(sum[e], alpha, b) : sum[e] * alpha;
+        poison_in = __builtin_fmaf(b, 0.0f, poison_in);
+        poison_out = __builtin_fmaf(v[e], 0.0f, poison_out);
+        nan |= v[e] != v[e];
+    }
+    if constexpr (DT == MECHA_F32) *reinterpret_cast<f32x4v *>(static_cast<float *>(out) + i) = f32x4v{v[0], v[1], v[2], v[3]};
+    else
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + i) =
+            DT == MECHA_BF16 ? u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])} : u32x2{pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
+    nan |= poison_in != 0.0f;
+    if (flags && (nan || poison_out != 0.0f)) atomicOr(flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+}
+int launch_join(const ProductParams &p, const void *parts, hipStream_t s) {
+    const int64_t count = p.m * p.n, blocks = (count / 4 + MECHA_BLOCK - 1) / MECHA_BLOCK;      // n is a multiple of 4
+    auto go = [&](auto dt, auto base) {
+        MECHA_LAUNCH(MK_BLOCKS_PRODUCT, (join_kernel<decltype(dt)::value, decltype(base)::value>), dim3((unsigned)blocks), dim3(MECHA_BLOCK), 0, s, static_cast<const float *>(parts),
+                     p.splits, count, p.base, p.out, p.alpha, p.flags);
+    };
+    auto with_base = [&](auto dt) { if (p.base) go(dt, std::true_type{}); else go(dt, std::false_type{}); };
+    switch (p.out_dt) {
+        case MECHA_F32: with_base(std::integral_constant<int, MECHA_F32>{}); break;
+        case MECHA_F16: with_base(std::integral_constant<int, MECHA_F16>{}); break;
+        default: with_base(std::integral_constant<int, MECHA_BF16>{}); break;
+    }
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+
+template <int MODE, bool B_UNIFORM, int MI, int OUT, bool BASE>
+int launch_tiles(ProductParams p, hipStream_t s) {
     p.tiles_m = (int)((p.m + 32 * MI - 1) / (32 * MI));
     p.tiles_n = (int)((p.n + BIG_N - 1) / BIG_N);
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, grid = tiles < BIG_CUS ? (tiles + 7) / 8 * 8 : BIG_CUS;
-    auto go = [&](auto bf16, auto base) -> int {
-        auto *const kernel = &product_big_kernel<MODE, B_UNIFORM, MI, decltype(bf16)::value, decltype(base)::value>;
-        MECHA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BigLds)));
-        MECHA_LAUNCH(MK_BLOCKS_PRODUCT, kernel, dim3((unsigned)grid), dim3(BIG_THREADS), sizeof(BigLds), s, p);
-        MECHA_CHECK_HIP(hipGetLastError());
-        return MECHA_OK;
-    };
-    auto with_base = [&](auto bf16) { return p.base ? go(bf16, std::true_type{}) : go(bf16, std::false_type{}); };
-    if constexpr (MODE == HW_SCALES || MODE == F32_SCALES) {
-        if (p.out_dt == MECHA_F16) return with_base(std::false_type{});
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits, grid = tiles < BIG_CUS ? (tiles + 7) / 8 * 8 : BIG_CUS;
+    auto *const kernel = &product_big_kernel<MODE, B_UNIFORM, MI, OUT, BASE>;
+    MECHA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BigLds)));
+    MECHA_LAUNCH(MK_BLOCKS_PRODUCT, kernel, dim3((unsigned)grid), dim3(BIG_THREADS), sizeof(BigLds), s, p);
+    MECHA_CHECK_HIP(hipGetLastError());
+    return MECHA_OK;
+}
+template <int MODE, bool B_UNIFORM, int MI>
+int launch_big(const ProductParams &p, void *workspace, hipStream_t s) {
+    constexpr bool EXACT = MODE == EXACT_F32 || MODE == EXACT_E8M0;
+    if constexpr (MI == 4) {
+        if (p.splits > 1) {
+            ProductParams part = p;
+            part.out = workspace; part.out_dt = MECHA_F32; part.base = nullptr; part.alpha = 1.0f; part.flags = nullptr;
+            const int st = launch_tiles<MODE, B_UNIFORM, MI, MECHA_F32, false>(part, s);
+            return st ? st : launch_join(p, workspace, s);
+        }
     }
-    return with_base(std::true_type{});
+    if constexpr (EXACT) return p.base ? launch_tiles<MODE, B_UNIFORM, MI, MECHA_F32, true>(p, s) : launch_tiles<MODE, B_UNIFORM, MI, MECHA_F32, false>(p, s);
+    else if (p.out_dt == MECHA_F16) return p.base ? launch_tiles<MODE, B_UNIFORM, MI, MECHA_F16, true>(p, s) : launch_tiles<MODE, B_UNIFORM, MI, MECHA_F16, false>(p, s);
+    else return p.base ? launch_tiles<MODE, B_UNIFORM, MI, MECHA_BF16, true>(p, s) : launch_tiles<MODE, B_UNIFORM, MI, MECHA_BF16, false>(p, s);
 }
 template <int MODE, bool B_UNIFORM>
-int launch_big(int mi, const ProductParams &p, hipStream_t s) {
+int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
     if constexpr (MODE == HW_SCALES || MODE == F32_SCALES) {
-        if (mi == 8) return launch_big<MODE, B_UNIFORM, 8>(p, s);
-        if (mi == 6) return launch_big<MODE, B_UNIFORM, 6>(p, s);
+        if (mi == 8) return launch_big<MODE, B_UNIFORM, 8>(p, workspace, s);
+        if (mi == 6) return launch_big<MODE, B_UNIFORM, 6>(p, workspace, s);
     }
-    return launch_big<MODE, B_UNIFORM, 4>(p, s);
+    return launch_big<MODE, B_UNIFORM, 4>(p, workspace, s);
 }
 
 // ---------------------------------------------------------------------------------------------------- which kernel
@@ -1015,8 +1101,12 @@ int launch_big(int mi, const ProductParams &p, hipStream_t s) {
 //   tiled:  rounds of tiles over the CUs, each n_kb steps and an epilogue.  128 x 128 tiles (two workgroups a CU) fill a few CUs more evenly:
 //           1024 x 1280 x 5120 36 us, 49 with 128 x 256 tiles; the larger ones share more: 8192 x 1280 x 5120 57 us (192 x 256), 80 with
 //           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 82 (128 x 256).
-struct Choice { int direct = -1, mi = 0; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
-Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
+//   in parts: results of fewer 128 x 256 tiles than CUs, k shared out among 2 to 32 workgroups a tile (4 blocks at least each): the parts are written
+//           and read once as float32 and joined by a second launch: 1280 x 1280 x 8269 32 us in 5 parts (55 in one; float32 results 39 and 100),
+//           1024 x 1280 x 5120 25 (36), 300 x 2560 x 8192 24 (53); 320 x 320 x 8269 stays with the direct kernel: 15 us, 16 in 13 parts.
+constexpr int MAX_SPLITS = 32;
+struct Choice { int direct = -1, mi = 0, splits = 1; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
+Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok, bool split_ok) {
     static const double step[3][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.57, 1.60, 0.0, 0.0}};    // 128 x 128, MI = 4, 6, 8
     const double *us = step[mode == HW_SCALES ? 0 : mode == F32_SCALES ? 1 : 2];
     const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
@@ -1029,12 +1119,17 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
             const double rounds = up((int64_t)(up(m, 32 * mi) * up(n, BIG_N)), BIG_CUS), t = 1.5 + rounds * (n_kb * us[mi / 2 - 1] + 0.25 * mi);
             if (t < best) { best = t; c.mi = mi; }
         }
+        const double tiles = up(m, 128) * up(n, BIG_N), part = (double)m * (double)n * 8.0 / 5e6;
+        for (int x = 2; split_ok && x <= MAX_SPLITS && 4 * x <= n_kb && (x - 1) * tiles < BIG_CUS; x++) {
+            const double rounds = up((int64_t)tiles * x, BIG_CUS), t = 8.5 + rounds * (up((int64_t)n_kb, x) * us[1] + 1.0) + x * part;
+            if (t < best) { best = t; c.mi = 4; c.splits = x; }
+        }
     }
     static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
     for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 32 us, 16 without it)
         const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * bytes / 5e6;
         const double t = 2.5 + (one > all ? one : all);
-        if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.direct = d; }     // a launch's threads
+        if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.splits = 1; c.direct = d; }     // a launch's threads
     }
     return c;
 }
@@ -1043,8 +1138,15 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok) {
 
 extern "C" {
 
+size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int out_dtype) {
+    const bool wide = out_dtype == MECHA_F32, e8m0 = scale_dtype == MECHA_SCALE_E8M0;
+    if (m < 1 || n < 1 || k <= 3 * SCALE_BLOCK || n % (wide ? 4 : 8) != 0) return 0;
+    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, true, true);
+    return c.splits > 1 ? (size_t)c.splits * (size_t)m * (size_t)n * sizeof(float) : 0;
+}
+
 int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
-                        float alpha, uint32_t *flags, void *stream) {
+                        float alpha, uint32_t *flags, void *workspace, size_t workspace_bytes, void *stream) {
     MECHA_REQUIRE(a != nullptr && b != nullptr, "a matrix is NULL");
     MECHA_REQUIRE(mecha_valid_dtype(out_dtype) && (base == nullptr || mecha_valid_dtype(base_dtype)), "unknown dtype code (base %d, out %d)", base_dtype, out_dtype);
     int st = mecha_check_blocks("a", *a);
@@ -1066,22 +1168,25 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     MECHA_REQUIRE(base == nullptr || (base == out && base_dtype == out_dtype) || !mecha_overlap(out, out_bytes, base, (size_t)m * n * mecha_dtype_size(base_dtype)),
                   "out may be base itself, of the same dtype, but not overlap it otherwise");
     ProductParams p{static_cast<const uint8_t *>(a->codes), a->pitch, a->scales, a->scale_pitch, a->tile, static_cast<const uint8_t *>(b->codes), b->pitch,
-                    b->scales, b->scale_pitch, b->tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn};
+                    b->scales, b->scale_pitch, b->tile, base, out, m, n, k, base_dtype, out_dtype, alpha, flags, (int)tm, (int)tn, 1};
     const int b_tile = b->tile, scale_dtype = a->scale_dtype;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
     // The large kernel stores and reads base in 16-byte pieces of the result's type, and reads scales four blocks at a time.
     const bool wide = out_dtype == MECHA_F32;
     const bool large_ok = k > 3 * SCALE_BLOCK && n % (wide ? 4 : 8) == 0 && mecha_aligned16(out) && (base == nullptr || (base_dtype == out_dtype && mecha_aligned16(base)));
-    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, large_ok);
+    const int mode = wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES;
+    Choice c = choose(m, n, k, mode, large_ok, workspace != nullptr);
+    if (c.splits > 1 && ((size_t)c.splits * (size_t)m * (size_t)n * sizeof(float) > workspace_bytes || !mecha_aligned16(workspace))) c = choose(m, n, k, mode, large_ok, false);
+    p.splits = c.splits;
     if (c.direct >= 0) {
         if (wide) return e8m0 ? launch_direct<EXACT_E8M0>(c.direct, p, s) : launch_direct<EXACT_F32>(c.direct, p, s);
         return e8m0 ? launch_direct<HW_SCALES>(c.direct, p, s) : launch_direct<F32_SCALES>(c.direct, p, s);
     }
     if (c.mi) {
-        if (wide) return e8m0 ? launch_big<EXACT_E8M0, false>(c.mi, p, s) : launch_big<EXACT_F32, false>(c.mi, p, s);
-        if (e8m0) return launch_big<HW_SCALES, false>(c.mi, p, s);
-        return b_tile ? launch_big<F32_SCALES, true>(c.mi, p, s) : launch_big<F32_SCALES, false>(c.mi, p, s);
+        if (wide) return e8m0 ? launch_big<EXACT_E8M0, false>(c.mi, p, workspace, s) : launch_big<EXACT_F32, false>(c.mi, p, workspace, s);
+        if (e8m0) return launch_big<HW_SCALES, false>(c.mi, p, workspace, s);
+        return b_tile ? launch_big<F32_SCALES, true>(c.mi, p, workspace, s) : launch_big<F32_SCALES, false>(c.mi, p, workspace, s);
     }
     auto go = [&](auto mode, auto dt) {
         constexpr int MODE = decltype(mode)::value, DT = decltype(dt)::value;

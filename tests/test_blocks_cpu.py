@@ -155,11 +155,16 @@ def test_c_entries_refuse_before_any_launch():
         assert un(**bad) < 0, bad
 
     def prod(a=matrix(), b=matrix(), base=None, bdt=0, out=at, odt=0):
-        return L.mecha_block_product(a, b, base, bdt, out, odt, 1.0, None, None)
+        return L.mecha_block_product(a, b, base, bdt, out, odt, 1.0, None, None, 0, None)
     for bad in (dict(a=matrix(rows=-1)), dict(a=matrix(cols=0), b=matrix(cols=0)), dict(a=matrix(cols=99)), dict(odt=3), dict(base=at, bdt=4), dict(a=matrix(sdt=2)),
                 dict(a=matrix(sdt=0)), dict(out=None), dict(a=None), dict(b=None), dict(a=matrix(codes=0)), dict(b=matrix(pitch=127)), dict(a=matrix(sp=0)),
                 dict(a=matrix(pitch=1 << 25)), dict(b=matrix(codes=at + 4)), dict(a=matrix(rows=1 << 20), b=matrix(rows=1 << 30)), dict(a=matrix(rows=1 << 31))):
         assert prod(**bad) < 0, bad
+
+    room = L.mecha_block_product_workspace_bytes
+    assert [room(*x) for x in ((0, 128, 4096, 1, 0), (128, -1, 4096, 1, 0), (1, 1280, 2816, 1, 2), (640, 641, 8192, 1, 0), (8192, 10240, 1280, 1, 2), (640, 640, 384, 1, 0))] == [0] * 6
+    for x in ((640, 640, 8192, 1, 2), (1280, 1280, 8192, 0, 0)):
+        assert room(*x) % (4 * x[0] * x[1]) == 0 and room(*x) >= 8 * x[0] * x[1]
 
     def ad(**k):
         return L.mecha_batched_adamw(packed(_lib.ADAMW, (

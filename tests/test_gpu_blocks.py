@@ -274,6 +274,52 @@ def test_product_middle(m, n, k, scales, dtype):
     assert torch.equal(amd.block_product(a, b, base.to(dtype), 2.0 ** -7, out=room[1:]).view(m, n), want)
 
 
+# few tiles and many blocks of k, whose parts are multiplied apart and joined
+PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4100), (900, 264, 8192)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", PARTS)
+def test_product_in_parts(m, n, k, scales, dtype):
+    import sd_mecha_amd as amd
+    assert amd.blocks._product_workspace(m, n, k, int(scales == "e8m0"), 0 if dtype == torch.float32 else 1) >= 2 * 4 * m * n
+    for fb in ("tile", "rows"):
+        a, b = matrix(m, k, "rows", scales, m + 3), matrix(n, k, fb, scales, n + 4)
+        a = amd.BlockScaled(a.values, (a.scales.float() / 2.0 ** 17).to(a.scales.dtype))
+        check_product(amd.block_product(a, b, out_dtype=dtype), a, b)
+        base = torch.randn(m, n, device="cuda").to(dtype)
+        out = base.clone()
+        assert amd.block_product(a, b, out, -2.0, out=out) is out
+        check_product(out, a, b, base, -2.0)
+        room = torch.empty(m * n + 1, dtype=dtype, device="cuda")                   # not in parts: 2 or 4 bytes off
+        check_product(amd.block_product(a, b, base, 0.5, out=room[1:]).view(m, n), a, b, base, 0.5)
+    v = a.values.clone()
+    v.view(torch.uint8)[m - 1, k - 1] = 0x7F
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = amd.block_product(amd.BlockScaled(v, a.scales), b, out_dtype=dtype, flags=flags, check_finite=False)
+    # (float16: many results are over 65504 and infinite)
+    assert int(flags) & 1 and bool(got[m - 1].isnan().all()) and not bool(got[:m - 1].isnan().any())
+    base[0, n - 1] = float("inf")
+    with pytest.raises(amd.NonFiniteStateDictKeyError):
+        amd.block_product(a, b, base, out_dtype=dtype)
+
+
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+def test_product_with_too_little_room_for_parts(scales):
+    """The C entry with no, a short and the whole workspace: the same sums, in float32's rounding."""
+    import sd_mecha_amd as amd
+    L, (m, n, k) = amd._lib.lib(), PARTS[1]
+    a, b = matrix(m, k, "rows", scales, 1, ints=True), matrix(n, k, "tile", scales, 2, ints=True)
+    want = torch.from_numpy(R.values(a) @ R.values(b).T).float().cuda()
+    size = L.mecha_block_product_workspace_bytes(m, n, k, a.scale_code, 0)
+    room = torch.empty(size, dtype=torch.uint8, device="cuda")
+    for at, given in ((None, 0), (room.data_ptr(), size - 1), (room.data_ptr(), size), (room.data_ptr() + 4, size - 4)):
+        out = torch.empty(m, n, device="cuda")
+        amd._lib.check(L.mecha_block_product(a._packed, b._packed, None, 0, out.data_ptr(), 0, 1.0, None, at, given, torch.cuda.current_stream().cuda_stream), "product")
+        assert torch.equal(out, want), given
+
+
 def test_product_extreme_scales():
     """Powers of two from 2^-127 on one side against large ones on the other."""
     import sd_mecha_amd as amd
@@ -470,7 +516,7 @@ def test_same_result_every_time_on_any_stream_and_in_a_graph():
 def test_large_products_in_a_graph_and_side_by_side(scales, dtype):
     """Results of many tiles, of every kind of kernel, captured together and replayed next to the same products on another stream."""
     import sd_mecha_amd as amd
-    pairs = [(matrix(m, k, "rows", scales, m), matrix(n, k, "tile", scales, n)) for m, n, k in ((2100, 2056, 1100), (2100, 1003, 700), (200, 640, 900))]
+    pairs = [(matrix(m, k, "rows", scales, m), matrix(n, k, "tile", scales, n)) for m, n, k in ((2100, 2056, 1100), (2100, 1003, 700), (200, 640, 900), (640, 640, 4000))]
     pairs = [(amd.BlockScaled(a.values, (a.scales.float() / 2.0 ** 17).to(a.scales.dtype)), b) for a, b in pairs]
 
     def call():
