@@ -38,7 +38,9 @@ __device__ __forceinline__ Vec8<DT> load_row8(const CastParams &p, int64_t row, 
         const u32x4 *at = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.a) + i * (DT == MECHA_F32 ? 4 : 2));
 #pragma unroll
         for (int h = 0; h < WORDS<DT> / 4; h++) {
-            const u32x4 r = __builtin_nontemporal_load(at + h);
+            // read once, past the caches; but float32's two halves of a line come with two instructions, the second out of the cache (10240 x 1280 both
+            // ways 22.2 us past it, 20.6 through it; 8269 x 5120 bfloat16 37.9 us past it, 40.4 through it)
+            const u32x4 r = DT == MECHA_F32 ? at[h] : __builtin_nontemporal_load(at + h);
             v.w[4 * h] = r.x; v.w[4 * h + 1] = r.y; v.w[4 * h + 2] = r.z; v.w[4 * h + 3] = r.w;
         }
     } else if constexpr (DT == MECHA_F32) {
@@ -126,8 +128,17 @@ __device__ __forceinline__ u32x2 with_nan(u32x2 codes, uint32_t bits) {
     return codes;
 }
 
+// Codes of float32 keys leave past the caches (10240 x 1280 both ways 20.6 -> 18.7 us, 8269 x 2560 rows 20.3 -> 19.6); of 16-bit keys, whose
+// loads go past them already, that costs 36.0 -> 37.4 us at 8269 x 5120 both ways.
+template <int DT>
+__device__ __forceinline__ void store_codes(uint8_t *at, u32x2 codes) {
+    if constexpr (DT == MECHA_F32) __builtin_nontemporal_store(codes, reinterpret_cast<u32x2 *>(at));
+    else *reinterpret_cast<u32x2 *>(at) = codes;
+}
+
 // Rows form, codes of the matrix as it lies: 16 lanes own a block of 128, 8 elements each; one pass over memory, the block's
-// maximum goes round the 16 lanes.  Dividing by a power of two is exact, the only rounding is the code's.
+// maximum goes round the 16 lanes.  Dividing by a power of two is exact, the only rounding is the code's.  Bound by memory: 8269 x 5120
+// bfloat16 25 us (5.1 TB/s), 77 x 768 2.6 us, which is a launch and one trip to memory.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, int64_t n_groups, int64_t blocks_per_row) {
     const int64_t group = (int64_t)blockIdx.x * (MECHA_BLOCK / 16) + (threadIdx.x >> 4);
@@ -145,7 +156,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
     const int e = exponent_of_mag<DT>(max_mag16<DT>(m));
     u32x2 codes = codes8<DT>(v, scale_bits(e + 127));
     if (nan) codes = with_nan(codes, nan);
-    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = codes;
+    store_codes<DT>(p.q + row * p.q_pitch + c, codes);
     if (l == 0) p.s[row * p.s_pitch + kb] = (uint8_t)(e + 127);
     if (nan && p.flags) atomicOr(p.flags, MECHA_FLAG_INPUT_NONFINITE);
 }
@@ -153,7 +164,9 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
 // 128 x 128 squares: tile scales and / or codes of the transposed matrix.  Thread (t / 16, t % 16) holds rows 8 (t / 16) .. + 7 and
 // columns 8 (t % 16) .. + 7 in registers, so that a row's maximum stays within 16 lanes, a column's takes one exchange between the
 // waves, and an 8 x 8 square of codes turns over in registers; transposed codes go through 16 KiB of LDS to leave as whole
-// 128-byte lines.
+// 128-byte lines.  Bound by memory, one pass over the key for both matrices: 10240 x 1280 float32 both ways 19 us (4.2 TB/s, 14 us with the key in
+// the last-level cache; a grid of all
+// the squares at once, which first all read and then all write), 8269 x 5120 bfloat16 both ways with scales of their own 36 us (4.7 TB/s).
 template <int DT, bool VEC, bool TILE>
 __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
     constexpr int W = WORDS<DT>;
@@ -239,7 +252,7 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_squ
                 u32x2 codes = codes8<DT>(v[i + h], scale_bits(e[h] + 127));
                 if (bad) codes = with_nan(codes, nan[(i + h) >> 2] >> (8 * ((i + h) & 3)));
                 if (row < p.rows) {
-                    *reinterpret_cast<u32x2 *>(p.q + row * p.q_pitch + c) = codes;
+                    store_codes<DT>(p.q + row * p.q_pitch + c, codes);
                     if (!TILE && tc == 0) p.s[row * p.s_pitch + sc] = (uint8_t)(e[h] + 127);
                 }
             }
@@ -299,12 +312,13 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_squ
             const int col = 16 * i + tr;
             const u32x2 w = turned[col][tc ^ (col >> 3)];
             const int64_t oc = sc * SCALE_BLOCK + col;
-            if (oc < p.cols) *reinterpret_cast<u32x2 *>(p.qt + oc * p.qt_pitch + sr * SCALE_BLOCK + 8 * tc) = w;
+            if (oc < p.cols) store_codes<DT>(p.qt + oc * p.qt_pitch + sr * SCALE_BLOCK + 8 * tc, w);
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------ uncast
+// 8 codes a thread, one scale for them.  Bound by memory: 5120 x 2816 to bfloat16 9.8 us (4.4 TB/s).
 template <int OUT_DT, bool E8M0, bool VEC>
 __global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, int64_t q_pitch, const void *s, int64_t s_pitch, int tile,
                                                              int64_t rows, int64_t cols, int64_t vec_per_row, void *out, uint32_t *flags) {
