@@ -481,7 +481,7 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
                         float alpha, uint32_t *flags, void *workspace, size_t workspace_bytes, void *stream);
 /* What a product of m x n results over k can use (0 for most): float32 sums of parts of k, for results too few to fill the chip.  With
  * less, or NULL, k is not shared out. */
-size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int out_dtype);
+size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype);
 
 /* ------------------------------------------------------------------ training step
  * One AdamW step (decoupled weight decay) for every key of the arenas, in place, in one launch:

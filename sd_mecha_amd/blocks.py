@@ -168,8 +168,8 @@ def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check
 
 
 @lru_cache(maxsize=4096)
-def _product_workspace(m: int, n: int, k: int, scale_code: int, out_code: int) -> int:
-    return _lib.lib().mecha_block_product_workspace_bytes(m, n, k, scale_code, out_code)
+def _product_workspace(m: int, n: int, k: int, scale_code: int, b_tile: bool, out_code: int) -> int:
+    return _lib.lib().mecha_block_product_workspace_bytes(m, n, k, scale_code, b_tile, out_code)
 
 
 def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] = None, alpha: float = 1.0, *, out: Optional[torch.Tensor] = None,
@@ -218,7 +218,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         a, b = (q if q.scale_code == SCALE_F32 else BlockScaled(q.values, q.scales.to(torch.float32)) for q in (a, b))
     with _on(device):
         word, fl = _flags(device, flags, check_finite)
-        size = _product_workspace(m, n, k, a.scale_code, _DT[out.dtype])
+        size = _product_workspace(m, n, k, a.scale_code, b.tile, _DT[out.dtype])
         room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _lib.check(_lib.lib().mecha_block_product(
             a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),

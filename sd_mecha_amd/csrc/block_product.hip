@@ -1088,7 +1088,9 @@ int launch_big(const ProductParams &p, void *workspace, hipStream_t s) {
 template <int MODE, bool B_UNIFORM>
 int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
     if constexpr (MODE == HW_SCALES || MODE == F32_SCALES) {
-        if (mi == 8) return launch_big<MODE, B_UNIFORM, 8>(p, workspace, s);
+        if constexpr (MODE == HW_SCALES || B_UNIFORM) {
+            if (mi == 8) return launch_big<MODE, B_UNIFORM, 8>(p, workspace, s);
+        }
         if (mi == 6) return launch_big<MODE, B_UNIFORM, 6>(p, workspace, s);
     }
     return launch_big<MODE, B_UNIFORM, 4>(p, workspace, s);
@@ -1106,16 +1108,18 @@ int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
 //           1024 x 1280 x 5120 25 (36), 300 x 2560 x 8192 24 (53); 320 x 320 x 8269 stays with the direct kernel: 15 us, 16 in 13 parts.
 constexpr int MAX_SPLITS = 32;
 struct Choice { int direct = -1, mi = 0, splits = 1; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
-Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok, bool split_ok) {
-    static const double step[3][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.57, 1.60, 0.0, 0.0}};    // 128 x 128, MI = 4, 6, 8
-    const double *us = step[mode == HW_SCALES ? 0 : mode == F32_SCALES ? 1 : 2];
+Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_ok, bool split_ok) {
+    // a step of 128 x 128, MI = 4, 6, 8: power-of-two scales; float32 scales with one of b's in a square; with one in every row of b, where MI = 8
+    // has no registers for them (8192 x 8192 x 2048: 267 us, 186 with MI = 6); float32 results
+    static const double step[4][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.33, 1.51, 1.78, 0.0}, {1.57, 1.60, 0.0, 0.0}};
+    const double *us = step[mode == HW_SCALES ? 0 : mode != F32_SCALES ? 3 : b_tile ? 1 : 2];
     const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
     auto up = [](int64_t a, int64_t b) { return (double)((a + b - 1) / b); };
     const double mid_tiles = up(m, 128) * up(n, 128) / BIG_CUS;
     double best = 1.5 + (mid_tiles > 1.0 ? mid_tiles : 1.0) * (n_kb * us[0] + 1.0);
     Choice c;
     if (large_ok) {
-        for (int mi = 4; mi <= (us[2] > 0.0 ? 8 : 4); mi += 2) {
+        for (int mi = 4; mi <= 8 && us[mi / 2 - 1] > 0.0; mi += 2) {
             const double rounds = up((int64_t)(up(m, 32 * mi) * up(n, BIG_N)), BIG_CUS), t = 1.5 + rounds * (n_kb * us[mi / 2 - 1] + 0.25 * mi);
             if (t < best) { best = t; c.mi = mi; }
         }
@@ -1138,10 +1142,10 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, bool large_ok, bool spl
 
 extern "C" {
 
-size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int out_dtype) {
+size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype) {
     const bool wide = out_dtype == MECHA_F32, e8m0 = scale_dtype == MECHA_SCALE_E8M0;
     if (m < 1 || n < 1 || k <= 3 * SCALE_BLOCK || n % (wide ? 4 : 8) != 0) return 0;
-    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, true, true);
+    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, b_tile, true, true);
     return c.splits > 1 ? (size_t)c.splits * (size_t)m * (size_t)n * sizeof(float) : 0;
 }
 
@@ -1176,8 +1180,8 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     const bool wide = out_dtype == MECHA_F32;
     const bool large_ok = k > 3 * SCALE_BLOCK && n % (wide ? 4 : 8) == 0 && mecha_aligned16(out) && (base == nullptr || (base_dtype == out_dtype && mecha_aligned16(base)));
     const int mode = wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES;
-    Choice c = choose(m, n, k, mode, large_ok, workspace != nullptr);
-    if (c.splits > 1 && ((size_t)c.splits * (size_t)m * (size_t)n * sizeof(float) > workspace_bytes || !mecha_aligned16(workspace))) c = choose(m, n, k, mode, large_ok, false);
+    Choice c = choose(m, n, k, mode, b_tile, large_ok, workspace != nullptr);
+    if (c.splits > 1 && ((size_t)c.splits * (size_t)m * (size_t)n * sizeof(float) > workspace_bytes || !mecha_aligned16(workspace))) c = choose(m, n, k, mode, b_tile, large_ok, false);
     p.splits = c.splits;
     if (c.direct >= 0) {
         if (wide) return e8m0 ? launch_direct<EXACT_E8M0>(c.direct, p, s) : launch_direct<EXACT_F32>(c.direct, p, s);

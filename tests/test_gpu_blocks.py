@@ -283,7 +283,7 @@ PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4
 @pytest.mark.parametrize("m, n, k", PARTS)
 def test_product_in_parts(m, n, k, scales, dtype):
     import sd_mecha_amd as amd
-    assert amd.blocks._product_workspace(m, n, k, int(scales == "e8m0"), 0 if dtype == torch.float32 else 1) >= 2 * 4 * m * n
+    assert amd.blocks._product_workspace(m, n, k, int(scales == "e8m0"), True, 0 if dtype == torch.float32 else 1) >= 2 * 4 * m * n
     for fb in ("tile", "rows"):
         a, b = matrix(m, k, "rows", scales, m + 3), matrix(n, k, fb, scales, n + 4)
         a = amd.BlockScaled(a.values, (a.scales.float() / 2.0 ** 17).to(a.scales.dtype))
@@ -312,7 +312,7 @@ def test_product_with_too_little_room_for_parts(scales):
     L, (m, n, k) = amd._lib.lib(), PARTS[1]
     a, b = matrix(m, k, "rows", scales, 1, ints=True), matrix(n, k, "tile", scales, 2, ints=True)
     want = torch.from_numpy(R.values(a) @ R.values(b).T).float().cuda()
-    size = L.mecha_block_product_workspace_bytes(m, n, k, a.scale_code, 0)
+    size = L.mecha_block_product_workspace_bytes(m, n, k, a.scale_code, 1, 0)
     room = torch.empty(size, dtype=torch.uint8, device="cuda")
     for at, given in ((None, 0), (room.data_ptr(), size - 1), (room.data_ptr(), size), (room.data_ptr() + 4, size - 4)):
         out = torch.empty(m, n, device="cuda")
