@@ -4,7 +4,9 @@
 //   p = p (1 - lr wd[key]) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // in float32, whatever the storage types.
 //
-// HBM-bound: 28 bytes an element with float32 throughout, 10 with 16-bit weights and gradients and 8-bit states.  One vector a
+// HBM-bound: 28 bytes an element with float32 throughout, 10 with 16-bit weights and gradients and 8-bit states: 174 M float32 elements with
+// bfloat16 gradients and a bfloat16 copy 810 us (6.0 TB/s, what a flat copy reaches is 6.2), 348 M bfloat16 ones with 8-bit states 675 us (5.2
+// TB/s; 59 vector instructions an element take 78 % of that time, the conversions' hashes most of them).  One vector a
 // thread on a flat grid, 4 elements with float32 states and 8 with 8-bit ones; a vector lies in one key (offsets are multiples of
 // 8), its key is found by a search over the segment table that a wave does once, behind the loads.
 //
@@ -286,7 +288,8 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
 
 // ------------------------------------------------------------------------------------------------------- gradient norm
 // Sum of squares over the keys' elements: fixed runs of the arena per block, float64 partials in a fixed order (no atomics, the same
-// sum every time), folded by one block into [norm, min(1, max_norm / (norm + 1e-6))]; NaN where an element is inf or NaN.
+// sum every time), folded by one block into [norm, min(1, max_norm / (norm + 1e-6))]; NaN where an element is inf or NaN.  One read of the
+// gradients: 174 M bfloat16 ones 65 us (5.4 TB/s) and 4.5 for the fold.
 constexpr int NORM_GRID = 2048;
 
 template <int G_DT, bool VEC>

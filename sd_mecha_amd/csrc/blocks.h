@@ -5,6 +5,28 @@
 constexpr int SCALE_BLOCK = MECHA_SCALE_BLOCK;      // 128
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// Rows need not be whole 16 bytes long: gfx950 loads and stores vectors at any element's address.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(2)));
+// the first `bytes` of 16 (a multiple of 2, from 2 to 14), for a row's last elements
+__device__ __forceinline__ void store_part(void *to, u32x4 v, int bytes) {
+    char *at = static_cast<char *>(to);
+    u32x2 w = {v.x, v.y};
+    if (bytes & 8) { *reinterpret_cast<u32x2_any *>(at) = w; at += 8; w = u32x2{v.z, v.w}; }
+    uint32_t x = w.x;
+    if (bytes & 4) { *reinterpret_cast<u32_any *>(at) = x; at += 4; x = w.y; }
+    if (bytes & 2) *reinterpret_cast<uint16_t *>(at) = (uint16_t)x;
+}
+__device__ __forceinline__ u32x4 load_part(const void *from, int bytes) {     // zeros behind them
+    const char *at = static_cast<const char *>(from);
+    u32x2 a = {0, 0}, w = {0, 0};
+    if (bytes & 8) { a = *reinterpret_cast<const u32x2_any *>(at); at += 8; }
+    if (bytes & 4) { w.x = *reinterpret_cast<const u32_any *>(at); at += 4; }
+    if (bytes & 2) { const uint32_t x = *reinterpret_cast<const uint16_t *>(at); if (bytes & 4) w.y = x; else w.x = x; }
+    return bytes & 8 ? u32x4{a.x, a.y, w.x, w.y} : u32x4{w.x, w.y, 0u, 0u};
+}
+
 // The smallest e >= -127 with amax <= 448 * 2^e, from the bits of amax (finite, >= 0): 448 = 1.75 * 2^8, so e is amax's exponent
 // less 8, one more where its mantissa is over 1.75.  Zero and subnormal amax end at the clamp.
 __device__ __forceinline__ int block_exponent(float amax) {

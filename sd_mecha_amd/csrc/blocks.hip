@@ -30,12 +30,12 @@ template <int DT> constexpr uint32_t MAG = DT == MECHA_F32 ? 0x7fffffffu : 0x7ff
 template <int DT> constexpr uint32_t INF = DT == MECHA_F32 ? 0x7f800000u : DT == MECHA_BF16 ? 0x7f80u : 0x7c00u;
 
 // 8 elements of row `row` from column c; zeros behind the last column
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ Vec8<DT> load_row8(const CastParams &p, int64_t row, int64_t c) {
     Vec8<DT> v;
     const int64_t i = row * p.ld + c;
-    if (VEC && c + 8 <= p.cols) {
-        const u32x4 *at = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.a) + i * (DT == MECHA_F32 ? 4 : 2));
+    if (c + 8 <= p.cols) {
+        const u32x4_any *at = reinterpret_cast<const u32x4_any *>(static_cast<const char *>(p.a) + i * (DT == MECHA_F32 ? 4 : 2));
 #pragma unroll
         for (int h = 0; h < WORDS<DT> / 4; h++) {
             // read once, past the caches; but float32's two halves of a line come with two instructions, the second out of the cache (10240 x 1280 both
@@ -139,7 +139,7 @@ __device__ __forceinline__ void store_codes(uint8_t *at, u32x2 codes) {
 // Rows form, codes of the matrix as it lies: 16 lanes own a block of 128, 8 elements each; one pass over memory, the block's
 // maximum goes round the 16 lanes.  Dividing by a power of two is exact, the only rounding is the code's.  Bound by memory: 8269 x 5120
 // bfloat16 25 us (5.1 TB/s), 77 x 768 2.6 us, which is a launch and one trip to memory.
-template <int DT, bool VEC>
+template <int DT>
 __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, int64_t n_groups, int64_t blocks_per_row) {
     const int64_t group = (int64_t)blockIdx.x * (MECHA_BLOCK / 16) + (threadIdx.x >> 4);
     if (group >= n_groups) return;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
     const int64_t kb = group - row * blocks_per_row;
     const int l = threadIdx.x & 15;
     const int64_t c = kb * SCALE_BLOCK + 8 * l;
-    Vec8<DT> v = load_row8<DT, VEC>(p, row, c);
+    Vec8<DT> v = load_row8<DT>(p, row, c);
     uint32_t m = one_mag<DT>(mag8<DT>(v)), nan = 0;
     if (m >= INF<DT>) {
         nan = take_out<DT>(v);
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void cast_rows_kernel(CastParams p, in
 // 128-byte lines.  Bound by memory, one pass over the key for both matrices: 10240 x 1280 float32 both ways 19 us (4.2 TB/s, 14 us with the key in
 // the last-level cache; a grid of all
 // the squares at once, which first all read and then all write), 8269 x 5120 bfloat16 both ways with scales of their own 36 us (4.7 TB/s).
-template <int DT, bool VEC, bool TILE>
+template <int DT, bool TILE>
 __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_square_kernel(CastParams p, int64_t squares_per_row) {
     constexpr int W = WORDS<DT>;
     __shared__ uint32_t wave_max[4][16][W];
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(MECHA_BLOCK, DT == MECHA_F32 ? 3 : 5) void cast_squ
     Vec8<DT> v[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        if (row0 + i < p.rows) v[i] = load_row8<DT, VEC>(p, row0 + i, c);
+        if (row0 + i < p.rows) v[i] = load_row8<DT>(p, row0 + i, c);
         else {
 #pragma unroll
             for (int j = 0; j < W; j++) v[i].w[j] = 0u;
@@ -339,10 +339,24 @@ __global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, i
     for (int j = 0; j < 8; j++) {
         bad_in |= c + j < cols && nonfinite_f32(v[j]);
         v[j] *= scale;
+        if constexpr (OUT_DT == MECHA_F16) asm volatile("" : "+v"(v[j]));    // (or the product and its conversion become one instruction with one rounding)
         bad_out |= c + j < cols && nonfinite_f32(v[j]);
     }
-    if (VEC && c + 8 <= cols) store8<OUT_DT, true>(out, row * cols + c, v);
-    else {
+    if (VEC) store8<OUT_DT, true>(out, row * cols + c, v);
+    else if (c + 8 <= cols) {
+        if constexpr (OUT_DT == MECHA_F32) {
+            u32x4_any *at = reinterpret_cast<u32x4_any *>(static_cast<float *>(out) + row * cols + c);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                at[h] = u32x4{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])};
+        } else {
+            u32x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[j] = OUT_DT == MECHA_BF16 ? f32_to_bf16_bits(v[2 * j]) | f32_to_bf16_bits(v[2 * j + 1]) << 16 : f32_to_f16_bits(v[2 * j]) | f32_to_f16_bits(v[2 * j + 1]) << 16;
+            *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(out) + row * cols + c) = x;
+        }
+    } else {
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (c + j < cols) store1<OUT_DT>(out, row * cols + c + j, v[j]);
@@ -374,25 +388,22 @@ int mecha_cast_blocks(const void *a, int64_t row_stride, int in_dtype, const mec
     CastParams p{a, rows, cols, row_stride, nullptr, 0, nullptr, 0, nullptr, 0, nullptr, 0, flags};
     if (straight) { p.q = static_cast<uint8_t *>(straight->codes); p.q_pitch = straight->pitch; p.s = static_cast<uint8_t *>(straight->scales); p.s_pitch = straight->scale_pitch; }
     if (transposed) { p.qt = static_cast<uint8_t *>(transposed->codes); p.qt_pitch = transposed->pitch; p.st = static_cast<uint8_t *>(transposed->scales); p.st_pitch = transposed->scale_pitch; }
-    const bool vec = mecha_aligned16(a) && (row_stride * (int64_t)mecha_dtype_size(in_dtype)) % 16 == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t bc = (cols + SCALE_BLOCK - 1) / SCALE_BLOCK, br = (rows + SCALE_BLOCK - 1) / SCALE_BLOCK;
     const bool flat = transposed == nullptr && !tile;
     const int64_t blocks = flat ? (rows * bc + MECHA_BLOCK / 16 - 1) / (MECHA_BLOCK / 16) : br * bc;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
     dim3 grid((unsigned)blocks), block(MECHA_BLOCK);
-    auto go = [&](auto dt, auto v) {
+    auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        constexpr bool V = decltype(v)::value;
-        if (flat) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_rows_kernel<DT, V>), grid, block, 0, s, p, rows * bc, bc);
-        else if (tile) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, V, true>), grid, block, 0, s, p, bc);
-        else MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, V, false>), grid, block, 0, s, p, bc);
+        if (flat) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_rows_kernel<DT>), grid, block, 0, s, p, rows * bc, bc);
+        else if (tile) MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, true>), grid, block, 0, s, p, bc);
+        else MECHA_LAUNCH(MK_BLOCKS_CAST, (cast_square_kernel<DT, false>), grid, block, 0, s, p, bc);
     };
-    auto with_vec = [&](auto dt) { if (vec) go(dt, std::true_type{}); else go(dt, std::false_type{}); };
     switch (in_dtype) {
-        case MECHA_F32: with_vec(std::integral_constant<int, MECHA_F32>{}); break;
-        case MECHA_F16: with_vec(std::integral_constant<int, MECHA_F16>{}); break;
-        default: with_vec(std::integral_constant<int, MECHA_BF16>{}); break;
+        case MECHA_F32: go(std::integral_constant<int, MECHA_F32>{}); break;
+        case MECHA_F16: go(std::integral_constant<int, MECHA_F16>{}); break;
+        default: go(std::integral_constant<int, MECHA_BF16>{}); break;
     }
     MECHA_CHECK_HIP(hipGetLastError());
     return MECHA_OK;
@@ -407,7 +418,7 @@ int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, u
     MECHA_REQUIRE(out != nullptr, "out is NULL");
     const int64_t vec_per_row = (cols + 7) / 8, blocks = (rows * vec_per_row + MECHA_BLOCK - 1) / MECHA_BLOCK;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
-    const bool vec = mecha_aligned16(out) && (cols * (int64_t)mecha_dtype_size(out_dtype)) % 16 == 0;
+    const bool vec = mecha_aligned16(out) && cols % 8 == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto dt, auto e8, auto v) {
         MECHA_LAUNCH(MK_BLOCKS_CAST, (uncast_kernel<decltype(dt)::value, decltype(e8)::value, decltype(v)::value>), dim3((unsigned)blocks), dim3(MECHA_BLOCK), 0, s,

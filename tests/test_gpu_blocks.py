@@ -254,8 +254,8 @@ def test_product_large_float32(m, n, k, scales):
     check_product(amd.block_product(a, b), a, b)
 
 
-# results of many tiles that are not whole 16-byte pieces, have a base of another type, or few k
-MIDDLE = [(2100, 1003, 700), (1500, 1501, 1700), (2100, 1000, 384), (1111, 2040, 200), (9000, 1100, 3), (70000, 200, 1)]
+# results of many tiles whose rows are not whole 16-byte pieces, with a base of another type, or of few k
+MIDDLE = [(2100, 1003, 700), (2100, 1004, 700), (1300, 2570, 1300), (1500, 1501, 1700), (2100, 1000, 384), (1111, 2040, 200), (9000, 1100, 3), (70000, 200, 1)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -275,7 +275,7 @@ def test_product_middle(m, n, k, scales, dtype):
 
 
 # few tiles and many blocks of k, whose parts are multiplied apart and joined
-PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4100), (900, 264, 8192)]
+PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4100), (900, 264, 8192), (700, 643, 8269), (1024, 1282, 5120)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -292,7 +292,7 @@ def test_product_in_parts(m, n, k, scales, dtype):
         out = base.clone()
         assert amd.block_product(a, b, out, -2.0, out=out) is out
         check_product(out, a, b, base, -2.0)
-        room = torch.empty(m * n + 1, dtype=dtype, device="cuda")                   # not in parts: 2 or 4 bytes off
+        room = torch.empty(m * n + 1, dtype=dtype, device="cuda")                   # 2 or 4 bytes off
         check_product(amd.block_product(a, b, base, 0.5, out=room[1:]).view(m, n), a, b, base, 0.5)
     v = a.values.clone()
     v.view(torch.uint8)[m - 1, k - 1] = 0x7F
