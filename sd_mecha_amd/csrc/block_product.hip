@@ -588,6 +588,14 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     const uint32_t run0 = all_tiles * xcd / 8, run1 = all_tiles * (xcd + 1) / 8;
     uint32_t tile = run0 + (blockIdx.x >> 3);
     if (tile >= run1) return;
+    // Tiles of one size end at one time, and all CUs' results together are bound by memory (5.4 us a round of 256 x 256 16-bit ones) while the matrix
+    // units wait.  Where workgroups have several tiles, half of an XCD's -- those that have the fewer, if any do -- begin about half a round's stores
+    // later (64 cycles a unit), and one half stores while the other multiplies: 8192 x 10240 x 1280 110 -> 105 us, 16384 x 5120 x 640 68 -> 61,
+    // 4096 x 8192 x 512 31 -> 26.  More groups (4, 8, 32) gain less.
+    if (run1 - run0 > per_xcd && (blockIdx.x >> 3) >= per_xcd / 2) {
+        constexpr int UNITS = ROWS * (OUT == MECHA_F32 ? 4 : 2) / 4;
+        for (int i = 0; i < UNITS; i += 16) __builtin_amdgcn_s_sleep(16);
+    }
     // bands of BIG_BAND rows of tiles, down the band first; blocks k0 .. k0 + count - 1 of k
     struct Place { uint32_t m0, n0, part; int k0, count; };
     auto one = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };      // the same in every lane
