@@ -743,6 +743,26 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         };
         bool nan = false;
         float poison_in = 0.0f, poison_out = 0.0f;
+        // base comes AHEAD fragments before it is added (8192 x 10240 x 1280 with a base 139 -> 134 us; float32 results have no registers for it)
+        constexpr int PAIRS = EXACT ? 2 : 1, AHEAD = EXACT ? 1 : 2;
+        u32x4 pre[AHEAD][PAIRS][2];
+        auto ask = [&](int i, int64_t from) {
+            if constexpr (BASE) {
+#pragma unroll
+                for (int pair = 0; pair < PAIRS; pair++) {
+                    const int64_t at = from + (EXACT ? 32 * ESIZE * pair : 0);
+                    const int left = cols - (EXACT ? 32 * pair : 0);
+                    u32x4 *c = pre[i % AHEAD][pair];
+                    c[0] = c[1] = u32x4{0, 0, 0, 0};
+                    if (left > 0 && 16 * i < rows) c[0] = get(at, left);
+                    if (left > 0 && 16 * i + 1 < rows) c[1] = get(at + line, left);
+                }
+            }
+        };
+        int64_t ask_at = at0;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) { ask(i, ask_at); ask_at += 16 * line; asm volatile("" : "+v"(ask_at)); }
+        if constexpr (BASE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MI; i++) {
 #pragma unroll
@@ -750,11 +770,10 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                 // this lane's pieces in memory: number 0 (even lane) or 1 (odd) of the pair
                 const int64_t at = at0 + (EXACT ? 32 * ESIZE * pair : 0);
                 const int left = cols - (EXACT ? 32 * pair : 0);
-                    const bool in = left > 0, above = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
+                const bool in = left > 0, above = in && 16 * i < rows, below = in && 16 * i + 1 < rows;
                 u32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
                 if constexpr (BASE) {
-                    if (above) c[0] = get(at, left);
-                    if (below) c[1] = get(at + line, left);
+                    c[0] = pre[i % AHEAD][pair][0]; c[1] = pre[i % AHEAD][pair][1];
                     exchange(c[0], c[1], odd);
                 }
 #pragma unroll
@@ -788,6 +807,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                 if (above) put(at, left, c[0]);
                 if (below) put(at + line, left, c[1]);
             }
+            if (BASE && i + AHEAD < MI) { ask(i + AHEAD, ask_at); ask_at += 16 * line; }
             at0 += 16 * line;
             asm volatile("" : "+v"(at0));                                 // (addresses one after the other, not all at once)
             if (i % 2) __builtin_amdgcn_sched_barrier(0);
