@@ -541,7 +541,7 @@ int launch_direct(int shape, const ProductParams &p, hipStream_t s) {
 // tiles (2 MiB of a and 1 MiB of b at k = 1024, MI = 8).
 //
 // Measured (no base): 8192 x 8192 x 8192 457 us (2.4 PFLOP/s; the matrix unit's own rate is 4.3, and a plain per-tensor library product takes 421);
-// 8192 x 10240 x 1280 105 us (2.0 PFLOP/s, 168 MB of results at 1.6 TB/s; the library 108); 8269 x 1280 x 5120 58 us (float32 scales: 64).  A
+// 8192 x 10240 x 1280 100 us (2.15 PFLOP/s with 168 MB of results; the library 108); 8269 x 1280 x 5120 58 us (float32 scales: 64).  A
 // 256 x 256 step takes 3900 cycles: 2048 of products at the unit's rate, and 1600 in which its 64 KiB come from L2 to LDS, which overlap
 // only in part: fewer or more of them asked for at a step's start, by four waves or by eight, made no difference.  Float32 results
 // multiply at bfloat16's rate (2.1 PFLOP/s): 1280 x 5120 x 8269 102 us (1.06 PFLOP/s on 200 of the 256 CUs).
