@@ -1205,9 +1205,10 @@ int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------------- which kernel
-// The time each would take, in microseconds, from what it measured on 256 CUs (times fit within 20 % from 1 x 1280 x 1280 to
-// 16384 x 5120 x 640, all three kinds of sums):
-//   direct: a launch, plus the slower of one workgroup's reads (33 KB a us) and all reads together (5 TB/s);
+// The time each would take, in microseconds, from what it measured on 256 CUs (138 random products up to 16384 x 10240 x 8192 of all four kinds, each
+// with every kernel: the choice is 2 to 3 % over the best in the mean):
+//   direct: a launch, the join of a workgroup's waves, and the slower of one workgroup's reads (33 KB a us) and all workgroups' (5 TB/s, 1 ns and their
+//           joins): 53 x 4077 x 659 4.9 us with 32 x 32 outputs a workgroup, 6.0 with 32 x 64;
 //   tiled:  rounds of tiles over the CUs, each n_kb steps and an epilogue.  128 x 128 tiles (two workgroups a CU) fill a few CUs more evenly:
 //           1024 x 1280 x 5120 36 us, 49 with 128 x 256 tiles; the larger ones share more: 8192 x 1280 x 5120 57 us (192 x 256), 80 with
 //           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 82 (128 x 256).
@@ -1219,16 +1220,16 @@ struct Choice { int direct = -1, mi = 0, splits = 1; };        // shape of the d
 Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_ok, bool split_ok) {
     // a step of 128 x 128, MI = 4, 6, 8: power-of-two scales; float32 scales with one of b's in a square; with one in every row of b, where MI = 8
     // has no registers for them (8192 x 8192 x 2048: 267 us, 186 with MI = 6); float32 results
-    static const double step[4][4] = {{0.90, 1.20, 1.36, 1.56}, {1.33, 1.34, 1.54, 1.81}, {1.33, 1.51, 1.78, 0.0}, {1.57, 1.60, 0.0, 0.0}};
+    static const double step[4][4] = {{0.75, 1.20, 1.36, 1.56}, {1.18, 1.34, 1.54, 1.81}, {1.18, 1.51, 1.78, 0.0}, {1.42, 1.60, 0.0, 0.0}};
     const double *us = step[mode == HW_SCALES ? 0 : mode != F32_SCALES ? 3 : b_tile ? 1 : 2];
     const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
     auto up = [](int64_t a, int64_t b) { return (double)((a + b - 1) / b); };
     const double mid_tiles = up(m, 128) * up(n, 128) / BIG_CUS;
-    double best = 1.5 + (mid_tiles > 1.0 ? mid_tiles : 1.0) * (n_kb * us[0] + 1.0);
+    double best = 6.0 + (mid_tiles > 1.0 ? mid_tiles : 1.0) * (n_kb * us[0] + 1.0);
     Choice c;
     if (large_ok) {
         for (int mi = 4; mi <= 8 && us[mi / 2 - 1] > 0.0; mi += 2) {
-            const double rounds = up((int64_t)(up(m, 32 * mi) * up(n, BIG_N)), BIG_CUS), t = 1.5 + rounds * (n_kb * us[mi / 2 - 1] + 0.25 * mi);
+            const double rounds = up((int64_t)(up(m, 32 * mi) * up(n, BIG_N)), BIG_CUS), t = 3.5 + rounds * (n_kb * us[mi / 2 - 1] + 0.25 * mi);
             if (t < best) { best = t; c.mi = mi; }
         }
         const double tiles = up(m, 128) * up(n, BIG_N), part = (double)m * (double)n * 8.0 / 5e6;
@@ -1239,8 +1240,8 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_
     }
     static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
     for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 32 us, 16 without it)
-        const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * bytes / 5e6;
-        const double t = 2.5 + (one > all ? one : all);
+        const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * (bytes / 5e6 + 0.001 + 2e-6 * rows[d] * cols[d]);
+        const double t = 2.5 + 0.001 * rows[d] * cols[d] + (one > all ? one : all);
         if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.splits = 1; c.direct = d; }     // a launch's threads
     }
     return c;
