@@ -255,7 +255,7 @@ def test_product_large_float32(m, n, k, scales):
 
 
 # results of many tiles whose rows are not whole 16-byte pieces, with a base of another type, or of few k
-MIDDLE = [(2100, 1003, 700), (2100, 1004, 700), (1300, 2570, 1300), (1500, 1501, 1700), (2100, 1000, 384), (1111, 2040, 200), (9000, 1100, 3), (70000, 200, 1)]
+MIDDLE = [(2100, 1003, 700), (2100, 1004, 700), (1300, 2570, 1300), (1500, 1501, 1700), (2100, 1000, 384), (1111, 2040, 200), (9000, 1100, 3), (70000, 200, 1), (5000, 3, 4100), (4000, 1, 8192)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -275,7 +275,7 @@ def test_product_middle(m, n, k, scales, dtype):
 
 
 # few tiles and many blocks of k, whose parts are multiplied apart and joined
-PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4100), (900, 264, 8192), (700, 643, 8269), (1024, 1282, 5120)]
+PARTS = [(640, 640, 8269), (1024, 1280, 5120), (300, 2560, 8192), (1281, 1288, 4100), (900, 264, 8192), (700, 643, 8269), (1024, 1282, 5120), (5100, 77, 6298)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
