@@ -15,7 +15,9 @@
 // smallest code, which squared would be only 2^9 of gradient magnitudes.  A code's distance is up to 1/8 of its value and a moving mean
 // changes by (1 - b2) of itself a step, so rounding to nearest would never move it: |x| is rounded up with probability equal
 // to its part of the distance, by 16 bits of a hash of (offset, step, seed).  A root that is not zero never becomes zero: the
-// next step would divide by eps alone.
+// next step would divide by eps alone.  A gradient over 1.8e19 has a square over float32's largest number: its element takes no part in its
+// block's scales and keeps the NaN code for its root, which the next step reads as an infinite one: that weight only decays from then on, as
+// with float32 states, and the other 127 of its block move as they would without it.
 #include <math.h>
 #include <type_traits>
 #include "blocks.h"
@@ -117,6 +119,9 @@ __device__ __forceinline__ float root_of(float v) {
     return small ? r * 2.3283064365386963e-10f : r;
 }
 
+// bit 7 of every byte whose code is NaN
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // 32 bits for an element: multiplications by odd constants (the first 32 fractional bits of the golden ratio and of the square roots
 // of 2, 3 and 5) and right shifts, modulo 2^32
 __device__ __forceinline__ uint32_t dither32(int64_t i, uint32_t key) {
@@ -216,6 +221,11 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
             m[j] = x.x; m[j + 1] = x.y;
             v[j] = y.x * y.x; v[j + 1] = y.y * y.y;
         }
+        if (nan_codes(vc.x) | nan_codes(vc.y)) {              // a root over the largest number (rare)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if ((nan_codes(vc[j / 4]) >> (8 * (j & 3))) & 0x80u) v[j] = INFINITY;
+        }
         if (valid < 8) {                                      // what lies between the keys takes no part in a scale, and its codes become 0
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -230,7 +240,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         root[j] = root_of(v[j]);
         const float den = __builtin_fmaf(root[j], root_size, a.eps);
         p[j] = __builtin_fmaf(m[j] * __builtin_amdgcn_rcpf(den), -size, p[j] * keep);
-        if (a.seg_flags && j < valid) poison_out = __builtin_fmaf(p[j], 0.0f, poison_out);
+        if (a.seg_flags && j < valid) poison_out = __builtin_fmaf(v[j], 0.0f, __builtin_fmaf(p[j], 0.0f, poison_out));
     }
     if (valid) {
         store(std::integral_constant<int, P_DT>{}, a.p, p);
@@ -244,6 +254,15 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         float mm = 0.0f, vm = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) { mm = fmaxf(mm, fabsf(m[j])); vm = fmaxf(vm, root[j]); }
+        if (!(fmaxf(mm, vm) < INFINITY)) {                    // (NaN takes no part in the maxima)
+            mm = vm = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (!(root[j] < INFINITY)) { m[j] = fabsf(m[j]) < INFINITY ? 0.0f : NAN; root[j] = NAN; }
+                mm = fmaxf(mm, fabsf(m[j]));
+                vm = fmaxf(vm, root[j]);
+            }
+        }
         const int em = block_exponent(max16(mm)), ev = block_exponent(max16(vm));
         const float sm = scale_bits(em + 127), sv = scale_bits(ev + 127);
         int mw[2] = {0, 0}, vw[2] = {0, 0};
