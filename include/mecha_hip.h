@@ -24,7 +24,9 @@
  *    bit 0 (MECHA_FLAG_INPUT_NONFINITE): some input element was inf/NaN -- the
  *    caller turns it into NonFiniteStateDictKeyError = "skip this key"
  *    (logistics.py:132-142).  bit 1 (MECHA_FLAG_OUTPUT_NONFINITE): some output
- *    element is inf/NaN -- warning only (merging.py:297-308).
+ *    element is inf/NaN -- warning only (merging.py:297-308); the merge methods
+ *    look at the fp32 value, the 8-bit weights and the training step at what
+ *    out_dtype stores (fp16: infinity from 65520 on).
  *  - Return value: 0 on success, negative on error; mecha_last_error() returns
  *    the message of the calling thread's last error.
  *  - Workspaces are caller-provided device memory sized by the *_workspace_bytes
@@ -501,7 +503,7 @@ typedef struct mecha_adamw {
     const float *key_weight_decay;    /* float[n_segments], may be NULL: weight_decay for all */
     const int64_t *step_dev;          /* read instead of `step` when the kernel runs (for captured graphs), may be NULL */
     const float *clip;                /* float[2] of mecha_batched_grad_norm, may be NULL; with a NaN coefficient the step changes nothing */
-    uint32_t *seg_flags;              /* uint32[n_segments], may be NULL: bit 0: a gradient or weight was inf / NaN, bit 1: a new weight or second moment is */
+    uint32_t *seg_flags;              /* uint32[n_segments], may be NULL: bit 0: a gradient or weight was inf / NaN, bit 1: a new weight (as stored, in the arena or the copy) or second moment is */
     int64_t total_elems;
     int64_t step;
     double lr, beta1, beta2, eps, weight_decay;

@@ -151,7 +151,8 @@ def cast_blocks(a, *, tile: bool = False, sides: str = "straight", key=None, fla
 
 
 def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check_finite: bool = True) -> torch.Tensor:
-    """``values * scales`` in float32 as a contiguous matrix of ``out_dtype`` (default float32)."""
+    """``values * scales`` in float32 as a contiguous matrix of ``out_dtype`` (default float32).  NaN codes and scales that are not finite raise
+    ``NonFiniteStateDictKeyError`` (``check_finite``) or set bit 0 of ``flags``; a result that its type stores as infinity sets bit 1."""
     _check_blocks(q, "uncast_blocks")
     dtype = out_dtype or torch.float32
     if dtype not in _DT:
@@ -181,7 +182,8 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
 
     A linear layer ``y = x @ w.T`` with w cast with ``tile=True, sides="both"`` to (w, wt), x and the output gradient g cast to (x, xt) and
     (g, gt): y = block_product(x, w), the input's gradient block_product(g, wt), the weight's block_product(gt, xt).
-    A NaN result or a non-finite base raises ``NonFiniteStateDictKeyError`` (``check_finite``) or sets bit 0 of ``flags``."""
+    A NaN result or a non-finite base raises ``NonFiniteStateDictKeyError`` (``check_finite``) or sets bit 0 of ``flags``; a result that its type
+    stores as infinity sets bit 1."""
     _check_blocks(a, "block_product")
     _check_blocks(b, "block_product")
     m, k, n, kb, device = a.rows, a.cols, b.rows, b.cols, a.values.device

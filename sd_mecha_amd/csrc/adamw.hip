@@ -44,6 +44,7 @@ struct AdamParams {
     double b1d, b2d, lrd;
     uint32_t seed;
     uint32_t *seg_flags;
+    float over;                        // a weight of this size is stored as infinity, in the arena or in the copy
 };
 
 // index of the last segment with offset <= elem, or -1: the 64 lanes look at 64 offsets at once (wave-uniform elem)
@@ -193,7 +194,8 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
             }
         }
     }
-    float poison_in = 0.0f, poison_out = 0.0f, root[N];       // fma(x, 0, poison) stays 0 while every x is finite
+    float poison_in = 0.0f, root[N];                          // fma(x, 0, poison) stays 0 while every x is finite
+    bool bad_out = false;
     if (a.seg_flags) {
 #pragma unroll
         for (int j = 0; j < N; j++)
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         root[j] = root_of(v[j]);
         const float den = __builtin_fmaf(root[j], root_size, a.eps);
         p[j] = __builtin_fmaf(m[j] * __builtin_amdgcn_rcpf(den), -size, p[j] * keep);
-        if (a.seg_flags && j < valid) poison_out = __builtin_fmaf(v[j], 0.0f, __builtin_fmaf(p[j], 0.0f, poison_out));
+        if (a.seg_flags && j < valid) bad_out |= !(fabsf(p[j]) < a.over) || !(v[j] < INFINITY);
     }
     if (valid) {
         store(std::integral_constant<int, P_DT>{}, a.p, p);
@@ -301,8 +303,8 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         store(std::integral_constant<int, MECHA_F32>{}, a.m, m);
         store(std::integral_constant<int, MECHA_F32>{}, a.v, v);
     }
-    if (a.seg_flags && valid && (poison_in != 0.0f || poison_out != 0.0f))
-        atomicOr(a.seg_flags + s, (poison_in != 0.0f ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+    if (a.seg_flags && valid && (poison_in != 0.0f || bad_out))
+        atomicOr(a.seg_flags + s, (poison_in != 0.0f ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (bad_out ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
 }
 
 // ------------------------------------------------------------------------------------------------------- gradient norm
@@ -466,6 +468,7 @@ int mecha_batched_adamw(const mecha_adamw *args, void *stream) {
     a.decay = x.key_weight_decay; a.decay_all = (float)x.weight_decay;
     a.lr = (float)x.lr; a.b1 = (float)x.beta1; a.b2 = (float)x.beta2; a.c1 = (float)(1.0 - x.beta1); a.c2 = (float)(1.0 - x.beta2); a.eps = (float)x.eps;
     a.lrd = x.lr; a.b1d = x.beta1; a.b2d = x.beta2; a.seed = x.seed; a.step_dev = x.step_dev; a.clip = x.clip; a.seg_flags = x.seg_flags;
+    a.over = fminf(stored_as_inf(x.param_dtype), x.copy ? stored_as_inf(x.copy_dtype) : INFINITY);
     if (x.step_dev == nullptr) {
         a.size = (float)(x.lr / (1.0 - pow(x.beta1, (double)x.step)));
         a.root_size = (float)(1.0 / sqrt(1.0 - pow(x.beta2, (double)x.step)));

@@ -101,14 +101,20 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// the larger magnitude, NaN if one is (gfx950's v_maximum3_f32), and the flags of results of which `top` is the largest
+__device__ __forceinline__ float larger(float top, float x) { return __builtin_elementwise_maximum(top, fabsf(x)); }
+__device__ __forceinline__ void report(uint32_t *flags, float poison_in, float top, int out_dt) {
+    const bool over = !(top < stored_as_inf(out_dt)), in = top != top || poison_in != 0.0f;
+    if (flags && (in || over)) atomicOr(flags, (in ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (over ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+}
+
 // 8 contiguous columns of one output row, of any base and alignment: base + alpha * acc.  Finite checks: fma(x, 0, poison) stays 0
-// while every x is finite.
+// while every x is finite; results by their largest magnitude or NaN.
 template <int OUT_DT, bool VEC>
 __device__ __forceinline__ void store_any8(const ProductParams &p, int64_t m, int64_t n, const float (&acc)[8]) {
     if (m >= p.m || n >= p.n) return;
     const int64_t i = m * p.n + n;
-    float r[8], b[8], poison_in = 0.0f, poison_out = 0.0f;
-    bool nan = false;
+    float r[8], b[8], poison_in = 0.0f, top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) b[j] = 0.0f;
     const int left = p.n - n < 8 ? (int)(p.n - n) : 8;
@@ -142,8 +148,7 @@ __device__ __forceinline__ void store_any8(const ProductParams &p, int64_t m, in
         r[j] = p.base ? __builtin_fmaf(acc[j], p.alpha, b[j]) : acc[j] * p.alpha;
         if (n + j < p.n) {
             poison_in = __builtin_fmaf(b[j], 0.0f, poison_in);
-            poison_out = __builtin_fmaf(r[j], 0.0f, poison_out);
-            nan |= r[j] != r[j];
+            top = larger(top, r[j]);
         }
     }
     if constexpr (VEC) store8<OUT_DT>(p.out, i, r);
@@ -164,8 +169,7 @@ __device__ __forceinline__ void store_any8(const ProductParams &p, int64_t m, in
         if (left == 8) *reinterpret_cast<u32x4_any *>(at) = w;
         else store_part(at, w, 2 * left);
     }
-    nan |= poison_in != 0.0f;
-    if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+    report(p.flags, poison_in, top, OUT_DT);
 }
 
 // Scales of a tile's 128 rows, CH words each: four blocks a word for the matrix unit, else a float a block.
@@ -481,15 +485,13 @@ __global__ __launch_bounds__(DIRECT_THREADS, 2) void product_direct_kernel(Produ
                     if (n + e < p.n) base[e] = p.base_dt == MECHA_F32 ? load1<MECHA_F32>(p.base, at + e) : p.base_dt == MECHA_F16 ? load1<MECHA_F16>(p.base, at + e) : load1<MECHA_BF16>(p.base, at + e);
             }
         }
-        float poison = 0.0f, poison_in = 0.0f;
-        bool nan = false;
+        float top = 0.0f, poison_in = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             out[e] = p.base ? __builtin_fmaf(sum[e], p.alpha, base[e]) : sum[e] * p.alpha;
             if (n + e < p.n) {
-                poison = __builtin_fmaf(out[e], 0.0f, poison);
+                top = larger(top, out[e]);
                 poison_in = __builtin_fmaf(base[e], 0.0f, poison_in);
-                nan |= out[e] != out[e];
             }
         }
         if (vec && p.out_dt == MECHA_F32)
@@ -506,8 +508,7 @@ __global__ __launch_bounds__(DIRECT_THREADS, 2) void product_direct_kernel(Produ
                     else store1<MECHA_BF16>(p.out, at + e, out[e]);
                 }
         }
-        nan |= poison_in != 0.0f;
-        if (p.flags && (nan || poison != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+        report(p.flags, poison_in, top, p.out_dt);
     }
 }
 
@@ -741,8 +742,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             else if (left >= EACH) *reinterpret_cast<u32x4_any *>(to) = v;
             else store_part(to, v, ESIZE * left);
         };
-        bool nan = false;
-        float poison_in = 0.0f, poison_out = 0.0f;
+        float poison_in = 0.0f, top = 0.0f;
         // base comes AHEAD fragments before it is added (8192 x 10240 x 1280 with a base 139 -> 134 us; float32 results have no registers for it)
         constexpr int PAIRS = EXACT ? 2 : 1, AHEAD = EXACT ? 1 : 2;
         u32x4 pre[AHEAD][PAIRS][2];
@@ -795,7 +795,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
                         const int64_t in_row = p.n - ((int64_t)here.n0 + wn + (EXACT ? 32 * pair + 16 * h + 4 * g : 32 * h + 8 * g));
 #pragma unroll
                         for (int j = 0; j < EACH; j++)
-                            if (j < in_row) { poison_out = __builtin_fmaf(v[j], 0.0f, poison_out); nan |= v[j] != v[j]; }
+                            if (j < in_row) top = larger(top, v[j]);
                     }
                     if constexpr (EXACT) c[h] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
                     else {
@@ -812,8 +812,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             asm volatile("" : "+v"(at0));                                 // (addresses one after the other, not all at once)
             if (i % 2) __builtin_amdgcn_sched_barrier(0);
         }
-        nan |= poison_in != 0.0f;
-        if (p.flags && (nan || poison_out != 0.0f)) atomicOr(p.flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+        report(p.flags, poison_in, top, OUT);
     };
     if constexpr (EXACT) {
         // Float32 results.  A step is four fragments of a, each multiplied a quarter of its k at a time: 4 instructions of 16 cycles.  The matrix unit
@@ -1105,8 +1104,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void join_kernel(const float *parts, i
     }
     constexpr int ESIZE = DT == MECHA_F32 ? 4 : 2;
     const int64_t to = (row * n + col) * ESIZE;
-    float v[4], b[4] = {0, 0, 0, 0}, poison_in = 0.0f, poison_out = 0.0f;
-    bool nan = false;
+    float v[4], b[4] = {0, 0, 0, 0}, poison_in = 0.0f, top = 0.0f;
     if constexpr (BASE) {
         const char *from = static_cast<const char *>(base) + to;
         if constexpr (DT == MECHA_F32) {
@@ -1129,8 +1127,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void join_kernel(const float *parts, i
         v[e] = BASE ? __builtin_fmaf(sum[e], alpha, b[e]) : sum[e] * alpha;
         if (e < left) {
             poison_in = __builtin_fmaf(b[e], 0.0f, poison_in);
-            poison_out = __builtin_fmaf(v[e], 0.0f, poison_out);
-            nan |= v[e] != v[e];
+            top = larger(top, v[e]);
         }
     }
     char *const put = static_cast<char *>(out) + to;
@@ -1143,8 +1140,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void join_kernel(const float *parts, i
         if (left == 4) *reinterpret_cast<u32x2_any *>(put) = w;
         else store_part(put, u32x4{w.x, w.y, 0u, 0u}, 2 * left);
     }
-    nan |= poison_in != 0.0f;
-    if (flags && (nan || poison_out != 0.0f)) atomicOr(flags, (nan ? MECHA_FLAG_INPUT_NONFINITE : 0u) | (poison_out != 0.0f ? MECHA_FLAG_OUTPUT_NONFINITE : 0u));
+    report(flags, poison_in, top, DT);
 }
 constexpr int64_t part_ld(int64_t n) { return (n + 7) / 8 * 8; }
 int launch_join(const ProductParams &p, const void *parts, hipStream_t s) {

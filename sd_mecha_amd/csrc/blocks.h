@@ -54,6 +54,10 @@ __device__ __forceinline__ float max16(float v) {
     return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x121, 0xf, 0xf, true)));
 }
 
+// The smallest magnitude that a type stores as infinity: half a step over its largest number (the tie goes to the even side, infinity).  Output
+// flags are about what is stored: !(|x| < this), which NaN sets as well.
+__host__ __device__ constexpr float stored_as_inf(int dt) { return dt == MECHA_F16 ? 65520.0f : dt == MECHA_BF16 ? 0x1.ffp127f : __builtin_inff(); }
+
 // A barrier for what the waves exchange through LDS: unlike __syncthreads() it does not wait for stores to memory.
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -340,7 +340,7 @@ __global__ __launch_bounds__(MECHA_BLOCK) void uncast_kernel(const uint8_t *q, i
         bad_in |= c + j < cols && nonfinite_f32(v[j]);
         v[j] *= scale;
         if constexpr (OUT_DT == MECHA_F16) asm volatile("" : "+v"(v[j]));    // (or the product and its conversion become one instruction with one rounding)
-        bad_out |= c + j < cols && nonfinite_f32(v[j]);
+        bad_out |= c + j < cols && !(fabsf(v[j]) < stored_as_inf(OUT_DT));
     }
     if (VEC) store8<OUT_DT, true>(out, row * cols + c, v);
     else if (c + 8 <= cols) {

@@ -61,7 +61,7 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
     number, or float32 [keys] on the device, one per key.  ``copy``: an arena that receives the new weights in its own dtype.
     ``max_norm``: the gradients of all keys together are scaled down to this 2-norm first, and the norm is returned ([1], on the device);
     if it is not finite, the step sets flags and changes nothing else.  The arenas share no memory.  ``flags``: int32 [keys], per-key flag words (bit 0: a gradient or weight is
-    inf / NaN, bit 1: a new weight or second moment is: a gradient over 1.8e19 has no square in float32, and its weight only decays from then
+    inf / NaN, bit 1: a new weight, as stored, or second moment is: a gradient over 1.8e19 has no square in float32, and its weight only decays from then
     on)."""
     for t, name in ((params, "params"), (segments, "segments")):
         if not isinstance(t, torch.Tensor):

@@ -8,6 +8,7 @@ import blocks_reference as R
 pytestmark = pytest.mark.gpu
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
+H = float.fromhex
 
 
 def raw(t):
@@ -53,3 +54,78 @@ def test_a_gradient_without_a_square_stays_with_its_element(bits, value):
             assert bool(bad[2][at].float().isnan()) and bool(bad[1][at].float().isnan()) == (not np.isfinite(value))
     # and the others do move: weights in every step, roots over the steps
     assert bool((runs[1][0][0] != p0)[others].all()) and all(bool((runs[1][t][0] != runs[1][t - 1][0])[others].all()) for t in range(1, steps))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [256, 253])                              # whole vectors, and a key's last elements
+def test_weights_that_their_type_stores_as_infinity_set_the_flag(n, bits):
+    """The largest number plus a little less than half a step is stored as the largest number, plus half a step as infinity; in the arena or in the
+    copy.  The gradient is zero and the decay, by 2^-12 of the weight, reaches the border from above."""
+    import sd_mecha_amd as amd
+    total = 256
+    seg = torch.tensor([[0, n]], device="cuda")
+    for p_dt, copy_dt, start, want in ((torch.float32, torch.float16, 65520.0, 0x7C00), (torch.float32, torch.float16, 65519.99, 0x7BFF), (torch.float32, torch.bfloat16, 3.3961775292304957e38, 0x7F80),
+                                       (torch.float32, torch.bfloat16, 3.39617732e38, 0x7F7F), (torch.float32, None, 3.4e38, None), (torch.bfloat16, torch.float16, 65536.0, 0x7C00)):
+        p = torch.zeros(total, dtype=p_dt, device="cuda")
+        p[n - 1] = start
+        copy = torch.zeros(total, dtype=copy_dt, device="cuda") if copy_dt else None
+        flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+        amd.adamw_step(p, torch.zeros(total, device="cuda"), segments=seg, step=1, lr=1e-3, weight_decay=0.0, copy=copy, flags=flags, **amd.adamw_state(total, "cuda", bits))
+        if copy is not None:
+            assert (int(copy.view(torch.int16)[n - 1]) & 0xFFFF) == want, (p_dt, start)
+        assert int(flags) == (2 if want in (0x7C00, 0x7F80) else 0), (p_dt, copy_dt, start)
+    # a float16 arena whose weight a step carries over the border: p - lr * m / (sqrt(v) + eps) = p + lr in the first step
+    for lr, over in ((15.0, False), (17.0, True)):
+        p, grad = torch.zeros(total, dtype=torch.float16, device="cuda"), torch.zeros(total, device="cuda")
+        p[n - 1], grad[n - 1] = 65504.0, -1.0
+        flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+        amd.adamw_step(p, grad, segments=seg, step=1, lr=lr, weight_decay=0.0, flags=flags, **amd.adamw_state(total, "cuda", bits))
+        assert bool(p[n - 1].isinf()) == over and int(flags) == (2 if over else 0), lr
+
+
+# --------------------------------------------------------------------------------------------------------------- uncast
+@pytest.mark.parametrize("cols", [128, 125])
+def test_uncast_values_that_their_type_stores_as_infinity_set_the_flag(cols):
+    import sd_mecha_amd as amd
+    for dtype, code, scale, inf in ((torch.float16, 448.0, 146.25, True), (torch.float16, 448.0, 146.24, False), (torch.bfloat16, 256.0, H("0x1.ffp119"), True),
+                                    (torch.bfloat16, 256.0, H("0x1.fefffep119"), False), (torch.float32, 256.0, H("0x1.ffp119"), False), (torch.float32, 256.0, 2.0 ** 120, True)):
+        v = torch.zeros(3, cols, device="cuda")
+        v[2, cols - 1] = code
+        flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = amd.uncast_blocks(amd.BlockScaled(v.to(E4M3), torch.full((3, 1), scale, device="cuda")), out_dtype=dtype, flags=flags)
+        assert bool(got[2, cols - 1].isinf()) == inf and int(flags) == (2 if inf else 0), (dtype, scale)
+        assert not got[:2].any()
+
+
+# -------------------------------------------------------------------------------------------------------------- product
+# one shape for each way a product takes: memory to registers, 128 x 128 tiles, larger tiles, parts of k that are joined
+WAYS = [(3, 40, 200), (40, 63, 300), (2100, 2056, 300), (2100, 1003, 700), (5000, 4200, 640), (1024, 1280, 5120), (900, 261, 8192)]
+
+
+@pytest.mark.parametrize("based", [False, True])
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_products_that_their_type_stores_as_infinity_set_the_flag(m, n, k, scales, based):
+    """One result, in the last row and column: a product of one pair of codes, 1 x 1 x 2^15 (float16) or 2^127, and alpha up to the border."""
+    import sd_mecha_amd as amd
+    a, b = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    a[m - 1, k - 1], b[n - 1, k - 1] = 1.0, 1.0
+    kb = R.blocks(k)
+    for dtype, e, alphas in ((torch.float16, 15, ((65520 / 32768, True), (65519.99 / 32768, False))), (torch.bfloat16, 120, ((H("0x1.ffp7"), True), (H("0x1.fefffep7"), False))),
+                             (torch.float32, 120, ((H("0x1.ffp7"), False), (H("0x1.fffffep7"), False), (2.0 ** 8, True)))):
+        s = torch.full((m, kb), 2.0 ** e, device="cuda")
+        one = torch.ones(n, kb, device="cuda")
+        if scales == "e8m0":
+            s, one = s.to(E8M0), one.to(E8M0)
+        qa, qb = amd.BlockScaled(a.to(E4M3), s), amd.BlockScaled(b.to(E4M3), one)
+        for alpha, inf in alphas:
+            flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+            base = torch.zeros(m, n, dtype=dtype, device="cuda") if based else None
+            got = amd.block_product(qa, qb, base, alpha, out_dtype=dtype, flags=flags)
+            assert bool(got[m - 1, n - 1].isinf()) == inf and int(flags) == (2 if inf else 0), (dtype, alpha)
+            assert int((got != 0).sum()) == 1
+    base = torch.zeros(m, n, dtype=torch.float16, device="cuda")              # a base that is not finite is the input's
+    base[m - 1, n - 1] = float("-inf")
+    flags.zero_()
+    amd.block_product(qa, qb, base, 0.0, out_dtype=torch.float16, flags=flags)
+    assert int(flags) == 3
