@@ -129,3 +129,59 @@ def test_products_that_their_type_stores_as_infinity_set_the_flag(m, n, k, scale
     flags.zero_()
     amd.block_product(qa, qb, base, 0.0, out_dtype=torch.float16, flags=flags)
     assert int(flags) == 3
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_product_of_a_block_of_zeros_with_large_scales(m, n, k, scales, dtype):
+    """A block whose codes are zeros on one side adds nothing, whatever its scales: 2^100 and 2^100 (their product is over float32's largest), in every
+    row and in squares of b.  All the rest whole numbers: the results are those without that block, bit for bit."""
+    import sd_mecha_amd as amd
+    g = torch.Generator(device="cuda").manual_seed(m)
+    va = torch.randint(-4, 5, (m, k), device="cuda", generator=g).float()
+    vb = torch.randint(-4, 5, (n, k), device="cuda", generator=g).float()
+    kb = R.blocks(k)
+    lone = 1 if kb > 1 else 0                                        # a's codes are zeros in this block, b's in the last
+    va[:, 128 * lone:128 * lone + 128] = 0
+    vb[:, 128 * (kb - 1):] = 0
+    want = (va.double() @ vb.double().t() * 2.0 ** -8).float().to(dtype)
+    for tile in (False, True):
+        sa = torch.ones(m, kb, device="cuda")
+        sb = torch.ones(R.blocks(n) if tile else n, kb, device="cuda")
+        for s in (sa, sb):
+            s[:, lone] = 2.0 ** 100
+            s[:, kb - 1] = 2.0 ** 100
+        if scales == "e8m0":
+            sa, sb = sa.to(E8M0), sb.to(E8M0)
+        got = amd.block_product(amd.BlockScaled(va.to(E4M3), sa), amd.BlockScaled(vb.to(E4M3), sb), alpha=2.0 ** -8, out_dtype=dtype)
+        assert torch.equal(got, want), tile
+
+
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_product_of_scales_whose_product_is_subnormal(m, n, k, tile):
+    """2^-70 and 2^-70 (1 + 2^-10): 2^-140 (1 + 2^-10) is no float32, but every block's sum times the first, and that times the second, is.  A block's
+    product and its addition are off by half a unit each of the sum so far, alpha by half of the result."""
+    import sd_mecha_amd as amd
+    kb = R.blocks(k)
+    a = amd.BlockScaled(torch.full((m, k), 448.0, device="cuda").to(E4M3), torch.full((m, kb), 2.0 ** -70, device="cuda"))
+    b = amd.BlockScaled(torch.full((n, k), 256.0, device="cuda").to(E4M3), torch.full((R.blocks(n) if tile else n, kb), 2.0 ** -70 * (1 + 2.0 ** -10), device="cuda"))
+    want = k * 448.0 * 256.0 * 2.0 ** -140 * (1 + 2.0 ** -10) * 2.0 ** 110
+    got = amd.block_product(a, b, alpha=2.0 ** 110).double()
+    assert bool(((got - want).abs() <= (2 * kb + 1) * 2.0 ** -24 * want).all())
+
+
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_product_with_one_scale_of_b_at_the_ends(m, n, k):
+    """Scales of b in squares, zero, subnormal and close to the largest, against ones of a that bring the results back to whole numbers."""
+    import sd_mecha_amd as amd
+    g = torch.Generator(device="cuda").manual_seed(n)
+    kb = R.blocks(k)
+    va, vb = (torch.randint(-4, 5, (x, k), device="cuda", generator=g).float() for x in (m, n))
+    whole = va.double() @ vb.double().t()
+    for sa, sb in ((2.0 ** 100, 2.0 ** -108), (2.0 ** -100, 2.0 ** 100), (1.0, 0.0), (2.0 ** 126, 0.0), (-3.0, 2.0 ** -60), (2.0 ** -140, 2.0 ** 100)):
+        for dtype in (torch.float32, torch.bfloat16):
+            a = amd.BlockScaled(va.to(E4M3), torch.full((m, kb), sa, device="cuda"))
+            b = amd.BlockScaled(vb.to(E4M3), torch.full((R.blocks(n), kb), sb, device="cuda"))
+            assert torch.equal(amd.block_product(a, b, out_dtype=dtype), (whole * (sa * sb)).float().to(dtype)), (sa, sb, dtype)
