@@ -6,6 +6,7 @@ from __future__ import annotations
 
 from contextlib import nullcontext
 from functools import lru_cache
+from operator import attrgetter
 from typing import Optional
 
 import torch
@@ -42,8 +43,9 @@ class BlockScaled:
     square (``tile``).  What a value stands for is ``values.float() * its scale``.
 
     The kernels read rows in whole blocks of 128 bytes: ``cast_blocks`` lays rows a multiple of 128 bytes apart (``pitch``), with zeros
-    behind the last column.  Values that lie otherwise (a stored tensor whose columns are no multiple of 128) are laid out so here, once."""
-    __slots__ = ("values", "scales", "rows", "cols", "tile", "pitch", "scale_pitch", "scale_code", "_packed")
+    behind the last column.  Values that lie otherwise (a stored tensor whose columns are no multiple of 128) are laid out so here, once.
+    The tensors' elements may change; which tensors they are may not."""
+    __slots__ = ("_values", "_scales", "_rows", "_cols", "_tile", "_pitch", "_scale_pitch", "_scale_code", "_packed")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor):
@@ -74,16 +76,29 @@ class BlockScaled:
         self._set(values, scales, rows, cols, s_rows != rows, pitch, s_pitch if s_rows > 1 else s_cols, code)
 
     def _set(self, values, scales, rows, cols, tile, pitch, scale_pitch, scale_code):
-        self.values, self.scales, self.rows, self.cols = values, scales, rows, cols
-        self.tile, self.pitch, self.scale_pitch, self.scale_code = tile, pitch, scale_pitch, scale_code
+        self._values, self._scales, self._rows, self._cols = values, scales, rows, cols
+        self._tile, self._pitch, self._scale_pitch, self._scale_code = tile, pitch, scale_pitch, scale_code
         self._packed = _pack(values.data_ptr(), scales.data_ptr(), rows, cols, pitch, scale_pitch, tile, scale_code)
+
+    # read-only: the addresses and sizes that the kernels get (_packed) are those of the tensors the matrix was made with
+    values, scales = property(attrgetter("_values")), property(attrgetter("_scales"))
+    rows, cols, tile = property(attrgetter("_rows")), property(attrgetter("_cols")), property(attrgetter("_tile"))
+    pitch, scale_pitch, scale_code = property(attrgetter("_pitch")), property(attrgetter("_scale_pitch")), property(attrgetter("_scale_code"))
 
     @property
     def shape(self) -> torch.Size:
-        return self.values.shape
+        return self._values.shape
+
+    def __reduce__(self):                                  # copies and pickles hold the tensors, as bytes: they get addresses of their own
+        scales = self._scales if self._scale_code == SCALE_F32 else self._scales.view(torch.uint8)
+        return _from_bytes, (self._values.view(torch.uint8), scales)
 
     def __repr__(self):
-        return f"BlockScaled({self.rows} x {self.cols}, {self.scales.dtype} scales {tuple(self.scales.shape)}, {self.values.device})"
+        return f"BlockScaled({self._rows} x {self._cols}, {self._scales.dtype} scales {tuple(self._scales.shape)}, {self._values.device})"
+
+
+def _from_bytes(values: torch.Tensor, scales: torch.Tensor) -> BlockScaled:
+    return BlockScaled(values.view(CODES), scales if scales.dtype == torch.float32 else scales.view(torch.float8_e8m0fnu))
 
 
 def _empty(rows: int, cols: int, tile: bool, device) -> BlockScaled:
@@ -101,8 +116,8 @@ def _empty(rows: int, cols: int, tile: bool, device) -> BlockScaled:
 def _check_blocks(q, what: str) -> None:
     if not isinstance(q, BlockScaled):
         raise TypeError(f"{what} takes a BlockScaled, got {type(q).__name__}")
-    if not q.values.is_cuda:
-        raise RuntimeError(f"{what}: the matrix is on {q.values.device}; the MI355X backend has no CPU path")
+    if not q._values.is_cuda:
+        raise RuntimeError(f"{what}: the matrix is on {q._values.device}; the MI355X backend has no CPU path")
 
 
 def _flags(device, flags, check_finite: bool):
@@ -157,7 +172,7 @@ def uncast_blocks(q: BlockScaled, *, key=None, out_dtype=None, flags=None, check
     dtype = out_dtype or torch.float32
     if dtype not in _DT:
         raise TypeError(f"uncast_blocks: unsupported out_dtype {dtype} (float32, float16, bfloat16)")
-    device, rows, cols = q.values.device, q.rows, q.cols
+    device, rows, cols = q._values.device, q._rows, q._cols
     out = torch.empty((rows, cols), dtype=dtype, device=device)
     if rows and cols:
         with _on(device):
@@ -186,9 +201,9 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
     stores as infinity sets bit 1."""
     _check_blocks(a, "block_product")
     _check_blocks(b, "block_product")
-    m, k, n, kb, device = a.rows, a.cols, b.rows, b.cols, a.values.device
-    if k != kb or b.values.get_device() != device.index:
-        raise ValueError(f"block_product: a {m} x {k} on {device} and b {n} x {kb} on {b.values.device} do not go together (a @ b.T)")
+    m, k, n, kb, device = a._rows, a._cols, b._rows, b._cols, a._values.device
+    if k != kb or b._values.get_device() != device.index:
+        raise ValueError(f"block_product: a {m} x {k} on {device} and b {n} x {kb} on {b._values.device} do not go together (a @ b.T)")
     if isinstance(alpha, torch.Tensor):
         if alpha.numel() != 1:
             raise NotImplementedError("block_product takes a scalar alpha")
@@ -216,11 +231,11 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         return out
     if k == 0:
         return out.zero_() if base is None else out if out is base else out.copy_(cast(base, out.dtype, key=key, flags=flags, check_finite=check_finite))
-    if a.scale_code != b.scale_code:
-        a, b = (q if q.scale_code == SCALE_F32 else BlockScaled(q.values, q.scales.to(torch.float32)) for q in (a, b))
+    if a._scale_code != b._scale_code:
+        a, b = (q if q._scale_code == SCALE_F32 else BlockScaled(q._values, q._scales.to(torch.float32)) for q in (a, b))
     with _on(device):
         word, fl = _flags(device, flags, check_finite)
-        size = _product_workspace(m, n, k, a.scale_code, b.tile, _DT[out.dtype])
+        size = _product_workspace(m, n, k, a._scale_code, b._tile, _DT[out.dtype])
         room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _lib.check(_lib.lib().mecha_block_product(
             a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),

@@ -185,3 +185,20 @@ def test_product_with_one_scale_of_b_at_the_ends(m, n, k):
             a = amd.BlockScaled(va.to(E4M3), torch.full((m, kb), sa, device="cuda"))
             b = amd.BlockScaled(vb.to(E4M3), torch.full((R.blocks(n), kb), sb, device="cuda"))
             assert torch.equal(amd.block_product(a, b, out_dtype=dtype), (whole * (sa * sb)).float().to(dtype)), (sa, sb, dtype)
+
+
+def test_product_of_copies_and_pickles():
+    """Copies multiply what they hold, also when the original has changed since."""
+    import copy
+    import pickle
+    import sd_mecha_amd as amd
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for scales in (torch.float32, E8M0):
+        a = amd.BlockScaled(torch.randn(40, 200, device="cuda", generator=g).to(E4M3), torch.full((40, 2), 0.5, device="cuda").to(scales))
+        b = amd.cast_blocks(torch.randn(50, 200, device="cuda", generator=g), tile=True)
+        want = amd.block_product(a, b)
+        copies = [copy.deepcopy((a, b)), pickle.loads(pickle.dumps((a, b)))]
+        a.values.view(torch.uint8).zero_()
+        assert not amd.block_product(a, b).any()
+        for x, y in copies:
+            assert x.scales.dtype == scales and torch.equal(amd.block_product(x, y), want)

@@ -1,0 +1,47 @@
+"""8-bit weights and the AdamW step without a GPU: copies, attributes and refusals."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def block_scaled(rows, cols, scales=torch.float32, tile=False):
+    import sd_mecha_amd as amd
+    g = torch.Generator().manual_seed(rows)
+    s = torch.rand((rows + 127) // 128 if tile else rows, (cols + 127) // 128, generator=g) + 0.5
+    return amd.BlockScaled(torch.randn(rows, cols, generator=g).to(E4M3), s.to(scales))
+
+
+def addresses(q):
+    from sd_mecha_amd import _lib
+    return _lib.BLOCK_MATRIX.unpack(q._packed)
+
+
+@pytest.mark.parametrize("rows, cols, scales, tile", [(4, 128, torch.float32, False), (300, 200, E8M0, True), (5, 77, torch.float32, False), (1, 1, E8M0, False)])
+def test_copies_of_a_block_scaled_matrix_have_addresses_of_their_own(rows, cols, scales, tile):
+    import sd_mecha_amd as amd
+    q = block_scaled(rows, cols, scales, tile)
+    file = io.BytesIO()
+    torch.save(q, file)
+    file.seek(0)
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), torch.load(file, weights_only=False), copy.copy(q)):
+        assert type(c) is amd.BlockScaled and c.shape == q.shape and c.tile == q.tile and c.scales.dtype == scales
+        assert torch.equal(c.values.view(torch.uint8), q.values.view(torch.uint8)) and torch.equal(c.scales.view(torch.uint8), q.scales.view(torch.uint8))
+        assert addresses(c) == (c.values.data_ptr(), c.scales.data_ptr(), rows, cols, c.pitch, c.scale_pitch, int(tile), c.scale_code)
+        assert c.pitch % 128 == 0 and c.values.stride(0) in (c.pitch, cols)
+    assert copy.deepcopy(q).values.data_ptr() != q.values.data_ptr()
+    assert addresses(q)[:2] == (q.values.data_ptr(), q.scales.data_ptr())
+
+
+def test_the_tensors_of_a_block_scaled_matrix_stay():
+    """The kernels get the addresses of the tensors that it was made with: others in their place would not be read."""
+    q = block_scaled(4, 256)
+    for name, value in (("values", q.values.clone()), ("scales", q.scales * 2), ("rows", 8), ("cols", 128), ("tile", True), ("pitch", 512), ("scale_pitch", 1), ("scale_code", 1)):
+        with pytest.raises(AttributeError):
+            setattr(q, name, value)
+    q.scales.mul_(2.0)                                                     # their elements may change
+    assert addresses(q)[1] == q.scales.data_ptr()
