@@ -102,6 +102,11 @@ class _Flags:
     """Device flag word for one call; raises like omit_non_finite / warns like _track_output."""
 
     def __init__(self, device, external: Optional[torch.Tensor], check: bool):
+        # the kernels OR 32 bits into its first element, by address
+        if external is not None and not (isinstance(external, torch.Tensor) and external.element_size() == 4 and not external.dtype.is_floating_point
+                                         and external.device == device and external.numel() >= 1):
+            got = f"{external.dtype} {tuple(external.shape)} on {external.device}" if isinstance(external, torch.Tensor) else type(external).__name__
+            raise ValueError(f"flags must be an int32 tensor of at least one element on {device}, got {got}")
         self.external = external
         self.check = check and external is None
         self.t = external if external is not None else (torch.zeros(1, dtype=torch.int32, device=device) if check else None)

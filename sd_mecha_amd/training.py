@@ -94,7 +94,7 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
         raise ValueError(f"adamw_step: weight_decay is a number or float32 [{keys}] on {device}")
     if max_norm is not None and not max_norm >= 0.0:
         raise ValueError(f"adamw_step: max_norm must not be negative, got {max_norm}")
-    if flags is not None and (flags.dtype != torch.int32 or flags.numel() != keys or flags.device != device or not flags.is_contiguous()):
+    if flags is not None and (not isinstance(flags, torch.Tensor) or flags.dtype != torch.int32 or flags.numel() != keys or flags.device != device or not flags.is_contiguous()):
         raise ValueError(f"adamw_step: flags must be int32 [{keys}] on {device}")
     if not params.is_cuda:
         raise RuntimeError(f"adamw_step: the arenas are on {device}; the MI355X backend has no CPU path")

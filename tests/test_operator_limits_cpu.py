@@ -45,3 +45,30 @@ def test_the_tensors_of_a_block_scaled_matrix_stay():
             setattr(q, name, value)
     q.scales.mul_(2.0)                                                     # their elements may change
     assert addresses(q)[1] == q.scales.data_ptr()
+
+
+@pytest.mark.parametrize("flags", [
+    torch.zeros(1, dtype=torch.int32),                                     # in host memory, where a kernel's atomic would fault
+    torch.zeros(1, dtype=torch.int32, device="meta"),
+    torch.zeros(1, dtype=torch.uint8),
+    torch.zeros(0, dtype=torch.int32),
+    torch.zeros(1),
+    [0],
+])
+def test_flag_words_that_a_kernel_could_not_write_are_refused(flags):
+    from sd_mecha_amd.merge_methods import _Flags
+    with pytest.raises(ValueError, match="flags must be"):
+        _Flags(torch.device("cuda", 0), flags, True)
+
+
+def test_flag_words_of_one_or_more_keys_are_taken():
+    from sd_mecha_amd.merge_methods import _Flags
+    for flags in (torch.zeros(1, dtype=torch.int32), torch.zeros(5, dtype=torch.int32)[2:], torch.zeros((), dtype=torch.int32), torch.zeros(3, dtype=torch.uint32)):
+        assert _Flags(torch.device("cpu"), flags, True).ptr.value == flags.data_ptr()
+
+
+def test_adamw_refuses_flags_that_are_no_tensor():
+    import sd_mecha_amd as amd
+    p = torch.zeros(128)
+    with pytest.raises(ValueError, match="flags"):
+        amd.adamw_step(p, p.clone(), segments=torch.tensor([[0, 128]]), step=1, flags=[0], **amd.adamw_state(128, "cpu"))
