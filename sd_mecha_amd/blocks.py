@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import SCALE_BLOCK, SCALE_E8M0, SCALE_F32
-from .merge_methods import _DT, _Flags, _resolve, cast
+from .merge_methods import _DT, _Flags, _resolve
 
 CODES = torch.float8_e4m3fn
 _SCALE_DT = {torch.float32: SCALE_F32, torch.float8_e8m0fnu: SCALE_E8M0}
@@ -229,8 +229,9 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
             raise ValueError("block_product: out may be base itself, of the same dtype, but not overlap it otherwise")
     if out.numel() == 0:
         return out
-    if k == 0:
-        return out.zero_() if base is None else out if out is base else out.copy_(cast(base, out.dtype, key=key, flags=flags, check_finite=check_finite))
+    if k == 0:                                             # an empty sum: one column of zeros
+        a, b = (BlockScaled(torch.zeros((rows, 1), dtype=torch.uint8, device=device).view(CODES), torch.ones((rows, 1), device=device)) for rows in (m, n))
+        k = 1
     if a._scale_code != b._scale_code:
         a, b = (q if q._scale_code == SCALE_F32 else BlockScaled(q._values, q._scales.to(torch.float32)) for q in (a, b))
     with _on(device):

@@ -202,3 +202,26 @@ def test_product_of_copies_and_pickles():
         assert not amd.block_product(a, b).any()
         for x, y in copies:
             assert x.scales.dtype == scales and torch.equal(amd.block_product(x, y), want)
+
+
+def test_product_over_no_columns_is_the_base():
+    """k = 0: the base, checked, flagged and written like that of any other product."""
+    import sd_mecha_amd as amd
+    m, n = 6, 40
+    a = amd.BlockScaled(torch.zeros(m, 0, device="cuda").to(E4M3), torch.ones(m, 0, device="cuda"))
+    b = amd.BlockScaled(torch.zeros(n, 0, device="cuda").to(E4M3), torch.ones(n, 0, device="cuda"))
+    base = torch.randn(m, n, device="cuda")
+    for dtype in TYPES:
+        assert torch.equal(amd.block_product(a, b, base, 3.0, out_dtype=dtype), base.to(dtype))
+        out = torch.empty(m * n, dtype=dtype, device="cuda")                   # of another shape than the base's
+        assert amd.block_product(a, b, base, out=out) is out and torch.equal(out.view(m, n), base.to(dtype))
+        assert not amd.block_product(a, b, out_dtype=dtype).any()
+    out = base.clone()
+    assert amd.block_product(a, b, out, out=out) is out and torch.equal(out, base)
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    base[m - 1, n - 1] = 65520.0
+    assert bool(amd.block_product(a, b, base, out_dtype=torch.float16, flags=flags)[m - 1, n - 1].isinf()) and int(flags) == 2
+    base[0, 0] = float("inf")
+    for out in (None, base, base.clone()):
+        with pytest.raises(amd.NonFiniteStateDictKeyError):
+            amd.block_product(a, b, base, out=out)
