@@ -10,6 +10,7 @@ from operator import attrgetter
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import SCALE_BLOCK, SCALE_E8M0, SCALE_F32
@@ -215,6 +216,7 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         base = base if base.is_contiguous() else base.contiguous()
     else:
         shape = (m, n)
+    given = out is not None
     if out is None:
         if out_dtype is not None and out_dtype not in _DT:
             raise TypeError(f"block_product: unsupported out_dtype {out_dtype} (float32, float16, bfloat16)")
@@ -241,6 +243,8 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         _lib.check(_lib.lib().mecha_block_product(
             a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),
             _DT[out.dtype], alpha, word, room.data_ptr() if size else None, size, _stream(device)), "mecha_block_product")
+        if given:                                         # written in place: a backward pass that saved it before raises
+            increment_version(out)
         if fl is not None:
             fl.finish(key)
     return out

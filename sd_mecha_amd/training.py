@@ -6,6 +6,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import SCALE_BLOCK
@@ -117,4 +118,6 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
             flags.data_ptr() if flags is not None else 0, n, 0 if on_device else int(step), lr, betas[0], betas[1], eps,
             0.0 if per_key else weight_decay, keys, _DT[params.dtype], _DT[grads.dtype], _DT[copy.dtype] if copy is not None else _lib.F32,
             8 if bits8 else 32, int(seed) & 0xFFFFFFFF), stream), "mecha_batched_adamw")
+    # written in place: a backward pass that saved one of them before raises, as behind torch's own steps
+    increment_version([t for t in (params, exp_avg, exp_avg_sq, exp_avg_scales, exp_avg_sq_scales, copy, flags) if t is not None])
     return norm[:1] if norm is not None else None

@@ -225,3 +225,36 @@ def test_product_over_no_columns_is_the_base():
     for out in (None, base, base.clone()):
         with pytest.raises(amd.NonFiniteStateDictKeyError):
             amd.block_product(a, b, base, out=out)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_between_forward_and_backward_is_noticed(bits):
+    """What a backward pass saved is written in place: it raises, as behind torch's own in-place operations, and makes no gradient of other weights."""
+    import sd_mecha_amd as amd
+    n = 256
+    seg, x = torch.tensor([[0, n]], device="cuda"), torch.randn(n, device="cuda", requires_grad=True)
+    st = amd.adamw_state(n, "cuda", bits)
+    p, copy = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+    w = p[:128].view(8, 16)                                          # a key's view of the arena
+    for saved in (p, copy, w):
+        loss = (x[:saved.numel()].view_as(saved) * saved).sum()
+        amd.adamw_step(p, torch.ones(n, device="cuda"), segments=seg, step=1, copy=copy, **st)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = [t._version for t in st.values()]
+    amd.adamw_step(p, torch.ones(n, device="cuda"), segments=seg, step=2, **st)
+    assert all(t._version > v for t, v in zip(st.values(), before))
+    (x * p).sum().backward()
+    assert torch.equal(x.grad, p)
+
+
+def test_a_product_into_a_saved_tensor_is_noticed():
+    import sd_mecha_amd as amd
+    a, b = amd.cast_blocks(torch.randn(8, 128, device="cuda")), amd.cast_blocks(torch.randn(16, 128, device="cuda"))
+    x, out = torch.randn(8, 16, device="cuda", requires_grad=True), torch.randn(8, 16, device="cuda")
+    loss = (x * out).sum()
+    amd.block_product(a, b, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        amd.block_product(a, b, out=torch.empty(8, 16, device="cuda"))
