@@ -497,11 +497,11 @@ typedef struct mecha_adamw {
     const void *grads;
     void *exp_avg;                    /* state_bits 32: m and v, float32; 8: e4m3 codes of m and of sqrt(v), 8-byte aligned, with */
     void *exp_avg_sq;                 /*   power-of-two scales [total_elems / 128] in *_scales; the codes are rounded up or down by a hash */
-    void *exp_avg_scales;             /*   of (offset, step, seed).  Segment offsets and total_elems are multiples of 128 then, and the */
-    void *exp_avg_sq_scales;          /*   codes behind a key's last element, up to a multiple of 128, become 0.  Moments that are not finite */
+    void *exp_avg_scales;             /*   of (offset, step, seed).  total_elems is a multiple of 128 then, and the codes behind a key's last */
+    void *exp_avg_sq_scales;          /*   element, up to the next key or a multiple of 128, become 0.  Moments that are not finite */
                                       /*   take no part in a scale; the NaN code of a root stands for an infinite one */
     void *copy;                       /* arena that receives the new weights once more, may be NULL */
-    const mecha_segment *segments;    /* sorted; elements outside them are left as they are */
+    const mecha_segment *segments;    /* sorted, at multiples of 8; elements outside them are left as they are */
     const float *key_weight_decay;    /* float[n_segments], may be NULL: weight_decay for all */
     const int64_t *step_dev;          /* read instead of `step` when the kernel runs (for captured graphs), may be NULL */
     const float *clip;                /* float[2] of mecha_batched_grad_norm, may be NULL; with a NaN coefficient the step changes nothing */

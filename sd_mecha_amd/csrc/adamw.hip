@@ -10,8 +10,8 @@
 // thread on a flat grid, 4 elements with float32 states and 8 with 8-bit ones; a vector lies in one key (offsets are multiples of
 // 8), its key is found by a search over the segment table that a wave does once, behind the loads.
 //
-// 8-bit states: e4m3 codes and a power-of-two scale for every 128 elements of the arena (segment offsets are multiples of 128, so
-// a block belongs to one key; 16 lanes own it).  The second moment is kept as its ROOT: e4m3 spans 2^18 between its largest and its
+// 8-bit states: e4m3 codes and a power-of-two scale for every 128 elements of the arena; 16 lanes own a block, also one that several
+// keys share.  The second moment is kept as its ROOT: e4m3 spans 2^18 between its largest and its
 // smallest code, which squared would be only 2^9 of gradient magnitudes.  A code's distance is up to 1/8 of its value and a moving mean
 // changes by (1 - b2) of itself a step, so rounding to nearest would never move it: |x| is rounded up with probability equal
 // to its part of the distance, by 16 bits of a hash of (offset, step, seed).  A root that is not zero never becomes zero: the
@@ -298,7 +298,9 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
             __builtin_nontemporal_store(u32x2{(uint32_t)mw[0], (uint32_t)mw[1]}, reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.m) + i));
             __builtin_nontemporal_store(u32x2{(uint32_t)vw[0], (uint32_t)vw[1]}, reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.v) + i));
         }
-        if ((threadIdx.x & 15) == 0 && valid) { a.ms[i >> 7] = (uint8_t)(em + 127); a.vs[i >> 7] = (uint8_t)(ev + 127); }
+        // (the block's first lane may lie in front of its first key)
+        const bool any = (__ballot(valid) >> (threadIdx.x & 48)) & 0xffffull;
+        if ((threadIdx.x & 15) == 0 && any) { a.ms[i >> 7] = (uint8_t)(em + 127); a.vs[i >> 7] = (uint8_t)(ev + 127); }
     } else {
         store(std::integral_constant<int, MECHA_F32>{}, a.m, m);
         store(std::integral_constant<int, MECHA_F32>{}, a.v, v);

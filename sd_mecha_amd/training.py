@@ -54,8 +54,8 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
         p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
 
     in float32, whatever the arenas hold.  ``params``, ``grads``: arenas of float32, float16 or bfloat16; ``segments``: the layout's
-    ``device_segments`` table (sorted; elements outside it stay as they are).  ``exp_avg``, ``exp_avg_sq``: m and v in float32, or, with
-    their ``_scales``, e4m3 codes of m and of sqrt(v) with a power of two for every 128 elements; segments then start at multiples of 128.
+    ``device_segments`` table (sorted, at multiples of 8 as every layout's; elements outside it stay as they are).  ``exp_avg``, ``exp_avg_sq``: m and v in float32, or, with
+    their ``_scales``, e4m3 codes of m and of sqrt(v) with a power of two for every 128 elements.
     8-bit codes are rounded up or down by a hash of (offset, step, ``seed``), so that slow means move on average.
 
     ``step`` counts from 1: an int, or an int64 tensor on the device that the kernel reads (for captured graphs).  ``weight_decay``: a

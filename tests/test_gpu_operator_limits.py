@@ -83,6 +83,30 @@ def test_weights_that_their_type_stores_as_infinity_set_the_flag(n, bits):
         assert bool(p[n - 1].isinf()) == over and int(flags) == (2 if over else 0), lr
 
 
+@pytest.mark.parametrize("step", [1, 50])
+def test_8bit_states_of_keys_that_share_blocks(step):
+    """Keys at multiples of 8: several in a block of 128, one behind the block's first elements, one over three blocks, one of one element."""
+    import sd_mecha_amd as amd
+    from sd_mecha_amd.arena import ArenaLayout
+    from test_gpu_adamw import HYPER, check_codes, expected, inside, make, near
+    layout = ArenaLayout(list("abcdefg"), [40, 20, 200, 1, 9, 77, 30], [8, 64, 184, 512, 520, 568, 760], 1024)
+    s, mask = make(layout, torch.bfloat16, torch.bfloat16, bits=8), inside(layout)
+    s["grads"] *= 64                                                # so that every block's scales change
+    decay = torch.linspace(0, 0.3, 7, device="cuda")
+    p, m, v, ep, em, ev = expected(s, layout, step, decay.cpu().numpy())
+    idle = s["exp_avg_scales"].view(torch.uint8)[7].clone()
+    s["exp_avg_scales"].view(torch.uint8)[7] = 3                     # no key reaches into the last block
+    amd.adamw_step(**s, step=step, weight_decay=decay, seed=11, **HYPER)
+    assert int(s["exp_avg_scales"].view(torch.uint8)[7]) == 3
+    s["exp_avg_scales"].view(torch.uint8)[7] = idle
+    near(s["params"], p, ep, mask)
+    assert bool((s["params"].float().cpu()[~torch.from_numpy(mask)] == 5.0).all())
+    u = R.dither(layout.total_elems, step, 11)
+    rel = float((em[mask] / np.maximum(np.abs(m[mask]), 1e-30)).mean())
+    check_codes(s["exp_avg"], s["exp_avg_scales"], m, rel, (u & np.uint64(0xFFFF)).astype(np.float64), False, mask)
+    check_codes(s["exp_avg_sq"], s["exp_avg_sq_scales"], np.sqrt(v), 5 * R.U, (u >> np.uint64(16)).astype(np.float64), True, mask)
+
+
 # --------------------------------------------------------------------------------------------------------------- uncast
 @pytest.mark.parametrize("cols", [128, 125])
 def test_uncast_values_that_their_type_stores_as_infinity_set_the_flag(cols):
