@@ -468,11 +468,11 @@ typedef struct mecha_block_matrix {
  * max|x| <= 448 * 2^e (e >= -127), codes to nearest even; the bytes of a row behind the last column, up to a multiple of 128, become 0.
  * `straight` [rows][cols] / `transposed` [cols][rows] (either may be NULL, their scales MECHA_SCALE_E8M0 and both of the same `tile`): where the
  * codes go of the matrix, and of its transpose -- with tile == 0 that has scales of its own, for 128 original rows of one column.  inf and
- * NaN become the NaN code, take no part in a scale, and set bit 0 of flags. */
+ * NaN become the NaN code, take no part in a scale, and set bit 0 of flags.  What is written shares no memory with the key or with each other. */
 int mecha_cast_blocks(const void *a, int64_t row_stride, int in_dtype, const mecha_block_matrix *straight, const mecha_block_matrix *transposed,
                       uint32_t *flags, void *stream);
 /* codes * scales in float32, then rounded to out_dtype; out is contiguous [rows][cols].  NaN codes and non-finite scales set bit 0 of
- * flags, non-finite results bit 1. */
+ * flags, non-finite results bit 1.  out shares no memory with the codes and scales. */
 int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, uint32_t *flags, void *stream);
 
 /* out[m][n] = base[m][n] + alpha * sum_k a[m][k] b[n][k], a and b block-scaled along k, both with scales of one type; base (may be
@@ -480,7 +480,8 @@ int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, u
  * neighbouring k are first cut off under 2^-13 of the largest of them (the 8-bit matrix instructions).  Values (code * scale) have to be
  * float32 numbers; float32 scales: a block's sum is multiplied by b's and then by a's, so those of b should lie from 2^-108 to 2^103 or be 0;
  * powers of two with a float32 result: values under 2^-123 may be rounded to a multiple of 2^-133.  bit 0 of flags: a NaN came out
- * or base holds inf / NaN; bit 1: an output is inf / NaN.  out shares no memory with a, b or (but for out == base) base. */
+ * or base holds inf / NaN; bit 1: an output is inf / NaN.  out shares no memory with a, b or (but for out == base) base,
+ * and the workspace none with any of them. */
 int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
                         float alpha, uint32_t *flags, void *workspace, size_t workspace_bytes, void *stream);
 /* What a product of m x n results over k can use (0 for most): float32 sums of parts of k, for results too few to fill the chip.  With

@@ -1310,6 +1310,12 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     Choice c = choose(m, n, k, mode, b_tile, large_ok, workspace != nullptr);
     if (c.splits > 1 && ((size_t)c.splits * (size_t)m * (size_t)part_ld(n) * sizeof(float) > workspace_bytes || !mecha_aligned16(workspace))) c = choose(m, n, k, mode, b_tile, large_ok, false);
     p.splits = c.splits;
+    if (c.splits > 1) {
+        const size_t parts = (size_t)c.splits * (size_t)m * (size_t)part_ld(n) * sizeof(float);
+        MECHA_REQUIRE(!mecha_overlap(workspace, parts, out, out_bytes) && !mecha_overlap(workspace, parts, base, (size_t)m * n * mecha_dtype_size(base_dtype)), "workspace shares memory with out or base");
+        for (const mecha_block_matrix *q : {a, b})
+            MECHA_REQUIRE(!mecha_overlap(workspace, parts, q->codes, mecha_codes_bytes(*q)) && !mecha_overlap(workspace, parts, q->scales, mecha_scales_bytes(*q)), "workspace shares memory with a or b");
+    }
     if (c.direct >= 0) {
         if (wide) return e8m0 ? launch_direct<EXACT_E8M0>(c.direct, p, s) : launch_direct<EXACT_F32>(c.direct, p, s);
         return e8m0 ? launch_direct<HW_SCALES>(c.direct, p, s) : launch_direct<F32_SCALES>(c.direct, p, s);

@@ -78,6 +78,17 @@ static inline size_t mecha_scales_bytes(const mecha_block_matrix &q) {
     return rows && q.cols ? ((size_t)(rows - 1) * q.scale_pitch + (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK) * (q.scale_dtype == MECHA_SCALE_F32 ? 4 : 1) : 0;
 }
 
+// whether two matrices' codes share memory; rows of one pitch may lie side by side
+static inline bool mecha_codes_overlap(const mecha_block_matrix &a, const mecha_block_matrix &b) {
+    if (!mecha_overlap(a.codes, mecha_codes_bytes(a), b.codes, mecha_codes_bytes(b))) return false;
+    if (a.pitch != b.pitch) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.codes), y = reinterpret_cast<uintptr_t>(b.codes);
+    const mecha_block_matrix &low = x < y ? a : b, &high = x < y ? b : a;
+    auto width = [](const mecha_block_matrix &q) { return (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK * SCALE_BLOCK; };
+    const int64_t apart = (int64_t)((x < y ? y - x : x - y) % (uintptr_t)a.pitch);
+    return apart < width(low) || apart + width(high) > a.pitch;
+}
+
 // the layout of include/mecha_hip.h for one matrix; an error message and code where it is not kept
 static inline int mecha_check_blocks(const char *what, const mecha_block_matrix &q) {
     const int64_t blocks = (q.cols + SCALE_BLOCK - 1) / SCALE_BLOCK;

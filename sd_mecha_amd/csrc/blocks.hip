@@ -385,6 +385,18 @@ int mecha_cast_blocks(const void *a, int64_t row_stride, int in_dtype, const mec
                       (long long)transposed->rows, (long long)transposed->cols, (long long)cols, (long long)rows);
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(a != nullptr && row_stride >= cols, "a is NULL or its rows overlap (stride %lld, %lld columns)", (long long)row_stride, (long long)cols);
+    const size_t a_bytes = ((size_t)(rows - 1) * row_stride + cols) * mecha_dtype_size(in_dtype);
+    for (const mecha_block_matrix *q : {straight, transposed}) {
+        if (!q) continue;
+        const size_t codes = mecha_codes_bytes(*q), scales = mecha_scales_bytes(*q);
+        MECHA_REQUIRE(!mecha_overlap(a, a_bytes, q->codes, codes) && !mecha_overlap(a, a_bytes, q->scales, scales) && !mecha_overlap(q->codes, codes, q->scales, scales),
+                      "a cast's codes or scales share memory with the key or with each other");
+    }
+    if (straight && transposed)
+        MECHA_REQUIRE(!mecha_codes_overlap(*straight, *transposed) && !mecha_overlap(straight->codes, mecha_codes_bytes(*straight), transposed->scales, mecha_scales_bytes(*transposed))
+                      && !mecha_overlap(straight->scales, mecha_scales_bytes(*straight), transposed->codes, mecha_codes_bytes(*transposed))
+                      && !mecha_overlap(straight->scales, mecha_scales_bytes(*straight), transposed->scales, mecha_scales_bytes(*transposed)),
+                      "a cast's two matrices share memory");
     CastParams p{a, rows, cols, row_stride, nullptr, 0, nullptr, 0, nullptr, 0, nullptr, 0, flags};
     if (straight) { p.q = static_cast<uint8_t *>(straight->codes); p.q_pitch = straight->pitch; p.s = static_cast<uint8_t *>(straight->scales); p.s_pitch = straight->scale_pitch; }
     if (transposed) { p.qt = static_cast<uint8_t *>(transposed->codes); p.qt_pitch = transposed->pitch; p.st = static_cast<uint8_t *>(transposed->scales); p.st_pitch = transposed->scale_pitch; }
@@ -416,6 +428,8 @@ int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, u
     const int64_t rows = q->rows, cols = q->cols;
     if (rows == 0 || cols == 0) return MECHA_OK;
     MECHA_REQUIRE(out != nullptr, "out is NULL");
+    const size_t out_bytes = (size_t)rows * cols * mecha_dtype_size(out_dtype);
+    MECHA_REQUIRE(!mecha_overlap(out, out_bytes, q->codes, mecha_codes_bytes(*q)) && !mecha_overlap(out, out_bytes, q->scales, mecha_scales_bytes(*q)), "out shares memory with the codes or scales");
     const int64_t vec_per_row = (cols + 7) / 8, blocks = (rows * vec_per_row + MECHA_BLOCK - 1) / MECHA_BLOCK;
     MECHA_REQUIRE(blocks * MECHA_BLOCK < (1ll << 32), "%lld x %lld is beyond one launch", (long long)rows, (long long)cols);
     const bool vec = mecha_aligned16(out) && cols % 8 == 0;

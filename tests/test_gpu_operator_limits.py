@@ -282,3 +282,18 @@ def test_a_product_into_a_saved_tensor_is_noticed():
         loss.backward()
     with torch.inference_mode():
         amd.block_product(a, b, out=torch.empty(8, 16, device="cuda"))
+
+
+@pytest.mark.parametrize("tile", [False, True])
+def test_cast_into_two_matrices_side_by_side(tile):
+    """Straight and transposed codes in the rows of one buffer, through the C entry: the bytes of one lie between those of the other."""
+    import sd_mecha_amd as amd
+    from sd_mecha_amd import _lib
+    n = 200
+    a = torch.randn(n, n, device="cuda")
+    want = amd.cast_blocks(a, tile=tile, sides="both")
+    room, scales = torch.full((n, 512), 0x55, dtype=torch.uint8, device="cuda"), [torch.zeros_like(q.scales.view(torch.uint8)) for q in want]
+    packed = [_lib.BLOCK_MATRIX.pack(room.data_ptr() + 256 * i, s.data_ptr(), n, n, 512, s.shape[1], tile, _lib.SCALE_E8M0) for i, s in enumerate(scales)]
+    _lib.check(_lib.lib().mecha_cast_blocks(a.data_ptr(), n, _lib.F32, packed[0], packed[1], None, torch.cuda.current_stream().cuda_stream), "mecha_cast_blocks")
+    for i, (q, s) in enumerate(zip(want, scales)):
+        assert torch.equal(room[:, 256 * i:256 * i + n], q.values.view(torch.uint8)) and not room[:, 256 * i + n:256 * i + 256].any() and torch.equal(s, q.scales.view(torch.uint8))

@@ -72,3 +72,34 @@ def test_adamw_refuses_flags_that_are_no_tensor():
     p = torch.zeros(128)
     with pytest.raises(ValueError, match="flags"):
         amd.adamw_step(p, p.clone(), segments=torch.tensor([[0, 128]]), step=1, flags=[0], **amd.adamw_state(128, "cpu"))
+
+
+def test_c_entries_refuse_shared_memory_before_any_launch():
+    """Host checks only: the addresses lie apart but for a byte or two, and nothing is launched."""
+    from sd_mecha_amd import _lib
+    L = _lib.lib()
+    far = [1 << 32, 2 << 32, 3 << 32, 4 << 32, 5 << 32, 6 << 32, 7 << 32]
+
+    def matrix(codes, scales, rows=100, cols=200, pitch=256, sp=2, tile=0, sdt=1):
+        return _lib.BLOCK_MATRIX.pack(codes, scales, rows, cols, pitch, sp, tile, sdt)
+
+    def cast(a=far[0], q=(far[1], far[2]), qt=(far[3], far[4]), ld=200, pitch=256):
+        return L.mecha_cast_blocks(a, ld, _lib.F32, matrix(*q, pitch=pitch) if q else None, matrix(*qt, rows=200, cols=100, pitch=pitch, sp=1) if qt else None, None, None)
+    codes, key = 99 * 256 + 256, 4 * (99 * 200 + 200)
+    for bad in (dict(q=(far[0] + (key - 16), far[2])), dict(q=(far[0] - (codes - 16), far[2]), qt=None), dict(q=(far[1], far[0] + key - 1)), dict(q=(far[1], far[1] + codes - 1), qt=None),
+                dict(qt=(far[0] - 16, far[4])), dict(q=None, qt=(far[3], far[3] + 5)), dict(q=None, qt=(far[3], far[0] - 199)),
+                dict(qt=(far[1] + codes - 16, far[4])), dict(qt=(far[1] + 128, far[4])), dict(qt=(far[3], far[1])), dict(qt=(far[2] + 192, far[4])), dict(qt=(far[3], far[2] + 199)),
+                dict(q=(far[1], far[2]), qt=(far[1] + 128, far[4]), pitch=384), dict(q=(far[1], far[2]), qt=(far[1] + 384, far[4]), pitch=384)):
+        assert cast(**bad) < 0 and b"share memory" in L.mecha_last_error(), bad
+
+    def un(out, rows=100, cols=200):
+        return L.mecha_uncast_blocks(matrix(far[0], far[1]), out, _lib.F16, None, None)
+    for out in (far[0], far[0] + codes - 1, far[0] - 2 * 100 * 200 + 1, far[1] + 199, far[1] - 1):
+        assert un(out) < 0 and b"shares memory" in L.mecha_last_error(), out
+
+    m, n, k = 1024, 1280, 5120
+    size = L.mecha_block_product_workspace_bytes(m, n, k, 1, 0, _lib.BF16)
+    assert size > 0
+    a, b = matrix(far[0], far[1], m, k, k, 40), matrix(far[2], far[3], n, k, k, 40)
+    for room in (far[0] - 16, far[1] - 16, far[2] + n * k - 16, far[3] + 16, far[4] + 2 * m * n - 16, far[4] - size + 16, far[5] + 2 * m * n - 16):
+        assert L.mecha_block_product(a, b, far[5], _lib.BF16, far[4], _lib.BF16, 1.0, None, room, size, None) < 0 and b"workspace shares" in L.mecha_last_error(), room
