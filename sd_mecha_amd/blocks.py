@@ -238,7 +238,8 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
         a, b = (q if q._scale_code == SCALE_F32 else BlockScaled(q._values, q._scales.to(torch.float32)) for q in (a, b))
     with _on(device):
         word, fl = _flags(device, flags, check_finite)
-        size = _product_workspace(m, n, k, a._scale_code, b._tile, _DT[out.dtype])
+        # (a base of another type is added by kernels that do not share k out)
+        size = _product_workspace(m, n, k, a._scale_code, b._tile, _DT[out.dtype]) if base is None or base.dtype == out.dtype else 0
         room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _lib.check(_lib.lib().mecha_block_product(
             a._packed, b._packed, base.data_ptr() if base is not None else None, _DT[base.dtype] if base is not None else _lib.F32, out.data_ptr(),

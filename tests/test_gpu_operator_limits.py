@@ -297,3 +297,18 @@ def test_cast_into_two_matrices_side_by_side(tile):
     _lib.check(_lib.lib().mecha_cast_blocks(a.data_ptr(), n, _lib.F32, packed[0], packed[1], None, torch.cuda.current_stream().cuda_stream), "mecha_cast_blocks")
     for i, (q, s) in enumerate(zip(want, scales)):
         assert torch.equal(room[:, 256 * i:256 * i + n], q.values.view(torch.uint8)) and not room[:, 256 * i + n:256 * i + 256].any() and torch.equal(s, q.scales.view(torch.uint8))
+
+
+def test_product_with_a_base_of_another_type_takes_no_room_for_parts():
+    import sd_mecha_amd as amd
+    m, n, k = 1024, 1280, 5120
+    a, b = amd.cast_blocks(torch.randn(m, k, device="cuda")), amd.cast_blocks(torch.randn(n, k, device="cuda"), tile=True)
+    assert amd.blocks._product_workspace(m, n, k, 1, True, 2) > 0
+    base = torch.randn(m, n, device="cuda")
+
+    def extra(**kw):
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        amd.block_product(a, b, base, out_dtype=torch.bfloat16, check_finite=False)
+        return torch.cuda.max_memory_allocated() - before
+    assert extra() == 2 * m * n
