@@ -487,6 +487,10 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
 /* What a product of m x n results over k can use (0 for most): float32 sums of parts of k, for results too few to fill the chip.  With
  * less, or NULL, k is not shared out. */
 size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype);
+/* How such a product is made, given its whole workspace: rows << 20 | columns << 8 | parts of k, of the results a workgroup makes (16 to 32 rows:
+ * straight from memory; 128 x 128; 128, 192 or 256 x 256, the only ones made in parts).  other_base: with a base of another type than the
+ * result's.  For profiles and tests; 0 for an empty product. */
+int mecha_block_product_tile(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype, int other_base);
 
 /* ------------------------------------------------------------------ training step
  * One AdamW step (decoupled weight decay) for every key of the arenas, in place, in one launch:

@@ -120,6 +120,7 @@ SIGNATURES = {
     "mecha_uncast_blocks": (c_i, [c_p, c_p, c_i, c_p, c_p]),
     "mecha_block_product": (c_i, [c_p, c_p, c_p, c_i, c_p, c_i, c_f, c_p, c_p, c_sz, c_p]),
     "mecha_block_product_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i, c_i, c_i]),
+    "mecha_block_product_tile": (c_i, [c_i64, c_i64, c_i64, c_i, c_i, c_i, c_i]),
     "mecha_batched_adamw": (c_i, [c_p, c_p]),
     "mecha_batched_grad_norm_workspace_bytes": (c_sz, [c_i64]),
     "mecha_batched_grad_norm": (c_i, [c_p, c_p, c_i, c_i64, c_i, c_d, c_p, c_p, c_sz, c_p]),

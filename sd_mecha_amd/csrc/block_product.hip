@@ -1233,6 +1233,13 @@ int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
 //           and read once as float32 and joined by a second launch: 1280 x 1280 x 8269 32 us in 5 parts (55 in one; float32 results 39 and 100),
 //           1024 x 1280 x 5120 25 (36), 300 x 2560 x 8192 24 (53); 320 x 320 x 8269 stays with the direct kernel: 15 us, 16 in 13 parts.
 constexpr int MAX_SPLITS = 32;
+int mode_of(int scale_dtype, int out_dtype) {
+    const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
+    return out_dtype == MECHA_F32 ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES;
+}
+// The large kernel reads base as it stores the result, and scales four blocks at a time.
+bool large_kernels(int64_t k, bool other_base) { return k > 3 * SCALE_BLOCK && !other_base; }
+constexpr int DIRECT_ROWS[4] = {16, 16, 32, 32}, DIRECT_COLS[4] = {16, 32, 32, 64};
 struct Choice { int direct = -1, mi = 0, splits = 1; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
 Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_ok, bool split_ok) {
     // a step of 128 x 128, MI = 4, 6, 8: power-of-two scales; float32 scales with one of b's in a square; with one in every row of b, where MI = 8
@@ -1255,7 +1262,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_
             if (t < best) { best = t; c.mi = 4; c.splits = x; }
         }
     }
-    static const int rows[4] = {16, 16, 32, 32}, cols[4] = {16, 32, 32, 64};
+    const int *const rows = DIRECT_ROWS, *const cols = DIRECT_COLS;
     for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 32 us, 16 without it)
         const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * (bytes / 5e6 + 0.001 + 2e-6 * rows[d] * cols[d]);
         const double t = 2.5 + 0.001 * rows[d] * cols[d] + (one > all ? one : all);
@@ -1269,10 +1276,16 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_
 extern "C" {
 
 size_t mecha_block_product_workspace_bytes(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype) {
-    const bool wide = out_dtype == MECHA_F32, e8m0 = scale_dtype == MECHA_SCALE_E8M0;
-    if (m < 1 || n < 1 || k <= 3 * SCALE_BLOCK) return 0;
-    const Choice c = choose(m, n, k, wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES, b_tile, true, true);
+    if (m < 1 || n < 1 || !large_kernels(k, false)) return 0;
+    const Choice c = choose(m, n, k, mode_of(scale_dtype, out_dtype), b_tile, true, true);
     return c.splits > 1 ? (size_t)c.splits * (size_t)m * (size_t)part_ld(n) * sizeof(float) : 0;
+}
+
+int mecha_block_product_tile(int64_t m, int64_t n, int64_t k, int scale_dtype, int b_tile, int out_dtype, int other_base) {
+    if (m < 1 || n < 1 || k < 1) return 0;
+    const Choice c = choose(m, n, k, mode_of(scale_dtype, out_dtype), b_tile, large_kernels(k, other_base), !other_base);
+    const int tm = c.direct >= 0 ? DIRECT_ROWS[c.direct] : c.mi ? 32 * c.mi : 128, tn = c.direct >= 0 ? DIRECT_COLS[c.direct] : c.mi ? BIG_N : 128;
+    return tm << 20 | tn << 8 | c.splits;
 }
 
 int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
@@ -1302,11 +1315,10 @@ int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b
     const int b_tile = b->tile, scale_dtype = a->scale_dtype;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
-    // The large kernel reads base as it stores the result, and scales four blocks at a time.
     const bool wide = out_dtype == MECHA_F32;
-    const bool large_ok = k > 3 * SCALE_BLOCK && (base == nullptr || base_dtype == out_dtype);
+    const bool large_ok = large_kernels(k, base != nullptr && base_dtype != out_dtype);
     p.aligned = n % (wide ? 4 : 8) == 0 && mecha_aligned16(out) && (base == nullptr || mecha_aligned16(base));
-    const int mode = wide ? (e8m0 ? EXACT_E8M0 : EXACT_F32) : e8m0 ? HW_SCALES : F32_SCALES;
+    const int mode = mode_of(scale_dtype, out_dtype);
     Choice c = choose(m, n, k, mode, b_tile, large_ok, workspace != nullptr);
     if (c.splits > 1 && ((size_t)c.splits * (size_t)m * (size_t)part_ld(n) * sizeof(float) > workspace_bytes || !mecha_aligned16(workspace))) c = choose(m, n, k, mode, b_tile, large_ok, false);
     p.splits = c.splits;

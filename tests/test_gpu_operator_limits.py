@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import blocks_reference as R
+from product_shapes import KERNELS
 
 pytestmark = pytest.mark.gpu
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -122,8 +123,9 @@ def test_uncast_values_that_their_type_stores_as_infinity_set_the_flag(cols):
 
 
 # -------------------------------------------------------------------------------------------------------------- product
-# one shape for each way a product takes: memory to registers, 128 x 128 tiles, larger tiles, parts of k that are joined
-WAYS = [(3, 40, 200), (40, 63, 300), (2100, 2056, 300), (2100, 1003, 700), (5000, 4200, 640), (1024, 1280, 5120), (900, 261, 8192)]
+# one shape for each kernel, for flags and scales
+WAYS = [(3, 41, 200), (300, 301, 1000), (200, 1000, 2300), (700, 701, 2300), (2100, 2056, 300), (1035, 3665, 2300), (6492, 2312, 700), (7241, 2080, 700), (8097, 2873, 700),
+        (1024, 1280, 5120), (900, 261, 8192)]
 
 
 @pytest.mark.parametrize("based", [False, True])
@@ -306,9 +308,89 @@ def test_product_with_a_base_of_another_type_takes_no_room_for_parts():
     assert amd.blocks._product_workspace(m, n, k, 1, True, 2) > 0
     base = torch.randn(m, n, device="cuda")
 
-    def extra(**kw):
+    def extra():
         torch.cuda.reset_peak_memory_stats()
         before = torch.cuda.memory_allocated()
         amd.block_product(a, b, base, out_dtype=torch.bfloat16, check_finite=False)
         return torch.cuda.max_memory_allocated() - before
     assert extra() == 2 * m * n
+
+
+# ------------------------------------------------------------------------------------------ every kernel, bit for bit
+def whole(rows, cols, form, scales, seed):
+    """Codes -4 .. 4 and scales 2^-1 .. 2^1 or 1 .. 3, and what they stand for in float64, on the GPU."""
+    import sd_mecha_amd as amd
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    v = torch.randint(-4, 5, (rows, cols), device="cuda", generator=g).float()
+    shape = (rows if form == "rows" else R.blocks(rows), R.blocks(cols))
+    s = torch.randint(1, 4, shape, device="cuda", generator=g).float()
+    if scales == "e8m0":
+        s = torch.exp2(s - 2).to(E8M0)
+    r, c = torch.arange(rows, device="cuda"), torch.arange(cols, device="cuda") // 128
+    return amd.BlockScaled(v.to(E4M3), s), v.double() * s.float().double()[r if form == "rows" else r // 128][:, c]
+
+
+@pytest.mark.parametrize("fa, fb", [("rows", "tile"), ("rows", "rows"), ("tile", "rows"), ("tile", "tile")])
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", [shape for shape, _ in KERNELS])
+def test_every_product_kernel_bit_for_bit(m, n, k, scales, fa, fb):
+    """Sums are multiples of 2^-2 and at most 64 k < 2^20 (powers of two), or of 1 and at most 144 k < 2^21 (whole scales): every partial sum is a float32
+    in any order, and so is 2^-7 of it with a whole base; products of codes up to 4 lie within 2^-13 of the largest.  So each result is the float64
+    one, rounded once."""
+    import sd_mecha_amd as amd
+    (a, va), (b, vb) = whole(m, k, fa, scales, m), whole(n, k, fb, scales, n + 1)
+    want = va @ vb.t() * 2.0 ** -7
+    base = torch.randint(-64, 65, (m, n), device="cuda")
+    onto = want + base.double()
+    for dtype in TYPES:
+        assert torch.equal(amd.block_product(a, b, alpha=2.0 ** -7, out_dtype=dtype), want.float().to(dtype)), dtype
+        bd, w = base.to(dtype), onto.float().to(dtype)
+        assert torch.equal(amd.block_product(a, b, bd, 2.0 ** -7, out_dtype=dtype), w), dtype
+        room = torch.full((m * n + 9,), 7.0, dtype=dtype, device="cuda")            # one element off, between others
+        assert torch.equal(amd.block_product(a, b, bd, 2.0 ** -7, out=room[1:m * n + 1]).view(m, n), w), dtype
+        assert float(room[0]) == 7.0 and bool((room[m * n + 1:] == 7.0).all())
+        assert torch.equal(amd.block_product(a, b, bd, 2.0 ** -7, out=bd), w), dtype
+        other = base.to(torch.float32 if dtype != torch.float32 else torch.bfloat16)
+        assert torch.equal(amd.block_product(a, b, other, 2.0 ** -7, out_dtype=dtype), w), dtype
+    v = a.values.clone()                                                            # a NaN code in the last row's last column
+    v.view(torch.uint8)[m - 1, k - 1] = 0x7F
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = amd.block_product(amd.BlockScaled(v, a.scales), b, alpha=2.0 ** -7, out_dtype=torch.bfloat16, flags=flags)
+    assert int(flags) == 3 and bool(got[m - 1].isnan().all()) and torch.equal(got[:m - 1], want[:m - 1].float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scales", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m, n, k", [(100, 300, 2300), (700, 701, 2300), (1035, 3672, 8500), (6492, 2312, 700), (8097, 2880, 700), (1024, 1280, 5120)])
+def test_what_the_8bit_instructions_lose(m, n, k, scales, dtype):
+    """1.5e-5 of a result (2-norm, normal codes) in front of the rounding to 16 bits: the first result as a base, negative, leaves what its rounding took off,
+    which its own rounding (half a step of half a step) hides nothing of.  A third more would be another instruction."""
+    import sd_mecha_amd as amd
+    from test_gpu_blocks import matrix
+    a, b = matrix(m, k, "rows", scales, 1), matrix(n, k, "tile", scales, 2)
+    r, c = torch.arange(n, device="cuda") // 128, torch.arange(k, device="cuda") // 128
+    want = (a.values.double() * a.scales.double()[:, c]) @ (b.values.double() * b.scales.double()[r][:, c]).t()
+    alpha = float(2.0 ** -torch.log2(want.abs().max()).ceil())                    # (within float16's range)
+    first = amd.block_product(a, b, alpha=alpha, out_dtype=dtype)
+    rest = amd.block_product(a, b, -first, alpha, out_dtype=dtype)
+    off = float((first.double() + rest.double() - want * alpha).norm() / (want * alpha).norm())
+    assert off < 2e-5, off
+
+
+# ------------------------------------------------------------------------------------------------------------------ cast
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_cast_16bit_magnitudes_at_the_ends(dtype, tile):
+    """Every pattern of the type that is finite, subnormal ones among them: blocks of neighbours, blocks of the smallest, and each next to a large one."""
+    import sd_mecha_amd as amd
+    from test_gpu_blocks import same_cast
+    bits = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype)
+    bits = bits[bits.isfinite()]
+    least = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -133
+    near = bits[:bits.numel() // 128 * 128].view(-1, 128)                           # neighbours in size
+    mixed = near.t().contiguous().view(-1, 128)                                     # all sizes in a block
+    small = (torch.arange(128 * 128).view(128, 128).double() * least).to(dtype)     # subnormal, and the first normal ones
+    for a in (near, mixed, small, small[:1], small[:3, :5], -small):
+        for x in (a.cuda(), a.cuda().t().contiguous()):
+            for q, y in zip(amd.cast_blocks(x, tile=tile, sides="both"), (x, x.t())):
+                same_cast(q, y, tile)

@@ -103,3 +103,27 @@ def test_c_entries_refuse_shared_memory_before_any_launch():
     a, b = matrix(far[0], far[1], m, k, k, 40), matrix(far[2], far[3], n, k, k, 40)
     for room in (far[0] - 16, far[1] - 16, far[2] + n * k - 16, far[3] + 16, far[4] + 2 * m * n - 16, far[4] - size + 16, far[5] + 2 * m * n - 16):
         assert L.mecha_block_product(a, b, far[5], _lib.BF16, far[4], _lib.BF16, 1.0, None, room, size, None) < 0 and b"workspace shares" in L.mecha_last_error(), room
+
+
+def test_the_shapes_of_the_product_tests_take_every_kernel():
+    """What the GPU tests rest on: if the choice of kernels changes, so do these shapes."""
+    from product_shapes import KERNELS, MODES
+    from sd_mecha_amd import _lib
+    L = _lib.lib()
+
+    def tile(m, n, k, scales, form, bits, other_base=0):
+        v = L.mecha_block_product_tile(m, n, k, _lib.SCALE_E8M0 if scales == "e8m0" else _lib.SCALE_F32, int(form == "tile"), _lib.F32 if bits == 32 else _lib.BF16, other_base)
+        return v >> 20, v >> 8 & 0xfff, v & 0xff
+    seen = [set() for _ in MODES]
+    for shape, tiles in KERNELS:
+        for i, (mode, want) in enumerate(zip(MODES, tiles)):
+            assert tile(*shape, *mode) == want, (shape, mode)
+            seen[i].add(want[:2] + (want[2] > 1,))
+            size = L.mecha_block_product_workspace_bytes(*shape, _lib.SCALE_E8M0 if mode[0] == "e8m0" else _lib.SCALE_F32, int(mode[1] == "tile"), _lib.F32 if mode[2] == 32 else _lib.BF16)
+            assert (size > 0) == (want[2] > 1)
+            assert tile(*shape, *mode, 1)[0] <= 128 and tile(*shape, *mode, 1)[2] == 1
+    few = {(16, 16, False), (16, 32, False), (32, 32, False), (128, 128, False), (128, 256, False), (128, 256, True)}
+    for got, more in zip(seen, ({(32, 64, False), (192, 256, False), (256, 256, False)}, {(32, 64, False), (192, 256, False), (256, 256, False)},
+                                {(32, 64, False), (192, 256, False)}, {(32, 64, False)}, set())):
+        assert got == few | more
+    assert L.mecha_block_product_tile(0, 8, 8, 1, 0, 0, 0) == 0
