@@ -394,3 +394,74 @@ def test_cast_16bit_magnitudes_at_the_ends(dtype, tile):
         for x in (a.cuda(), a.cuda().t().contiguous()):
             for q, y in zip(amd.cast_blocks(x, tile=tile, sides="both"), (x, x.t())):
                 same_cast(q, y, tile)
+
+
+@pytest.mark.parametrize("form", ["tile", "rows"])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_every_product_kernel_with_powers_of_two_at_the_ends(m, n, k, form):
+    """2^-127 and 2^-124 of a against large ones of b, bit for bit; and a NaN scale on either side makes its rows or columns, and only those, NaN."""
+    import sd_mecha_amd as amd
+    g = torch.Generator(device="cuda").manual_seed(k)
+    kb = R.blocks(k)
+    va, vb = (torch.randint(-4, 5, (x, k), device="cuda", generator=g).float() for x in (m, n))
+    exact = va.double() @ vb.double().t()
+
+    def matrix(v, byte, rows):
+        return amd.BlockScaled(v.to(E4M3), torch.full((rows, kb), byte, dtype=torch.uint8, device="cuda").view(E8M0))
+    rows_b = n if form == "rows" else R.blocks(n)
+    for ea, eb in ((0, 220), (3, 250), (240, 14), (127, 1)):
+        for dtype in (torch.float32, torch.bfloat16):
+            got = amd.block_product(matrix(va, ea, m), matrix(vb, eb, rows_b), out_dtype=dtype)
+            assert torch.equal(got, (exact * 2.0 ** (ea + eb - 254)).float().to(dtype)), (ea, eb, dtype)
+    a, b = matrix(va, 127, m), matrix(vb, 127, rows_b)
+    a.scales.view(torch.uint8)[m // 2, kb - 1] = 255
+    b.scales.view(torch.uint8)[rows_b - 1, 0] = 255
+    last = slice(n - 1, n) if form == "rows" else slice((rows_b - 1) * 128, n)
+    for scales in ("e8m0", "fp32"):
+        if scales == "fp32":
+            a, b = (amd.BlockScaled(q.values, q.scales.float()) for q in (a, b))
+        for dtype in (torch.float32, torch.float16):
+            want = exact.float().clone()
+            want[m // 2], want[:, last] = float("nan"), float("nan")
+            got = amd.block_product(a, b, alpha=2.0 ** -8, out_dtype=dtype, check_finite=False)
+            assert torch.equal(got.nan_to_num(7.0), (want * 2.0 ** -8).to(dtype).nan_to_num(7.0)), (scales, dtype)
+
+
+def test_a_layer_trained_as_the_readme_shows():
+    """The calls of README.md: a layer, its gradients, the weight's straight into the gradient arena, and the step; captured and replayed as they stand."""
+    import sd_mecha_amd as amd
+    from sd_mecha_amd.arena import plan_arena
+    out_f, in_f, tokens = 640, 320, 77
+    layout = plan_arena([("w", out_f * in_f), ("b", out_f)])
+    segments = layout.device_segments("cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, g = torch.randn(tokens, in_f, device="cuda", generator=gen).bfloat16(), torch.randn(tokens, out_f, device="cuda", generator=gen).bfloat16()
+    start = torch.randn(layout.total_elems, device="cuda", generator=gen) * 0.02
+
+    def program():
+        params, grads, t = start.clone(), torch.zeros_like(start), torch.zeros(1, dtype=torch.int64, device="cuda")
+        w, w_grad = params[:out_f * in_f].view(out_f, in_f), grads[:out_f * in_f].view(out_f, in_f)
+        state = amd.adamw_state(layout, "cuda", bits=8)
+
+        def step():
+            t.add_(1)
+            w8, wt8 = amd.cast_blocks(w, tile=True, sides="both", check_finite=False)
+            (x8, xt8), (g8, gt8) = amd.cast_blocks(x, sides="both", check_finite=False), amd.cast_blocks(g, sides="both", check_finite=False)
+            y = amd.block_product(x8, w8, out_dtype=torch.bfloat16, check_finite=False)
+            dx = amd.block_product(g8, wt8, out_dtype=torch.bfloat16, check_finite=False)
+            amd.block_product(gt8, xt8, out=w_grad, check_finite=False)
+            norm = amd.adamw_step(params, grads, **state, segments=segments, step=t, lr=1e-4, max_norm=1.0)
+            return [y, dx, norm, params, grads, *state.values()]
+        return step
+    eager, captured = program(), program()
+    captured()                                                     # (the first step warms up)
+    graph, first = torch.cuda.CUDAGraph(), eager()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = captured()
+    for _ in range(4):
+        want = [v.clone() for v in eager()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o.view(-1).view(torch.uint8), v.view(-1).view(torch.uint8)) for o, v in zip(outs, want))
+    assert bool((first[3] != start)[:out_f * in_f].any())
