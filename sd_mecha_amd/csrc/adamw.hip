@@ -242,7 +242,11 @@ __global__ __launch_bounds__(MECHA_BLOCK) void adamw_kernel(AdamParams a) {
         root[j] = root_of(v[j]);
         const float den = __builtin_fmaf(root[j], root_size, a.eps);
         p[j] = __builtin_fmaf(m[j] * __builtin_amdgcn_rcpf(den), -size, p[j] * keep);
-        if (a.seg_flags && j < valid) bad_out |= !(fabsf(p[j]) < a.over) || !(v[j] < INFINITY);
+    }
+    if (a.seg_flags) {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (j < valid) bad_out |= !(fabsf(p[j]) < a.over) || !(root[j] < INFINITY);
     }
     if (valid) {
         store(std::integral_constant<int, P_DT>{}, a.p, p);
