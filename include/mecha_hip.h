@@ -481,7 +481,7 @@ int mecha_uncast_blocks(const mecha_block_matrix *q, void *out, int out_dtype, u
  * float32 numbers; float32 scales: a block's sum is multiplied by b's and then by a's, so those of b should lie from 2^-108 to 2^103 or be 0;
  * powers of two with a float32 result: values under 2^-123 may be rounded to a multiple of 2^-133.  bit 0 of flags: a NaN came out
  * or base holds inf / NaN; bit 1: an output is inf / NaN.  out shares no memory with a, b or (but for out == base) base,
- * and the workspace none with any of them. */
+ * and the workspace none with any of them.  Rows of codes lie at most 2^24 bytes apart. */
 int mecha_block_product(const mecha_block_matrix *a, const mecha_block_matrix *b, const void *base, int base_dtype, void *out, int out_dtype,
                         float alpha, uint32_t *flags, void *workspace, size_t workspace_bytes, void *stream);
 /* What a product of m x n results over k can use (0 for most): float32 sums of parts of k, for results too few to fill the chip.  With

@@ -134,7 +134,8 @@ def cast_blocks(a, *, tile: bool = False, sides: str = "straight", key=None, fla
     smallest 2^e with ``max|x| <= 448 * 2^e`` over the block, codes to nearest even.  ``tile``: a scale for a 128 x 128 square,
     else for 128 columns of a row.  ``sides``: ``"straight"`` the matrix, ``"transposed"`` its transpose (without ``tile`` that has scales of
     its own, for 128 original rows of a column), ``"both"`` the pair of them from one pass over the key.
-    Non-finite elements raise ``NonFiniteStateDictKeyError`` (``check_finite``) or set bit 0 of ``flags``, and become NaN codes."""
+    Non-finite elements raise ``NonFiniteStateDictKeyError`` (``check_finite``, which waits for the kernel: not in a captured graph) or set bit 0 of
+    ``flags``, and become NaN codes."""
     a = _resolve(a, key)
     if sides not in SIDES:
         raise ValueError(f"cast_blocks: sides is one of {SIDES}, got {sides!r}")
@@ -193,13 +194,13 @@ def block_product(a: BlockScaled, b: BlockScaled, base: Optional[torch.Tensor] =
                   key=None, out_dtype=None, flags=None, check_finite: bool = True) -> torch.Tensor:
     """``base + alpha * a @ b.T`` (``base=None``: ``alpha * a @ b.T``) of two 8-bit matrices a [m, k], b [n, k], summed in float32 and rounded once to
     ``out_dtype`` (default float32; for 16-bit results the 8-bit matrix instructions first cut the products of 8 neighbouring k off under
-    2^-13 of the largest, 1.5e-5 of a typical result) -- add_difference(base, product, alpha).  ``base``: m * n elements; the result has its shape.  ``out``: where
+    2^-13 of the largest, 1.5e-5 of a typical result: about 1 % of bfloat16 results are the neighbour of the nearest number) -- add_difference(base, product, alpha).  ``base``: m * n elements; the result has its shape.  ``out``: where
     the result goes (contiguous, m * n elements, of the result's dtype); it may be ``base`` itself, and otherwise shares no memory with an input.
 
     A linear layer ``y = x @ w.T`` with w cast with ``tile=True, sides="both"`` to (w, wt), x and the output gradient g cast to (x, xt) and
     (g, gt): y = block_product(x, w), the input's gradient block_product(g, wt), the weight's block_product(gt, xt).
     A NaN result or a non-finite base raises ``NonFiniteStateDictKeyError`` (``check_finite``) or sets bit 0 of ``flags``; a result that its type
-    stores as infinity sets bit 1."""
+    stores as infinity sets bit 1.  The check waits for the kernel (18 us a call): ``check_finite=False`` in a step that is captured or repeated."""
     _check_blocks(a, "block_product")
     _check_blocks(b, "block_product")
     m, k, n, kb, device = a._rows, a._cols, b._rows, b._cols, a._values.device

@@ -5,8 +5,8 @@
 // in float32, whatever the storage types.
 //
 // HBM-bound: 28 bytes an element with float32 throughout, 10 with 16-bit weights and gradients and 8-bit states: 174 M float32 elements with
-// bfloat16 gradients and a bfloat16 copy 810 us (6.0 TB/s, what a flat copy reaches is 6.2), 348 M bfloat16 ones with 8-bit states 675 us (5.2
-// TB/s; 59 vector instructions an element take 78 % of that time, the conversions' hashes most of them).  One vector a
+// bfloat16 gradients and a bfloat16 copy 810 us (6.0 TB/s, what a flat copy reaches is 6.2), 348 M bfloat16 ones with 8-bit states 605 to 690 us
+// (5.1 to 5.8 TB/s, by the weights' and states' values; 59 vector instructions an element take four fifths of it, the conversions' hashes most of them).  One vector a
 // thread on a flat grid, 4 elements with float32 states and 8 with 8-bit ones; a vector lies in one key (offsets are multiples of
 // 8), its key is found by a search over the segment table that a wave does once, behind the loads.
 //
@@ -111,8 +111,9 @@ __device__ __forceinline__ void store_n(void *base, int64_t i, const float (&v)[
     }
 }
 
-// The square root to one unit in the last place, v_sqrt_f32's own error: float32's rounded root takes ten instructions more, and the code
-// or the weight that comes of it moves by far less than its rounding.  Under 2^-96 (where the instruction would take subnormals
+// The square root to one unit in the last place, v_sqrt_f32's own error, and the reciprocal below likewise: with the rounded root and division 348 M
+// elements with 8-bit states take 685 us, 625 without, and what comes of them is no nearer to float64: 4.75e-7 of the roots' codes are another's
+// than float64 would take here, 4.89e-7 there; weights are off by 3.88e-8 either way.  Under 2^-96 (where the instruction would take subnormals
 // for zeros) the root of 2^64 v.
 __device__ __forceinline__ float root_of(float v) {
     const bool small = v < 1.262177448e-29f;

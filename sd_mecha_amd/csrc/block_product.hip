@@ -13,9 +13,10 @@ namespace {
 //
 // What the 8-bit matrix instructions lose (all of them; measured with single products): the products of 8 neighbouring k are aligned to
 // the largest, and what lies under 2^-13 of it is cut off; the groups are then added in float32.  That is 1.5e-5 of a result (2-norm, normal
-// codes), 1/14 of what rounding to float16 loses and 1/110 of bfloat16's, so results of 16 bits are made this way.  A float32 result
-// would show it: there the codes are turned into bfloat16, which holds each exactly, and multiplied on v_mfma_f32_16x16x32_bf16, which
-// adds in float32 (1e-8 to 5e-8 measured) at half the rate.
+// codes), 1/14 of what rounding to float16 loses and 1/110 of bfloat16's, so results of 16 bits are made this way: about 1 % of bfloat16
+// results are the neighbour of the nearest number, and the error after the rounding is the rounding's (1.658e-3 at 8192 x 10240 x 1280, either
+// way).  A float32 result would show it: there the codes are turned into bfloat16, which holds each exactly, and multiplied on
+// v_mfma_f32_16x16x32_bf16, which adds in float32 (7e-8 to 1.2e-7 measured) at half the rate.
 //
 // b's rows are the instruction's A operand (accumulator rows) and a's rows its B operand (accumulator columns): lane l holds 4
 // accumulators of output row m = l % 16.  b's rows are dealt to the fragments so that a lane's accumulators of 2 fragments are 8
@@ -556,11 +557,11 @@ int launch_direct(int shape, const ProductParams &p, hipStream_t s) {
 // Workgroups go round the 8 XCDs, each with its own L2: an XCD gets a run of tiles, ordered so that the 32 at work at a time are 8 x 4
 // tiles (2 MiB of a and 1 MiB of b at k = 1024, MI = 8).
 //
-// Measured (no base): 8192 x 8192 x 8192 457 us (2.4 PFLOP/s; the matrix unit's own rate is 4.3, and a plain per-tensor library product takes 421);
-// 8192 x 10240 x 1280 100 us (2.15 PFLOP/s with 168 MB of results; the library 108); 8269 x 1280 x 5120 58 us (float32 scales: 64).  A
+// Measured (no base): 8192 x 8192 x 8192 426 to 454 us (2.4 to 2.6 PFLOP/s; the matrix unit's own rate is 4.3, and a plain per-tensor library product
+// takes 428); 8192 x 10240 x 1280 100 to 112 us (2.0 PFLOP/s with 168 MB of results; the library 108); 8269 x 1280 x 5120 58 us (float32 scales: 64).  A
 // 256 x 256 step takes 3900 cycles: 2048 of products at the unit's rate, and 1600 in which its 64 KiB come from L2 to LDS, which overlap
 // only in part: fewer or more of them asked for at a step's start, by four waves or by eight, made no difference.  Float32 results
-// multiply at bfloat16's rate (2.1 PFLOP/s): 1280 x 5120 x 8269 102 us (1.06 PFLOP/s on 200 of the 256 CUs).
+// multiply at bfloat16's rate (2.1 PFLOP/s): 1280 x 5120 x 8269 109 us (0.99 PFLOP/s on 200 of the 256 CUs).
 constexpr int BIG_N = 256, BIG_M = 256, BIG_THREADS = 512, BIG_CH = 4, BIG_CUS = 256, BIG_BAND = 8;
 struct BigLds {
     uint8_t stage[2][2][BIG_M * 128];             // [stage][a, b][row][128]
@@ -606,8 +607,8 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
     if (tile >= run1) return;
     // Tiles of one size end at one time, and all CUs' results together are bound by memory (5.4 us a round of 256 x 256 16-bit ones) while the matrix
     // units wait.  Where workgroups have several tiles, half of an XCD's -- those that have the fewer, if any do -- begin about half a round's stores
-    // later (64 cycles a unit), and one half stores while the other multiplies: 8192 x 10240 x 1280 110 -> 105 us, 16384 x 5120 x 640 68 -> 61,
-    // 4096 x 8192 x 512 31 -> 26.  More groups (4, 8, 32) gain less.
+    // later (64 cycles a unit), and one half stores while the other multiplies: 8192 x 10240 x 1280 112 us, 116 without, 16384 x 5120 x 640 64 and 67,
+    // 4096 x 8192 x 512 28 and 33.  More groups (4, 8, 32) gain less.
     if (run1 - run0 > per_xcd && (blockIdx.x >> 3) >= per_xcd / 2) {
         constexpr int UNITS = ROWS * (OUT == MECHA_F32 ? 4 : 2) / 4;
         for (int i = 0; i < UNITS; i += 16) __builtin_amdgcn_s_sleep(16);
@@ -737,7 +738,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             return;
         }
         // 16-byte pieces of two rows change places between two lanes, so that 8 lanes store a row's 128 bytes with one instruction;
-        // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280: 121 -> 103 us).
+        // base comes in the same way.  Non-temporal: whole lines, touched once (8192 x 10240 x 1280 112 us, 130 through the caches).
         constexpr int EACH = EXACT ? 4 : 8, ESIZE = EXACT ? 4 : 2;        // elements of a piece, bytes of one
         const bool odd = lane & 1;
         const int64_t row0 = (int64_t)here.m0 + wm + (r & ~1), line = p.ld * ESIZE;
@@ -758,7 +759,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
             else store_part(to, v, ESIZE * left);
         };
         float poison_in = 0.0f, top = 0.0f;
-        // base comes AHEAD fragments before it is added (8192 x 10240 x 1280 with a base 139 -> 134 us; float32 results have no registers for it)
+        // base comes AHEAD fragments before it is added (8192 x 10240 x 1280 with a base 146 us, 153 with one; float32 results have no registers for it)
         constexpr int PAIRS = EXACT ? 2 : 1, AHEAD = EXACT ? 1 : 2;
         u32x4 pre[AHEAD][PAIRS][2];
         auto ask = [&](int i, int64_t from) {
@@ -835,7 +836,7 @@ __global__ __launch_bounds__(BIG_THREADS, 2) void product_big_kernel(ProductPara
         // fragment's of a, and, while the last one is multiplied, the next step's of b, each in the place of the quarter that was used last (the last
         // quarter's in the next step).  Behind the second fragment all that is left of this stage is in registers: there the waves meet, the step
         // after the next is asked for into this one's place, and the next step's codes are read.  A wave that is in its last fragment goes first, which
-        // keeps the two waves of a SIMD apart: 1280 x 5120 x 8269 102 us, 110 without.
+        // keeps the two waves of a SIMD apart: 1280 x 5120 x 8269 110 us, 116 without.
         static_assert(MI == 4, "fragments");
         i32x8 fa[2], raw[4];
         uint32_t sa[2], rawscale[4];
@@ -1223,15 +1224,15 @@ int launch_big(int mi, const ProductParams &p, void *workspace, hipStream_t s) {
 
 // ---------------------------------------------------------------------------------------------------- which kernel
 // The time each would take, in microseconds, from what it measured on 256 CUs (138 random products up to 16384 x 10240 x 8192 of all four kinds, each
-// with every kernel: the choice is 2 to 3 % over the best in the mean):
+// with every kernel: the choice is 2 % over the best in the mean, 35 % at worst):
 //   direct: a launch, the join of a workgroup's waves, and the slower of one workgroup's reads (33 KB a us) and all workgroups' (5 TB/s, 1 ns and their
-//           joins): 53 x 4077 x 659 4.9 us with 32 x 32 outputs a workgroup, 6.0 with 32 x 64;
+//           joins): 600 x 1280 x 1280 (float32 scales and results) 17 us with 32 x 32 outputs a workgroup, 22 in 128 x 128 tiles;
 //   tiled:  rounds of tiles over the CUs, each n_kb steps and an epilogue.  128 x 128 tiles (two workgroups a CU) fill a few CUs more evenly:
-//           1024 x 1280 x 5120 36 us, 49 with 128 x 256 tiles; the larger ones share more: 8192 x 1280 x 5120 57 us (192 x 256), 80 with
-//           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 82 (128 x 256).
+//           1024 x 1280 x 5120 38 us, 50 with 128 x 256 tiles; the larger ones share more: 8192 x 1280 x 5120 59 us (192 x 256), 84 with
+//           128 x 128; 16384 x 5120 x 640 63 us (256 x 256), 79 (128 x 256).
 //   in parts: results of fewer 128 x 256 tiles than CUs, k shared out among 2 to 32 workgroups a tile (4 blocks at least each): the parts are written
-//           and read once as float32 and joined by a second launch: 1280 x 1280 x 8269 32 us in 5 parts (55 in one; float32 results 39 and 100),
-//           1024 x 1280 x 5120 25 (36), 300 x 2560 x 8192 24 (53); 320 x 320 x 8269 stays with the direct kernel: 15 us, 16 in 13 parts.
+//           and read once as float32 and joined by a second launch: 1280 x 1280 x 8269 34 us in 5 parts (58 in 128 x 128 tiles; float32 results 41 and 80),
+//           1024 x 1280 x 5120 27 (38), 300 x 2560 x 8192 26 (55).
 constexpr int MAX_SPLITS = 32;
 int mode_of(int scale_dtype, int out_dtype) {
     const bool e8m0 = scale_dtype == MECHA_SCALE_E8M0;
@@ -1243,7 +1244,7 @@ constexpr int DIRECT_ROWS[4] = {16, 16, 32, 32}, DIRECT_COLS[4] = {16, 32, 32, 6
 struct Choice { int direct = -1, mi = 0, splits = 1; };        // shape of the direct kernel; else MI of the large one; else the 128 x 128 one
 Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_ok, bool split_ok) {
     // a step of 128 x 128, MI = 4, 6, 8: power-of-two scales; float32 scales with one of b's in a square; with one in every row of b, where MI = 8
-    // has no registers for them (8192 x 8192 x 2048: 267 us, 186 with MI = 6); float32 results
+    // has no registers for them (8192 x 8192 x 2048: 264 us, 194 with MI = 6); float32 results
     static const double step[4][4] = {{0.75, 1.20, 1.36, 1.56}, {1.18, 1.34, 1.54, 1.81}, {1.18, 1.51, 1.78, 0.0}, {1.42, 1.60, 0.0, 0.0}};
     const double *us = step[mode == HW_SCALES ? 0 : mode != F32_SCALES ? 3 : b_tile ? 1 : 2];
     const double n_kb = (double)((k + SCALE_BLOCK - 1) / SCALE_BLOCK);
@@ -1263,7 +1264,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int mode, int b_tile, bool large_
         }
     }
     const int *const rows = DIRECT_ROWS, *const cols = DIRECT_COLS;
-    for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 32 us, 16 without it)
+    for (int d = 0; d < (mode == EXACT_F32 ? 3 : 4); d++) {     // (float32 scales, float32 results: the last shape's registers spill, 600 x 1280 x 1280 34 us, 17 with 32 x 32)
         const double blocks = up(m, rows[d]) * up(n, cols[d]), bytes = (rows[d] + cols[d]) * n_kb * SCALE_BLOCK, one = bytes / 33e3, all = blocks * (bytes / 5e6 + 0.001 + 2e-6 * rows[d] * cols[d]);
         const double t = 2.5 + 0.001 * rows[d] * cols[d] + (one > all ? one : all);
         if (t < best && blocks * DIRECT_THREADS < 4294967296.0) { best = t; c.mi = 0; c.splits = 1; c.direct = d; }     // a launch's threads

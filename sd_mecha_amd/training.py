@@ -58,7 +58,8 @@ def adamw_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor,
     their ``_scales``, e4m3 codes of m and of sqrt(v) with a power of two for every 128 elements.
     8-bit codes are rounded up or down by a hash of (offset, step, ``seed``), so that slow means move on average.
 
-    ``step`` counts from 1: an int, or an int64 tensor on the device that the kernel reads (for captured graphs).  ``weight_decay``: a
+    ``step`` counts from 1: an int, or an int64 tensor on the device that the kernel reads (for captured graphs).  ``lr``, ``betas``, ``eps`` and ``max_norm``
+    are numbers of the host: a captured step keeps the ones it was captured with, so a schedule captures again.  ``weight_decay``: a
     number, or float32 [keys] on the device, one per key.  ``copy``: an arena that receives the new weights in its own dtype.
     ``max_norm``: the gradients of all keys together are scaled down to this 2-norm first, and the norm is returned ([1], on the device);
     if it is not finite, the step sets flags and changes nothing else.  The arenas share no memory.  ``flags``: int32 [keys], per-key flag words (bit 0: a gradient or weight is
