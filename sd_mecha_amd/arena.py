@@ -32,7 +32,7 @@ class ArenaLayout:
 
     def device_segments(self, device) -> torch.Tensor:
         """The same table as an int64 [n, 2] DEVICE tensor (layout-compatible with mecha_segment[])."""
-        t = torch.tensor([[o, n] for o, n in zip(self.offsets, self.numels)], dtype=torch.int64)
+        t = torch.tensor([[o, n] for o, n in zip(self.offsets, self.numels)], dtype=torch.int64).view(-1, 2)
         return t.to(device)
 
 

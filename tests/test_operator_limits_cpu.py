@@ -127,3 +127,15 @@ def test_the_shapes_of_the_product_tests_take_every_kernel():
                                 {(32, 64, False), (192, 256, False)}, {(32, 64, False)}, set())):
         assert got == few | more
     assert L.mecha_block_product_tile(0, 8, 8, 1, 0, 0, 0) == 0
+
+
+def test_the_segment_table_of_a_layout_without_keys():
+    """Every key frozen or empty: a table of no rows, which a step takes and does nothing with."""
+    import sd_mecha_amd as amd
+    from sd_mecha_amd.arena import plan_arena
+    layout = plan_arena([("a", 0)])
+    segments = layout.device_segments("cpu")
+    assert segments.shape == (0, 2) and segments.dtype == torch.int64
+    p = torch.zeros(layout.total_elems)
+    with pytest.raises(RuntimeError, match="no CPU path"):                 # all else is in order
+        amd.adamw_step(p, p.clone(), segments=segments, step=1, **amd.adamw_state(layout, "cpu"))
